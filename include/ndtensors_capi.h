@@ -438,6 +438,78 @@ int ndt_b200_contract_f64_noalloc(const double* a, const size_t* shape_a, size_t
                                   const double* b, const size_t* shape_b, size_t ndim_b, const long* labels_b,
                                   double* c, size_t c_len, size_t* out_shape, size_t* out_ndim, void* stream);
 
+/* ---- Language-model operators on device memory (no counterpart in the
+ * reference).  Row-major matrices of the current device, element types by the
+ * codes below, a cudaStream_t as `stream` (NULL: the legacy default stream).
+ * Asynchronous; workspaces come from the stream-ordered pool.  Sizes of zero
+ * are allowed where no result is then left undefined.  Status codes as
+ * elsewhere: bad arguments NDT_INVALID_ARGUMENT, sizes that do not fit
+ * NDT_SHAPE_MISMATCH, CUDA failures NDT_INTERNAL_ERROR, the text in
+ * ndt_b200_last_error. */
+#define NDT_F32 2
+#define NDT_BF16 3
+#define NDT_F16 4
+#define NDT_E4M3 5
+#define NDT_E5M2 6
+
+/* 8-bit block quantisation of x [rows, cols] (NDT_F32 / BF16 / F16, any
+ * strides).  Blocks of block_rows (1 or 128) x 128 elements, cut at the edge:
+ *   amax = max(2^-100, largest finite |x|),  scale = amax / F  (F: 448 e4m3,
+ *   57344 e5m2),  q = x / scale rounded to 32 bits, then to 8 (ties to even).
+ * NaN stays NaN; an infinity becomes e5m2's, or NaN in e4m3.
+ * q [rows, cols] with leading dimension ldq, scale of (block row, block
+ * column) at scales[br * scale_row_stride + bc * scale_col_stride].  qt: the
+ * same of x transposed ([cols, rows], blocks of block_rows x 128 of it), from
+ * the same pass over x.  Either of q and qt may be NULL.  ldq / ldqt:
+ * multiples of 16 that cover a row, bases 16-byte aligned; bytes between the
+ * row's end and the next multiple of 16 may be overwritten. */
+int ndt_b200_quantize_dev(int x_type, const void* x, long rows, long cols, long row_stride, long col_stride,
+                          int block_rows, int q_type, void* q, long ldq, float* scales, long scale_row_stride,
+                          long scale_col_stride, void* qt, long ldqt, float* scales_t, long scale_t_row_stride,
+                          long scale_t_col_stride, void* stream);
+/* c [m, n] (+)= sum over blocks of 128 along k of
+ *   a_scale(i, kb) * b_scale(j, kb) * sum_k a[i, k] * b[j, k]
+ * for 8-bit a [m, k], b [n, k] (e4m3 or e5m2 each) whose scales are for 1 or
+ * 128 rows; sums in 32 bits, c rounded once.  Operands with unit column
+ * stride, 16-byte aligned bases and row strides that are multiples of 16 are
+ * read in place, others are copied to a workspace first. */
+int ndt_b200_scaled_gemm_dev(long m, long n, long k, int a_type, const void* a, long a_row_stride, long a_col_stride,
+                             int a_block_rows, const float* a_scales, long a_scale_row_stride, long a_scale_col_stride,
+                             int b_type, const void* b, long b_row_stride, long b_col_stride, int b_block_rows,
+                             const float* b_scales, long b_scale_row_stride, long b_scale_col_stride, int c_type,
+                             void* c, long ldc, int accumulate, void* stream);
+/* y [tokens, n] = x [tokens, k] w^T with x quantised (e4m3, blocks of 1 x 128)
+ * in the call and stored 8-bit w [n, k] with scales of 128 x 128 blocks. */
+int ndt_b200_scaled_linear_dev(int x_type, const void* x, long tokens, long k, long x_row_stride, long x_col_stride,
+                               int w_type, const void* w, long n, long w_row_stride, long w_col_stride,
+                               const float* w_scales, long w_scale_row_stride, long w_scale_col_stride, int y_type,
+                               void* y, long ldy, void* stream);
+/* out[i, :] = scale * table[ids[i] - first, :] for n ids (int32, or int64 with
+ * ids64), rounded once; zeros where the id names no row (a table that holds a
+ * slice of the vocabulary passes its first id). */
+int ndt_b200_embedding_dev(int type, const void* table, long rows, long dim, long ld, const void* ids, int ids64, long n,
+                           long first, float scale, void* out, long ldo, void* stream);
+/* out [rows, dim]: out[v, :] (+)= scale * sum over i with ids[i] - first == v
+ * of grad[i, :], summed in 32 bits in one order (the result is the same in
+ * every call).  accumulate = 0 writes every row, zeros without an id. */
+int ndt_b200_embedding_grad_dev(int grad_type, const void* grad, long ldg, const void* ids, int ids64, long n, long rows,
+                                long dim, long first, float scale, int out_type, void* out, long ldo, int accumulate,
+                                void* stream);
+/* A mixture-of-experts layer for a few tokens: x [tokens, h] (bf16 / f16),
+ * router [experts, h], w_in [experts, 2 i, h] (gate rows, then up rows), w_out
+ * [experts, h, i].  The `top` experts of a token are those of the largest
+ * router products (ties to the lowest index), their weights exp(l) / sum
+ * exp(l) over all experts, or over the chosen with renormalize;
+ *   y = sum of weight * w_out (silu(gate) * up).
+ * Weights have x's type, or are e4m3 with the scales of their 128 x 128 blocks
+ * (in_scales [experts, ceil(2 i / 128), ceil(h / 128)], out_scales [experts,
+ * ceil(h / 128), ceil(i / 128)]).  ids, weights [tokens, top] receive the
+ * choice.  At most 1024 experts. */
+int ndt_b200_expert_layer_dev(int x_type, const void* x, long tokens, long h, long ldx, const void* router, long experts,
+                              int w_type, const void* w_in, const float* in_scales, const void* w_out,
+                              const float* out_scales, long i, long top, int renormalize, void* y, long ldy, int* ids,
+                              float* weights, void* stream);
+
 /* Library control and diagnostics */
 int ndt_b200_device_available(void);
 int ndt_b200_set_stream(void* stream); /* NULL restores the library's own stream */

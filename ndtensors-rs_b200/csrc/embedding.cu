@@ -1,0 +1,431 @@
+// Embedding lookup with scaling, and the gradient of the table.
+//
+//   out[i, :]    = scale * table[ids[i] - first, :]      (zero outside the table)
+//   dtable[v, :] = scale * sum over i with ids[i] - first == v of grad[i, :]
+//
+// Both are bound by memory.  The sum has to have one order, so that a step
+// gives the same gradient twice: the ids are sorted by (row, position), then
+// tiles of kEntries sorted entries are summed in 32 bits in that order.  A
+// row whose entries cross tiles leaves a part in each, and a last kernel adds
+// the parts in tile order.  Tiles of entries, not of rows, keep the work even
+// when a few ids make up most of a batch.
+//
+// The sort is one kernel without communication: every CTA owns a range of
+// rows, counts over all ids how many lie below its range (its offset in the
+// sorted list) and places its own, stably.  It writes the zeros of its rows
+// that no id names as well, so the dense result is written once.
+#include <algorithm>
+
+#include "model_ops.h"
+
+namespace ndt {
+namespace {
+
+constexpr int kSortThreads = 1024;
+constexpr int kPerThread = 4;                      // ids a thread takes in turn
+constexpr int kList = kSortThreads * kPerThread + kSortThreads;  // compacted ids of a range
+constexpr int kEntries = 32;                       // sorted entries a tile
+constexpr int kSumThreads = 256;
+
+// The table's row of id i; at least 2^63 for an id below the table's first.
+template <bool IDS64>
+__device__ __forceinline__ uint64_t row_at(const void* ids, int64_t i, int64_t first) {
+  return (uint64_t)(IDS64 ? ((const int64_t*)ids)[i] : (int64_t)((const int*)ids)[i]) - (uint64_t)first;
+}
+
+// ---------------------------------------------------------------- lookup
+// A warp takes one row (or one of `parts` pieces of it), four 16-byte vectors
+// a lane at a time.
+template <typename T, bool IDS64, bool VEC>
+__global__ void __launch_bounds__(256) lookup_kernel(const T* __restrict__ table, int64_t v, int64_t d, int64_t ldt,
+                                                     const void* __restrict__ ids, int64_t n, int64_t first, float scale,
+                                                     T* __restrict__ out, int64_t ldo, int parts) {
+  pdl_release();
+  pdl_wait();
+  constexpr int kN = VEC ? 16 / sizeof(T) : 1;
+  const int lane = threadIdx.x & 31;
+  const int64_t w = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) >> 5;
+  const int64_t i = w / parts;
+  if (i >= n) return;
+  const int64_t vecs = d / kN, per = (vecs + parts - 1) / parts;
+  const int64_t c0 = (w - i * parts) * per, c1 = min(vecs, c0 + per);
+  const uint64_t row = row_at<IDS64>(ids, i, first);
+  const bool in = row < (uint64_t)v;
+  const T* src = table + (in ? row : 0) * ldt;
+  T* dst = out + i * ldo;
+  if constexpr (VEC) {
+    for (int64_t c = c0 + lane; c < c1; c += 128) {
+      uint4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        x[j] = in && c + 32 * j < c1 ? __ldg(reinterpret_cast<const uint4*>(src) + c + 32 * j) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (c + 32 * j >= c1) break;
+        T* e = reinterpret_cast<T*>(&x[j]);
+#pragma unroll
+        for (int q = 0; q < kN; q++) e[q] = from_f32<T>(in ? to_f32<T>(e[q]) * scale : 0.f);
+        reinterpret_cast<uint4*>(dst)[c + 32 * j] = x[j];
+      }
+    }
+  } else {
+    for (int64_t c = c0 + lane; c < c1; c += 32) dst[c] = from_f32<T>(in ? to_f32<T>(src[c]) * scale : 0.f);
+  }
+}
+
+// ------------------------------------------------------------------ sort
+__device__ __forceinline__ int block_exclusive_scan(int v, int* warp_sums, int* total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(~0u, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int s = warp_sums[lane], t = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(~0u, t, o);
+      if (lane >= o) t += y;
+    }
+    warp_sums[lane] = t - s;
+    if (lane == 31) *total = t;
+  }
+  __syncthreads();
+  const int r = warp_sums[warp] + x - v;
+  const int tot = *total;
+  __syncthreads();
+  v = r;
+  *total = tot;
+  return v;
+}
+
+struct SortArgs {
+  const void* ids;
+  int64_t n, first, v, range;  // range: rows of one CTA
+  int* order;                  // sorted positions
+  int* rows;                   // their rows
+  int* count;                  // how many ids are in the table
+  void* out;                   // zeros go to the rows without an id; null: nowhere
+  int64_t d_bytes, ld_bytes;
+};
+
+template <bool IDS64>
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortArgs a) {
+  extern __shared__ int sm[];
+  int* start = sm;                  // [range] counts, then where the next id of a row goes
+  int* list_key = sm + a.range;     // [kList]
+  int* list_pos = list_key + kList;
+  __shared__ int warp_sums[32];
+  __shared__ int total, list_n;
+  __shared__ int below_s;
+  pdl_release();
+  pdl_wait();
+  const uint64_t v0 = blockIdx.x * (uint64_t)a.range, v1 = min((uint64_t)a.v, v0 + a.range);
+  const int rows = (int)(v1 - v0);
+  for (int i = threadIdx.x; i < a.range; i += kSortThreads) start[i] = 0;
+  if (threadIdx.x == 0) below_s = 0, list_n = 0;
+  __syncthreads();
+  int below = 0;
+  for (int64_t i = threadIdx.x; i < a.n; i += kSortThreads) {
+    const uint64_t r = row_at<IDS64>(a.ids, i, a.first);
+    if (r < v0) below++;
+    if (r >= v0 && r < v1) atomicAdd(&start[r - v0], 1);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) below += __shfl_xor_sync(~0u, below, o);
+  if ((threadIdx.x & 31) == 0 && below) atomicAdd(&below_s, below);
+  __syncthreads();
+  // the zeros of rows without an id
+  if (a.out) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const bool vec = a.d_bytes % 16 == 0 && a.ld_bytes % 16 == 0 && (uintptr_t)a.out % 16 == 0;
+    for (int r = warp; r < rows; r += kSortThreads / 32) {
+      if (start[r]) continue;
+      unsigned char* p = (unsigned char*)a.out + (v0 + r) * a.ld_bytes;
+      if (vec)
+        for (int64_t c = lane * 16; c < a.d_bytes; c += 512) *reinterpret_cast<uint4*>(p + c) = make_uint4(0, 0, 0, 0);
+      else
+        for (int64_t c = lane * 2; c < a.d_bytes; c += 64) *reinterpret_cast<uint16_t*>(p + c) = 0;
+    }
+  }
+  __syncthreads();
+  // counts -> first places
+  int base = below_s;
+  for (int64_t i0 = 0; i0 < a.range; i0 += kSortThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    const int c = i < a.range ? start[i] : 0;
+    const int before = block_exclusive_scan(c, warp_sums, &total);
+    if (i < a.range) start[i] = base + before;
+    base += total;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0 && v1 == (uint64_t)a.v) *a.count = base;
+  if (base == below_s) return;  // no id in this range
+  // ids of the range, compacted in order of position, then placed
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto place = [&](int upto) {  // whole list: batches of one entry a thread
+    for (int b = 0; b < upto; b += kSortThreads) {
+      const int m = min(kSortThreads, upto - b);
+      const bool on = (int)threadIdx.x < m;
+      const int key = on ? list_key[b + threadIdx.x] : -1;
+      const unsigned same = __match_any_sync(~0u, key);
+      const int rank = __popc(same & ((1u << lane) - 1)), leader = __ffs(same) - 1;
+      for (int w = 0; w * 32 < m; w++) {
+        if (warp == w) {
+          int at = 0;
+          if (on && lane == leader) {
+            at = start[key];
+            start[key] = at + __popc(same);
+          }
+          at = __shfl_sync(~0u, at, leader) + rank;
+          if (on) {
+            a.order[at] = list_pos[b + threadIdx.x];
+            a.rows[at] = (int)(v0 + key);
+          }
+        }
+        __syncthreads();
+      }
+    }
+  };
+  for (int64_t i0 = 0; i0 < a.n; i0 += kSortThreads * kPerThread) {
+    int key[kPerThread], mine = 0;
+#pragma unroll
+    for (int j = 0; j < kPerThread; j++) {
+      const int64_t i = i0 + threadIdx.x * kPerThread + j;
+      const uint64_t r = i < a.n ? row_at<IDS64>(a.ids, i, a.first) : ~0ull;
+      key[j] = r >= v0 && r < v1 ? (int)(r - v0) : -1;
+      mine += key[j] >= 0;
+    }
+    int at = list_n + block_exclusive_scan(mine, warp_sums, &total);
+#pragma unroll
+    for (int j = 0; j < kPerThread; j++)
+      if (key[j] >= 0) {
+        list_key[at] = key[j];
+        list_pos[at++] = (int)(i0 + threadIdx.x * kPerThread + j);
+      }
+    const int have = list_n + total;
+    __syncthreads();
+    if (have > kSortThreads || i0 + kSortThreads * kPerThread >= a.n) {
+      place(have);
+      if (threadIdx.x == 0) list_n = 0;
+    } else if (threadIdx.x == 0) {
+      list_n = have;
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------- sum
+template <typename T>
+__device__ __forceinline__ void add_vec(const T* p, float* acc, int n, bool vec) {
+  constexpr int kN = 16 / sizeof(T);
+  if (vec) {
+    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+    const T* e = reinterpret_cast<const T*>(&x);
+#pragma unroll
+    for (int q = 0; q < kN; q++) acc[q] += to_f32<T>(e[q]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < kN; q++)
+      if (q < n) acc[q] += to_f32<T>(p[q]);
+  }
+}
+__device__ __forceinline__ void put(void* out, int64_t i, MType t, float v, bool add) {
+  if (t == MType::F32) {
+    float* p = (float*)out + i;
+    *p = add ? *p + v : v;
+  } else if (t == MType::BF16) {
+    __nv_bfloat16* p = (__nv_bfloat16*)out + i;
+    *p = __float2bfloat16_rn(add ? __bfloat162float(*p) + v : v);
+  } else {
+    __half* p = (__half*)out + i;
+    *p = __float2half_rn(add ? __half2float(*p) + v : v);
+  }
+}
+
+struct SumArgs {
+  const void* grad;
+  int64_t ldg, d;
+  const int* order;
+  const int* rows;
+  const int* count;
+  float scale;
+  void* out;
+  int64_t ldo;
+  MType ot;
+  bool accumulate, vec;
+  float* head;  // [tiles, d] a tile's part of the row it shares with the tile before
+  float* tail;  // [tiles, d] ... of the row it shares with the tile after (and not before)
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kSumThreads) sum_kernel(const SumArgs a) {
+  constexpr int kN = 16 / sizeof(T);
+  __shared__ int order[kEntries], rows[kEntries + 2];
+  pdl_release();
+  pdl_wait();
+  const int n = *a.count;
+  const int64_t e0 = blockIdx.x * (int64_t)kEntries;
+  if (e0 >= n) return;
+  const int m = (int)min((int64_t)kEntries, n - e0);
+  if (threadIdx.x < kEntries + 2) {  // rows[0] and rows[m + 1]: the neighbours' (or -1)
+    const int64_t e = e0 + (int)threadIdx.x - 1;
+    rows[threadIdx.x] = e >= 0 && e < n ? a.rows[e] : -1;
+  }
+  if (threadIdx.x < m) order[threadIdx.x] = a.order[e0 + threadIdx.x];
+  __syncthreads();
+  const int64_t c = (blockIdx.y * (int64_t)kSumThreads + threadIdx.x) * kN;
+  if (c >= a.d) return;
+  const int nc = (int)min((int64_t)kN, a.d - c);
+  float acc[kN] = {};
+  bool started_before = rows[0] == rows[1];
+  for (int e = 0; e < m; e++) {
+    add_vec<T>((const T*)a.grad + (int64_t)order[e] * a.ldg + c, acc, nc, a.vec);
+    const int row = rows[e + 1];
+    if (rows[e + 2] == row && e + 1 < m) continue;
+    const bool goes_on = rows[e + 2] == row;  // into the next tile
+    if (started_before || goes_on) {
+      float* p = (started_before ? a.head : a.tail) + blockIdx.x * a.d + c;
+#pragma unroll
+      for (int q = 0; q < kN; q++)
+        if (q < nc) p[q] = acc[q];
+    } else {
+#pragma unroll
+      for (int q = 0; q < kN; q++)
+        if (q < nc) put(a.out, row * a.ldo + c + q, a.ot, acc[q] * a.scale, a.accumulate);
+    }
+#pragma unroll
+    for (int q = 0; q < kN; q++) acc[q] = 0.f;
+    started_before = false;
+  }
+}
+
+// Rows that cross tiles: the CTA of the tile where the row starts adds its
+// tail and the heads of the tiles after it, in order.  Eight warps take
+// neighbouring stretches of the tiles and are added in warp order.
+__global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
+  __shared__ float part[8][32];
+  __shared__ int last_s;
+  pdl_release();
+  pdl_wait();
+  const int n = *a.count;
+  const int64_t t = blockIdx.x, e0 = t * kEntries, e1 = e0 + kEntries;
+  if (e1 >= n) return;
+  const int row = a.rows[e1 - 1];
+  if (a.rows[e1] != row) return;
+  if (a.rows[e0] == row && e0 > 0 && a.rows[e0 - 1] == row) return;  // starts earlier
+  if (threadIdx.x == 0) {
+    int64_t lo = e1, hi = n;  // first entry of another row
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (a.rows[mid] == row)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    last_s = (int)((lo - 1) / kEntries);
+  }
+  __syncthreads();
+  const int64_t heads = last_s - t;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t per = (heads + 7) / 8, h0 = t + 1 + warp * per, h1 = min(t + 1 + heads, h0 + per);
+  for (int64_t c0 = 0; c0 < a.d; c0 += 32) {
+    const int64_t c = c0 + lane;
+    float v = 0.f;
+    if (c < a.d) {
+#pragma unroll 8
+      for (int64_t h = h0; h < h1; h++) v += a.head[h * a.d + c];
+    }
+    part[warp][lane] = v;
+    __syncthreads();
+    if (warp == 0 && c < a.d) {
+      float s = a.tail[t * a.d + c];
+#pragma unroll
+      for (int w = 0; w < 8; w++) s += part[w][lane];
+      put(a.out, row * a.ldo + c, a.ot, s * a.scale, a.accumulate);
+    }
+    __syncthreads();
+  }
+}
+
+}  // namespace
+
+void embedding(MType t, const void* table, int64_t v, int64_t d, int64_t ldt, const void* ids, bool ids64, int64_t n,
+               int64_t first, float scale, void* out, int64_t ldo, cudaStream_t s) {
+  if (n == 0 || d == 0) return;
+  auto go = [&](auto tv) {
+    using T = decltype(tv);
+    const int kn = 16 / (int)sizeof(T);
+    const bool vec = d % kn == 0 && ldt % kn == 0 && ldo % kn == 0 && (uintptr_t)table % 16 == 0 && (uintptr_t)out % 16 == 0;
+    // few rows: several warps a row, down to 512 bytes each
+    const int64_t want = (int64_t)ctx().sm_count * 16;
+    const int64_t most = std::max<int64_t>(1, d * (int64_t)sizeof(T) / 512);
+    const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(most, want / n));
+    const int64_t blocks = (n * parts + 7) / 8;
+    if (blocks > 0x7fffffff) throw Error(ErrKind::InvalidArgument, "embedding: too many ids");
+    auto launch = [&](auto kern) {
+      launch_pdl(kern, dim3((unsigned)blocks), dim3(256), 0, s, (const T*)table, v, d, ldt, ids, n, first, scale, (T*)out, ldo, parts);
+    };
+    if (ids64)
+      vec ? launch(lookup_kernel<T, true, true>) : launch(lookup_kernel<T, true, false>);
+    else
+      vec ? launch(lookup_kernel<T, false, true>) : launch(lookup_kernel<T, false, false>);
+    count_launch();
+  };
+  if (t == MType::F32)
+    go(float{});
+  else if (t == MType::BF16)
+    go(__nv_bfloat16{});
+  else
+    go(__half{});
+}
+
+void embedding_grad(MType gt, const void* grad, int64_t ldg, const void* ids, bool ids64, int64_t n, int64_t v,
+                    int64_t d, int64_t first, float scale, MType ot, void* out, int64_t ldo, bool accumulate,
+                    cudaStream_t s) {
+  if (v == 0 || d == 0) return;
+  if (n >= (int64_t)1 << 31 || v >= (int64_t)1 << 31) throw Error(ErrKind::InvalidArgument, "embedding_grad: 2^31 ids or rows");
+  const int sms = ctx().sm_count;
+  const int64_t range = std::min<int64_t>((v + sms - 1) / sms, 32768);  // its counters fit shared memory
+  const int ctas = (int)((v + range - 1) / range);
+  const size_t smem = (size_t)(range + 2 * kList) * 4;
+  const int64_t tiles = (n + kEntries - 1) / kEntries;
+  Workspace ws((size_t)(2 * n + 4) * 4 + (size_t)(2 * tiles * d) * 4, s);
+  SortArgs a{};
+  a.ids = ids, a.n = n, a.first = first, a.v = v, a.range = range;
+  float* parts = (float*)ws.p;
+  a.order = (int*)(parts + 2 * tiles * d), a.rows = a.order + n, a.count = a.rows + n;
+  a.out = accumulate ? nullptr : out;
+  a.d_bytes = d * msize(ot), a.ld_bytes = ldo * msize(ot);
+  auto sort = [&](auto kern) {
+    ensure_dynamic_smem((const void*)kern, smem);
+    launch_pdl(kern, dim3((unsigned)ctas), dim3(kSortThreads), smem, s, a);
+    count_launch();
+  };
+  ids64 ? sort(sort_kernel<true>) : sort(sort_kernel<false>);
+  if (n == 0) return;
+  SumArgs b{};
+  b.grad = grad, b.ldg = ldg, b.d = d, b.order = a.order, b.rows = a.rows, b.count = a.count;
+  b.scale = scale, b.out = out, b.ldo = ldo, b.ot = ot, b.accumulate = accumulate;
+  b.head = parts, b.tail = parts + tiles * d;
+  const int kn = 16 / msize(gt);
+  b.vec = d % kn == 0 && ldg % kn == 0 && (uintptr_t)grad % 16 == 0;
+  const dim3 grid((unsigned)tiles, (unsigned)((d + kSumThreads * kn - 1) / (kSumThreads * kn)));
+  if (gt == MType::F32)
+    launch_pdl(sum_kernel<float>, grid, dim3(kSumThreads), 0, s, b);
+  else if (gt == MType::BF16)
+    launch_pdl(sum_kernel<__nv_bfloat16>, grid, dim3(kSumThreads), 0, s, b);
+  else
+    launch_pdl(sum_kernel<__half>, grid, dim3(kSumThreads), 0, s, b);
+  count_launch();
+  if (tiles > 1) {
+    launch_pdl(join_kernel, dim3((unsigned)(tiles - 1)), dim3(256), 0, s, b);
+    count_launch();
+  }
+}
+
+}  // namespace ndt

@@ -1,0 +1,595 @@
+// Products of block-scaled 8-bit matrices on the fifth-generation tensor cores.
+//
+//   C[i, j] = sum over kb of sa(i, kb) * sb(j, kb) * P_kb[i, j] (+ C[i, j])
+//   P_kb[i, j] = sum over the 128 k of block kb of a[i, k] * b[j, k]
+//
+// The scales change every 128 k, so the tensor core sums one block at a time
+// (four k = 32 steps of tcgen05.mma kind::f8f6f4, 32-bit accumulators in
+// TMEM) and the epilogue warps multiply each P_kb by its scales and add it to
+// accumulators in registers, in 32 bits.  Two TMEM buffers let the tensor
+// core work on block kb + 1 meanwhile.
+//
+// Roles (11 warps): 0 loads the operand tiles by TMA into a ring of 128-byte
+// swizzled stages, 1 issues the MMAs, 2 loads the scales into a ring of its
+// own (cp.async), 3 - 10 scale and sum (a thread holds one row and half the
+// tile's columns).
+//
+// Two forms.  CTAS = 1: one CTA computes a 128 x BN tile; where there are few
+// tiles a cluster of CTAs splits k and adds its parts through distributed
+// shared memory, in rank order (no workspace, no atomics).  CTAS = 2: a CTA
+// pair computes 256 x 256 with cta_group::2 MMAs, each CTA staging its half of
+// both operands; persistent.
+//
+// sa * sb is formed in 32 bits: it stays finite while the product of two
+// blocks' largest values is below 2^127.
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "model_ops.h"
+
+namespace ndt {
+namespace {
+
+constexpr int kBK = 128;     // one scale block, one swizzled row
+constexpr int kThreads = 352;
+constexpr int kEpiWarp0 = 3;
+constexpr int kEpiWarps = 8;
+constexpr int kSlots = 8;    // scale ring
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+
+struct GemmArgs {
+  const float* sa;
+  const float* sb;
+  int64_t sa_rs, sa_cs, sb_rs, sb_cs;
+  void* c;
+  int64_t ldc;
+  int m, n, kblocks;
+  int tiles_m, tiles_n;
+  int ksplit;
+  uint32_t idesc;
+  int a_row;       // a scale for each row of A (else for each 128)
+  int ctype;       // MType of C
+  int accumulate;
+  int vec;         // 16-byte stores are aligned
+  int* flag;       // set when a bounded wait ran out
+};
+
+// ------------------------------------------------------------- PTX pieces
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+__device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// A wait that ends: after two seconds, or once another wait of this CTA has
+// given up, it raises the flags and returns false.
+__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
+  const uint64_t t0 = now_ns();
+  while (true) {
+    for (int i = 0; i < 32; i++)
+      if (mbar_try(bar, parity)) return true;
+    if (*gave_up) return false;
+    if (now_ns() - t0 > kWaitLimitNs) {
+      *gave_up = 1;
+      atomicExch_system(flag, 1);
+      return false;
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
+  if (mbar_try(bar, parity)) return true;
+  return mbar_wait_slow(bar, parity, gave_up, flag);
+}
+// For a whole warp: all lanes go on, or none.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
+  return __all_sync(~0u, mbar_wait(bar, parity, gave_up, flag));
+}
+
+template <int CTAS>
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+  else  // bar is the leader's
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+        "[%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+
+// K-major operand tile of 128-byte rows, 128-byte swizzle: 8-row groups are
+// 1024 bytes apart.  (Start address, offsets in units of 16 bytes; bit 46 is
+// the descriptor version of sm_100, 2 at bit 61 the 128-byte swizzle.)
+__device__ __forceinline__ uint64_t tile_desc(uint32_t addr) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 |
+         (uint64_t)2 << 61;
+}
+template <int CTAS>
+__device__ __forceinline__ void mma_f8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(add)
+        : "memory");
+}
+// The barrier (of both CTAs of a pair) is arrived at when the MMAs issued so
+// far are done.
+template <int CTAS>
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  if constexpr (CTAS == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+// One 4-byte element into shared memory; zero where !valid.
+__device__ __forceinline__ void cp4(uint32_t dst, const float* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+
+__device__ __forceinline__ float load_c(const void* c, int64_t i, int type) {
+  if (type == (int)MType::F32) return ((const float*)c)[i];
+  if (type == (int)MType::BF16) return __bfloat162float(((const __nv_bfloat16*)c)[i]);
+  return __half2float(((const __half*)c)[i]);
+}
+__device__ __forceinline__ void store_c(void* c, int64_t i, int type, float v) {
+  if (type == (int)MType::F32)
+    ((float*)c)[i] = v;
+  else if (type == (int)MType::BF16)
+    ((__nv_bfloat16*)c)[i] = __float2bfloat16_rn(v);
+  else
+    ((__half*)c)[i] = __float2half_rn(v);
+}
+
+// tile index -> (row tile, column tile): bands of 8 row tiles are walked
+// column by column, so the tiles in flight share operand tiles in L2.
+__device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
+  constexpr int kBand = 8;
+  const int band = t / (kBand * tiles_n), first = band * kBand;
+  const int rows = min(kBand, tiles_m - first);
+  const int in = t - band * kBand * tiles_n;
+  tm = first + in % rows;
+  tn = in / rows;
+}
+
+template <int CTAS, int BN>
+struct Shape {
+  static constexpr int kBM = 128;                    // rows of one CTA
+  static constexpr int kBRows = BN / CTAS;           // rows of B that one CTA stages
+  static constexpr int kABytes = kBM * kBK, kBBytes = kBRows * kBK;
+  static constexpr int kStage = kABytes + kBBytes;
+  static constexpr int kStages = (192 * 1024) / kStage;
+  static constexpr int kScaleFloats = kBM + BN;      // a slot of the scale ring
+  static constexpr int kTmemCols = 2 * BN;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + (size_t)kSlots * kScaleFloats * 4;
+  static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns");
+  static_assert((size_t)BN * 129 * 4 <= (size_t)kStages * kStage || CTAS == 2, "the split's buffer reuses the stages");
+};
+
+template <int CTAS, int BN, bool BROW>
+__global__ void __launch_bounds__(kThreads, 1)
+    scaled_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                       const GemmArgs g) {
+  using S = Shape<CTAS, BN>;
+  constexpr int kHalf = BN / 2;  // columns of one epilogue thread
+  extern __shared__ unsigned char raw[];
+  __shared__ __align__(8) uint64_t bars[2 * S::kStages + 2 * kSlots + 4];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ int gave_up_s;
+  const uint32_t stage0 = (smem_u32(raw) + 1023) & ~1023u;
+  float* scale_ring = reinterpret_cast<float*>(raw + (stage0 - smem_u32(raw)) + (size_t)S::kStages * S::kStage);
+  const uint32_t full = smem_u32(bars), empty = full + 8 * S::kStages, sfull = empty + 8 * S::kStages,
+                 sempty = sfull + 8 * kSlots, tfull = sempty + 8 * kSlots, tempty = tfull + 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = CTAS == 2 ? cluster_rank() : 0;
+  const bool clustered = CTAS == 2 || g.ksplit > 1;
+  volatile int* gave_up = &gave_up_s;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kStages; i++) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+    for (int i = 0; i < kSlots; i++) mbar_init(sfull + 8 * i, 32), mbar_init(sempty + 8 * i, kEpiWarps);
+    for (int i = 0; i < 2; i++) mbar_init(tfull + 8 * i, 1), mbar_init(tempty + 8 * i, CTAS * kEpiWarps);
+    gave_up_s = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    const uint32_t where = smem_u32(&tmem_base_s);
+    if constexpr (CTAS == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(S::kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "n"(S::kTmemCols) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (clustered) cluster_sync();
+  fence_after();
+  const uint32_t tmem = tmem_base_s;
+  pdl_release();
+  pdl_wait();
+
+  const int split = CTAS == 1 && g.ksplit > 1 ? (int)cluster_rank() : 0;
+  const int unit = CTAS == 1 ? blockIdx.x / g.ksplit : blockIdx.x / 2;
+  const int units = CTAS == 1 ? gridDim.x / g.ksplit : gridDim.x / 2;
+  const int ntiles = g.tiles_m * g.tiles_n;
+  const int kb0 = CTAS == 1 ? (int)((int64_t)g.kblocks * split / g.ksplit) : 0;
+  const int kb1 = CTAS == 1 ? (int)((int64_t)g.kblocks * (split + 1) / g.ksplit) : g.kblocks;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = unit; t < ntiles && ok; t += units) {
+        int tm, tn;
+        tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
+        const int row_a = tm * 128 * CTAS + rank * 128, row_b = tn * BN + rank * S::kBRows;
+        for (int kb = kb0; kb < kb1; kb++) {
+          if (!(ok = mbar_wait(empty + 8 * stage, phase ^ 1, gave_up, g.flag))) break;
+          const uint32_t dst = stage0 + stage * S::kStage;
+          uint32_t bar = full + 8 * stage;
+          if (rank == 0) mbar_expect_tx(bar, CTAS * S::kStage);
+          if (CTAS == 2) bar = mapa(bar, 0);
+          tma_load<CTAS>(dst, &map_a, bar, kb * kBK, row_a);
+          tma_load<CTAS>(dst + S::kABytes, &map_b, bar, kb * kBK, row_b);
+          if (++stage == S::kStages) stage = 0, phase ^= 1;
+        }
+      }
+      // after a wait that gave up: let the copies in flight land before the CTA's memory goes
+      if (!ok)
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0 && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t it = 0;  // k blocks so far: TMEM buffer it & 1
+      bool ok = true;
+      for (int t = unit; t < ntiles && ok; t += units) {
+        for (int kb = kb0; kb < kb1; kb++, it++) {
+          const uint32_t buf = it & 1;
+          if (!(ok = mbar_wait(tempty + 8 * buf, ((it >> 1) & 1) ^ 1, gave_up, g.flag))) break;
+          if (!(ok = mbar_wait(full + 8 * stage, phase, gave_up, g.flag))) break;
+          fence_after();
+          const uint64_t da = tile_desc(stage0 + stage * S::kStage), db = tile_desc(stage0 + stage * S::kStage + S::kABytes);
+#pragma unroll
+          for (int s = 0; s < 4; s++)  // k = 32 a step: 32 bytes along the swizzled row
+            mma_f8<CTAS>(tmem + buf * BN, da + 2 * s, db + 2 * s, g.idesc, s > 0);
+          mma_commit<CTAS>(empty + 8 * stage);
+          mma_commit<CTAS>(tfull + 8 * buf);
+          if (++stage == S::kStages) stage = 0, phase ^= 1;
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = unit; t < ntiles && ok; t += units) {
+      int tm, tn;
+      tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
+      const int row_a = tm * 128 * CTAS + rank * 128, row_b = tn * BN;
+      // this lane's rows: their addresses at k block 0
+      const float* pa[4];
+      bool va[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int r = row_a + lane + 32 * j;
+        va[j] = r < g.m;
+        pa[j] = g.sa + (va[j] ? (int64_t)(g.a_row ? r : r >> 7) * g.sa_rs : 0);
+      }
+      constexpr int kNB = BROW ? BN / 32 : 1;
+      const float* pb[kNB];
+      bool vb[kNB];
+#pragma unroll
+      for (int j = 0; j < kNB; j++) {
+        const int r = BROW ? row_b + lane + 32 * j : row_b + lane * 128;
+        vb[j] = r < g.n && (BROW || lane < (BN + 127) / 128);
+        pb[j] = g.sb + (vb[j] ? (int64_t)(BROW ? r : r >> 7) * g.sb_rs : 0);
+      }
+      for (int kb = kb0; kb < kb1; kb++, it++) {
+        const uint32_t slot = it % kSlots, ph = (it / kSlots) & 1;
+        if (!(ok = warp_wait(sempty + 8 * slot, ph ^ 1, gave_up, g.flag))) break;
+        const uint32_t dst = smem_u32(scale_ring + slot * S::kScaleFloats) + 4 * lane;
+#pragma unroll
+        for (int j = 0; j < 4; j++) cp4(dst + 128 * j, pa[j] + (int64_t)kb * g.sa_cs, va[j]);
+#pragma unroll
+        for (int j = 0; j < kNB; j++)
+          if (BROW || lane < (BN + 127) / 128) cp4(dst + 512 + 128 * j, pb[j] + (int64_t)kb * g.sb_cs, vb[j]);
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sfull + 8 * slot) : "memory");
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncwarp();
+  } else {
+    const int quad = warp & 3, half = (warp - kEpiWarp0) >> 2;
+    const int row = quad * 32 + lane;
+    const uint32_t tmem_row = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
+    const uint32_t tempty_leader = CTAS == 2 ? mapa(tempty, 0) : tempty;
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = unit; t < ntiles && ok; t += units) {
+      int tm, tn;
+      tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
+      float acc[kHalf];
+#pragma unroll
+      for (int j = 0; j < kHalf; j++) acc[j] = 0.f;
+      for (int kb = kb0; kb < kb1; kb++, it++) {
+        const uint32_t slot = it % kSlots, sph = (it / kSlots) & 1, buf = it & 1, ph = (it >> 1) & 1;
+        if (!(ok = warp_wait(sfull + 8 * slot, sph, gave_up, g.flag))) break;
+        const float* sc = scale_ring + slot * S::kScaleFloats;
+        const float sa = sc[row];
+        const float sab = BROW ? sa : sa * sc[128 + (BN == 256 ? half : 0)];
+        if (!(ok = warp_wait(tfull + 8 * buf, ph, gave_up, g.flag))) break;
+        fence_after();
+        uint32_t d[2][16];
+        tmem_ld16(tmem_row + buf * BN, d[0]);
+#pragma unroll
+        for (int q = 0; q < kHalf / 16; q++) {
+          tmem_ld_wait();
+          if (q + 1 < kHalf / 16) tmem_ld16(tmem_row + buf * BN + (q + 1) * 16, d[(q + 1) & 1]);
+          if (BROW) {
+#pragma unroll
+            for (int j = 0; j < 16; j += 4) {
+              const float4 b = *reinterpret_cast<const float4*>(sc + 128 + half * kHalf + q * 16 + j);
+              acc[q * 16 + j] = fmaf(__uint_as_float(d[q & 1][j]), sab * b.x, acc[q * 16 + j]);
+              acc[q * 16 + j + 1] = fmaf(__uint_as_float(d[q & 1][j + 1]), sab * b.y, acc[q * 16 + j + 1]);
+              acc[q * 16 + j + 2] = fmaf(__uint_as_float(d[q & 1][j + 2]), sab * b.z, acc[q * 16 + j + 2]);
+              acc[q * 16 + j + 3] = fmaf(__uint_as_float(d[q & 1][j + 3]), sab * b.w, acc[q * 16 + j + 3]);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 16; j++) acc[q * 16 + j] = fmaf(__uint_as_float(d[q & 1][j]), sab, acc[q * 16 + j]);
+          }
+        }
+        fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if (CTAS == 2)
+            mbar_arrive_cluster(tempty_leader + 8 * buf);
+          else
+            mbar_arrive(tempty + 8 * buf);
+          mbar_arrive(sempty + 8 * slot);
+        }
+      }
+      if (!ok) break;
+      const int row_c = tm * 128 * CTAS + rank * 128 + row, col_c = tn * BN + half * kHalf;
+      if (CTAS == 1 && g.ksplit > 1) {
+        // this CTA's part, column-major with an odd pitch, over the stages (all consumed)
+        float* part = reinterpret_cast<float*>(raw + (stage0 - smem_u32(raw)));
+#pragma unroll
+        for (int j = 0; j < kHalf; j++) part[(half * kHalf + j) * 129 + row] = acc[j];
+      } else if (row_c < g.m) {
+        const int64_t base = (int64_t)row_c * g.ldc + col_c;
+        const int cols = min(kHalf, g.n - col_c);
+        if (g.vec && cols == kHalf && !g.accumulate) {
+          if (g.ctype == (int)MType::F32) {
+            float4* p = reinterpret_cast<float4*>((float*)g.c + base);
+#pragma unroll
+            for (int j = 0; j < kHalf / 4; j++) p[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+          } else {
+            uint4* p = reinterpret_cast<uint4*>((uint16_t*)g.c + base);
+#pragma unroll
+            for (int j = 0; j < kHalf / 8; j++) {
+              uint32_t w[4];
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                if (g.ctype == (int)MType::BF16) {
+                  const __nv_bfloat162 h = __floats2bfloat162_rn(acc[8 * j + 2 * i], acc[8 * j + 2 * i + 1]);
+                  w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                } else {
+                  const __half2 h = __floats2half2_rn(acc[8 * j + 2 * i], acc[8 * j + 2 * i + 1]);
+                  w[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+              }
+              p[j] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < kHalf; j++)
+            if (j < cols) {
+              float v = acc[j];
+              if (g.accumulate) v += load_c(g.c, base + j, g.ctype);
+              store_c(g.c, base + j, g.ctype, v);
+            }
+        }
+      }
+    }
+  }
+
+  // every role is done with this CTA's barriers, TMEM and (pair) the peer's
+  fence_before();
+  __syncthreads();
+  if (CTAS == 1 && g.ksplit > 1) {
+    cluster_sync();
+    // each CTA adds its share of the tile's columns over all parts, in rank order
+    int tm, tn;
+    tile_at(unit, g.tiles_m, g.tiles_n, tm, tn);
+    const int rows = min(128, g.m - tm * 128), cols = BN / g.ksplit;
+    const uint32_t part = stage0;
+    for (int e = threadIdx.x; e < rows * cols; e += kThreads) {
+      const int r = e / cols, j = split * cols + e % cols;
+      const uint32_t at = part + (uint32_t)(j * 129 + r) * 4;
+      float v = 0.f;
+      for (int p = 0; p < g.ksplit; p++) v += ld_cluster(mapa(at, p));
+      const int col = tn * BN + j;
+      if (col < g.n && !*gave_up) {
+        const int64_t i = (int64_t)(tm * 128 + r) * g.ldc + col;
+        if (g.accumulate) v += load_c(g.c, i, g.ctype);
+        store_c(g.c, i, g.ctype, v);
+      }
+    }
+    cluster_sync();
+  } else if (CTAS == 2) {
+    cluster_sync();
+  }
+  fence_after();
+  if (warp == 1) {
+    if constexpr (CTAS == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kTmemCols));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kTmemCols));
+  }
+}
+
+// ------------------------------------------------------------------- host
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    NDT_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r));
+    if (!p || r != cudaDriverEntryPointSuccess) throw Error(ErrKind::Cuda, "cuTensorMapEncodeTiled is not in this driver");
+    return (EncodeFn)p;
+  }();
+  return fn;
+}
+// Boxes of box_rows x 128 bytes; bytes outside the matrix read as zeros (0.0 in both 8-bit types).
+CUtensorMap operand_map(const ScaledOperand& o, int64_t k, int box_rows) {
+  CUtensorMap m;
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)o.rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)o.ld};
+  const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows};
+  const cuuint32_t one[2] = {1, 1};
+  const CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(o.p), dims, strides, box, one,
+                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Error(ErrKind::Cuda, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return m;
+}
+
+template <int CTAS, int BN, bool BROW>
+void launch(const ScaledOperand& a, const ScaledOperand& b, int64_t k, GemmArgs g, int grid, int cluster, cudaStream_t s) {
+  using S = Shape<CTAS, BN>;
+  const CUtensorMap ma = operand_map(a, k, 128), mb = operand_map(b, k, S::kBRows);
+  auto kern = scaled_gemm_kernel<CTAS, BN, BROW>;
+  ensure_dynamic_smem((const void*)kern, S::kSmem);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  NDT_CUDA(cudaLaunchKernelEx(&cfg, kern, ma, mb, g));
+  count_launch();
+}
+
+}  // namespace
+
+void scaled_gemm(const ScaledOperand& a, const ScaledOperand& b, int64_t k, MType ct, void* c, int64_t ldc,
+                 bool accumulate, cudaStream_t s) {
+  GemmArgs g{};
+  g.sa = a.s, g.sa_rs = a.srs, g.sa_cs = a.scs;
+  g.sb = b.s, g.sb_rs = b.srs, g.sb_cs = b.scs;
+  g.c = c, g.ldc = ldc;
+  g.m = (int)a.rows, g.n = (int)b.rows;
+  g.kblocks = (int)((k + kBK - 1) / kBK);
+  g.a_row = a.per_row, g.ctype = (int)ct, g.accumulate = accumulate;
+  g.vec = (uintptr_t)c % 16 == 0 && ldc * msize(ct) % 16 == 0;
+  g.flag = wait_flag_device();
+  g.ksplit = 1;
+  const int sms = ctx().sm_count;
+  auto cdiv = [](int64_t x, int64_t y) { return (int)((x + y - 1) / y); };
+  // bits of the instruction descriptor: 32-bit accumulators, the operands'
+  // types (0 e4m3, 1 e5m2), both K-major, N / 8 and M / 16
+  auto idesc = [&](int m, int n) {
+    return 1u << 4 | (a.type == MType::E5M2 ? 1u : 0u) << 7 | (b.type == MType::E5M2 ? 1u : 0u) << 10 |
+           (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
+  };
+  const int pair_tiles = cdiv(g.m, 256) * cdiv(g.n, 256);
+  if (pair_tiles * 2 >= sms / 2) {
+    g.tiles_m = cdiv(g.m, 256), g.tiles_n = cdiv(g.n, 256);
+    g.idesc = idesc(256, 256);
+    const int grid = 2 * std::min(pair_tiles, sms / 2);
+    if (b.per_row)
+      launch<2, 256, true>(a, b, k, g, grid, 2, s);
+    else
+      launch<2, 256, false>(a, b, k, g, grid, 2, s);
+    return;
+  }
+  g.tiles_m = cdiv(g.m, 128), g.tiles_n = cdiv(g.n, 128);
+  g.idesc = idesc(128, 128);
+  int split = 1;
+  while (split < 8 && g.tiles_m * g.tiles_n * split * 2 <= sms && g.kblocks >= 4 * split) split *= 2;
+  g.ksplit = split;
+  const int grid = g.tiles_m * g.tiles_n * split;
+  if (b.per_row)
+    launch<1, 128, true>(a, b, k, g, grid, split, s);
+  else
+    launch<1, 128, false>(a, b, k, g, grid, split, s);
+}
+
+}  // namespace ndt

@@ -34,14 +34,31 @@ def set_stream(stream_ptr) -> None:
     check_status(get_lib().ndt_b200_set_stream(ctypes.c_void_p(stream_ptr) if stream_ptr else None), "set_stream")
 
 
-def __getattr__(name: str):
-    """``torch_contract`` loads on first use, as in the reference binding
-    (python/ndtensors_rs/src/ndtensors_rs/__init__.py)."""
-    if name == "torch_contract":
-        from .torch_ops import torch_contract
+#: names that load torch on first use, and the modules that hold them
+_TORCH_NAMES = {
+    "torch_contract": "torch_ops",
+    "quantize_blocks": "scaled",
+    "scaled_gemm": "scaled",
+    "scaled_linear": "scaled",
+    "torch_scaled_linear": "scaled",
+    "embedding": "embeddings",
+    "embedding_grad": "embeddings",
+    "torch_embedding": "embeddings",
+    "expert_layer": "experts",
+}
 
-        return torch_contract
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+def __getattr__(name: str):
+    """The torch operators load on first use, as ``torch_contract`` does in the
+    reference binding (python/ndtensors_rs/src/ndtensors_rs/__init__.py)."""
+    module = _TORCH_NAMES.get(name)
+    if module is None:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from importlib import import_module
+
+    value = getattr(import_module(f".{module}", __name__), name)
+    globals()[name] = value
+    return value
 
 
 __all__ = [
@@ -63,4 +80,5 @@ __all__ = [
     "synchronize",
     "launch_count",
     "set_stream",
+    *_TORCH_NAMES,
 ]

@@ -29,6 +29,7 @@ c_int_p = ctypes.POINTER(ctypes.c_int)
 c_long_p = ctypes.POINTER(ctypes.c_long)
 c_double_p = ctypes.POINTER(ctypes.c_double)
 vp = ctypes.c_void_p
+ci, cl, cf = ctypes.c_int, ctypes.c_long, ctypes.c_float
 
 # (name, restype, argtypes) for every exported symbol
 SIGNATURES = [
@@ -166,6 +167,17 @@ SIGNATURES = [
         [vp, c_size_p, ctypes.c_size_t, c_long_p, vp, c_size_p, ctypes.c_size_t, c_long_p, vp, ctypes.c_size_t,
          c_size_p, c_size_p, vp],
     ),
+    # ---- language-model operators on device memory
+    ("ndt_b200_quantize_dev", ctypes.c_int,
+     [ci, vp, cl, cl, cl, cl, ci, ci, vp, cl, vp, cl, cl, vp, cl, vp, cl, cl, vp]),
+    ("ndt_b200_scaled_gemm_dev", ctypes.c_int,
+     [cl, cl, cl, ci, vp, cl, cl, ci, vp, cl, cl, ci, vp, cl, cl, ci, vp, cl, cl, ci, vp, cl, ci, vp]),
+    ("ndt_b200_scaled_linear_dev", ctypes.c_int,
+     [ci, vp, cl, cl, cl, cl, ci, vp, cl, cl, cl, vp, cl, cl, ci, vp, cl, vp]),
+    ("ndt_b200_embedding_dev", ctypes.c_int, [ci, vp, cl, cl, cl, vp, ci, cl, cl, cf, vp, cl, vp]),
+    ("ndt_b200_embedding_grad_dev", ctypes.c_int, [ci, vp, cl, vp, ci, cl, cl, cl, cl, cf, ci, vp, cl, ci, vp]),
+    ("ndt_b200_expert_layer_dev", ctypes.c_int,
+     [ci, vp, cl, cl, cl, vp, cl, ci, vp, vp, vp, vp, cl, cl, ci, vp, cl, vp, vp, vp]),
     ("ndt_b200_device_available", ctypes.c_int, []),
     ("ndt_b200_set_stream", ctypes.c_int, [vp]),
     ("ndt_b200_get_stream", vp, []),

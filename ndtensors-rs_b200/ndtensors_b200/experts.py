@@ -1,0 +1,71 @@
+"""A mixture-of-experts layer for a few tokens: a block-sparse contraction
+whose blocks the data choose, in one kernel on torch's current stream."""
+
+from __future__ import annotations
+
+import torch
+
+from ._model import CODES, call, check_cuda, check_type, on, rows_of, unit_rows
+
+E4M3 = torch.float8_e4m3fn
+
+
+def expert_layer(x, router, w_in, w_out, top: int, in_scales=None, out_scales=None, renormalize: bool = True):
+    """The layer's output for x [..., h], and each token's choice.
+
+    ``router`` is [experts, h], ``w_in`` [experts, 2 i, h] (gate rows, then up
+    rows), ``w_out`` [experts, h, i].  A token goes to the ``top`` experts of
+    its largest router products (ties to the lowest index), weighted by their
+    softmax over all experts, divided by the sum of the chosen with
+    ``renormalize``; an expert computes ``w_out (silu(gate) * up)``.
+
+    x is bfloat16 or float16, router too; the experts' weights have x's type or
+    are float8 e4m3 with the float32 scales of their 128 x 128 blocks
+    (``in_scales`` [experts, ceil(2 i / 128), ceil(h / 128)], ``out_scales``
+    [experts, ceil(h / 128), ceil(i / 128)]).
+
+    Returns ``(y, ids, weights)``: x's shape and type, and int32 / float32
+    [..., top].  Made for at most about a hundred tokens (a decoding batch);
+    more are right, but each 8 to 32 tokens of an expert read its weights anew.
+    """
+    check_cuda("expert_layer", x, router, w_in, w_out, in_scales, out_scales)
+    check_type("expert_layer", "x", x.dtype, (torch.bfloat16, torch.float16))
+    check_type("expert_layer", "router", router.dtype, (x.dtype,))
+    check_type("expert_layer", "w_in", w_in.dtype, (x.dtype, E4M3))
+    check_type("expert_layer", "w_out", w_out.dtype, (w_in.dtype,))
+    if router.dim() != 2 or w_in.dim() != 3 or w_out.dim() != 3 or x.dim() < 1:
+        raise ValueError("expert_layer: router is a matrix, w_in and w_out have three axes")
+    e, h = router.shape
+    i = w_out.shape[2]
+    if x.shape[-1] != h or w_in.shape != (e, 2 * i, h) or w_out.shape != (e, h, i):
+        raise ValueError("expert_layer: the sizes of x, router, w_in and w_out do not fit")
+    if not 1 <= top <= e:
+        raise ValueError("expert_layer: top must be from 1 to the number of experts")
+    if w_in.dtype == E4M3:
+        if in_scales is None or out_scales is None:
+            raise ValueError("expert_layer: float8 weights need in_scales and out_scales")
+        hb, ib, jb = (h + 127) // 128, (i + 127) // 128, (2 * i + 127) // 128
+        if in_scales.shape != (e, jb, hb) or out_scales.shape != (e, hb, ib):
+            raise ValueError("expert_layer: scales do not fit the weights' 128 x 128 blocks")
+        check_type("expert_layer", "in_scales", in_scales.dtype, (torch.float32,))
+        check_type("expert_layer", "out_scales", out_scales.dtype, (torch.float32,))
+        in_scales, out_scales = in_scales.contiguous(), out_scales.contiguous()
+    elif in_scales is not None or out_scales is not None:
+        raise ValueError("expert_layer: scales are for float8 weights")
+    x2 = unit_rows(rows_of(x))
+    router, w_in, w_out = router.contiguous(), w_in.contiguous(), w_out.contiguous()
+    t = x2.shape[0]
+    y = torch.empty((t, h), dtype=x.dtype, device=x.device)
+    ids = torch.empty((t, top), dtype=torch.int32, device=x.device)
+    weights = torch.empty((t, top), dtype=torch.float32, device=x.device)
+    ctx, stream = on(x.device)
+    with ctx:
+        call("ndt_b200_expert_layer_dev", CODES[x.dtype], x2.data_ptr(), t, h, max(h, x2.stride(0)), router.data_ptr(), e,
+             CODES[w_in.dtype], w_in.data_ptr(), None if in_scales is None else in_scales.data_ptr(), w_out.data_ptr(),
+             None if out_scales is None else out_scales.data_ptr(), i, top, renormalize, y.data_ptr(), h,
+             ids.data_ptr(), weights.data_ptr(), stream)
+    lead = x.shape[:-1]
+    return (y, ids, weights) if x.dim() == 2 else (y.view(x.shape), ids.view(lead + (top,)), weights.view(lead + (top,)))
+
+
+__all__ = ["expert_layer"]
