@@ -484,6 +484,21 @@ int ndt_b200_scaled_linear_dev(int x_type, const void* x, long tokens, long k, l
                                int w_type, const void* w, long n, long w_row_stride, long w_col_stride,
                                const float* w_scales, long w_scale_row_stride, long w_scale_col_stride, int y_type,
                                void* y, long ldy, void* stream);
+/* A trained layer's output and its gradients, all products in 8 bits.
+ * fwd: y [tokens, n] (x's type) = q(x) q128(w)^T, w [n, k] in NDT_F32 / BF16 /
+ * F16; q128(w) transposed ([k, n], leading dimension ldwt, a multiple of 16)
+ * and its scales ([ceil(n / 128)][ceil(k / 128)] floats, the k blocks
+ * contiguous) are left in wt, wt_scales for the gradient (wt may be NULL).
+ * vjp: dx [tokens, k] (x's type) = q(dy) q128(w) from wt, and dw [n, k] =
+ * q(dy^T) q(x^T)^T; dy has x's type.  dx or dw may be NULL.  q: e4m3, blocks of
+ * 1 x 128 along the contracted index (dy: grad8_type). */
+int ndt_b200_scaled_linear_fwd_dev(int x_type, const void* x, long tokens, long k, long x_row_stride, long x_col_stride,
+                                   int w_type, const void* w, long n, long w_row_stride, long w_col_stride, void* y,
+                                   long ldy, void* wt, long ldwt, float* wt_scales, void* stream);
+int ndt_b200_scaled_linear_vjp_dev(int x_type, const void* dy, long tokens, long n, long dy_row_stride, long dy_col_stride,
+                                   const void* x, long k, long x_row_stride, long x_col_stride, const void* wt, long ldwt,
+                                   const float* wt_scales, int grad8_type, void* dx, long lddx, int dw_type, void* dw,
+                                   long lddw, void* stream);
 /* out[i, :] = scale * table[ids[i] - first, :] for n ids (int32, or int64 with
  * ids64), rounded once; zeros where the id names no row (a table that holds a
  * slice of the vocabulary passes its first id). */

@@ -12,12 +12,17 @@
 // SMs.
 //
 // Products run on the warp-level tensor cores with the weights as the 16-row
-// operand and up to 8 tokens a column tile: a lane loads 16 contiguous bytes
+// operand and up to 8 tokens a column tile: a lane copies 16 contiguous bytes
 // of two weight rows, and since the order of k within a product is free, those
 // bytes are its operand fragments as they are (the tokens' fragments are
 // loaded with the same order).  In the first product the two rows are the gate
 // and the up row of the same output, so silu(gate) * up needs no exchange.
 // The warps of a CTA split k and add their parts through shared memory.
+//
+// The weights stream through a ring of cp.async copies in shared memory, each
+// lane reading back only what it copied itself, so no barrier stands between a
+// copy and its use.  The ring runs across tasks, and from the first product
+// into the second before the grid barrier between them.
 //
 // All sums are in 32 bits.  The activations b enter the second product as the
 // sum of two 16-bit numbers (16 or 22 bits of mantissa), so it loses nothing
@@ -40,14 +45,17 @@ constexpr int kMaxSlots = 4096;    // (token, chosen expert) pairs of one launch
 constexpr int kMaxTokens = 256;
 constexpr int kMaxExperts = 1024;
 constexpr int kGroup = 8;          // tokens of one router product
+constexpr int kMaxUnits = kMaxExperts + kMaxSlots / 32;
 
 struct LayerArgs {
   ExpertArgs e;
   int tokens, experts, top, h, i;
+  int ip;           // i rounded up to 8: the pitch of b's rows
   float* logits;    // [tokens, experts]
-  float* b;         // [slots, i]
+  void* b;          // [slots, 2, ip] bf16 high and low parts, or [slots, ip] floats (float16 layers)
   float* o;         // [slots, h]
   unsigned* bmax;   // [slots] bits of max |b|
+  unsigned* done;   // [row tiles of w_out] parts of a tile that are finished
 };
 
 template <typename M>
@@ -103,8 +111,21 @@ __device__ __forceinline__ uint4 row16(const T* row, int k, int n, bool on) {
     return v;
   }
 }
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// The same into shared memory: an asynchronous copy where rows are whole vectors.
+template <typename T, bool VEC>
+__device__ __forceinline__ void copy16(void* dst, const T* row, int k, int n, bool on) {
+  if constexpr (VEC) {
+    const bool in = on && k < n;
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(in ? row + k : row),
+                 "r"(in ? 16 : 0)
+                 : "memory");
+  } else {
+    *reinterpret_cast<uint4*>(dst) = row16<T, false>(row, k, n, on);
+  }
+}
 
-// The weights' side of one step of k: a lane's two rows as pairs of M.
+// The weights' side of one step of k: a lane's 16 bytes of a row as pairs of M.
 template <typename W, typename M>
 struct Step {
   static constexpr int kPerLane = 16 / sizeof(W);  // k of a lane
@@ -123,328 +144,499 @@ struct Step {
 };
 
 struct Lists {
-  int* slots;    // [tokens * top] slots (token * top + place) expert by expert, in order
-  int* first;    // [experts + 1]
-  int* active;   // experts with tokens
-  int n_active;
+  uint16_t chosen[kMaxSlots];     // the expert of each slot (token * top + place)
+  uint16_t slots[kMaxSlots];      // slots expert by expert, in order
+  int first[kMaxExperts + 1];     // where an expert's slots start
+  uint16_t unit_expert[kMaxUnits];  // an expert with up to 8 NT of its slots
+  uint16_t unit_first[kMaxUnits];   // ... from this place of `slots` on
+  int units;
 };
+
+// The sortable form of a product: NaN above all, as in a sort; -0 and 0 equal.
+__device__ __forceinline__ uint32_t sortable(float f) {
+  f += 0.f;
+  const uint32_t u = __float_as_uint(f);
+  return f != f ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+// One token's choice, by a warp that holds PER of its products a lane.
+template <int PER>
+__device__ __forceinline__ void choose(const LayerArgs& a, int t, Lists& L) {
+  const int lane = threadIdx.x & 31;
+  const float* l = a.logits + (int64_t)t * a.experts;
+  float v[PER];
+  uint32_t key[PER];
+  float top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    const bool on = j * 32 + lane < a.experts;
+    v[j] = on ? l[j * 32 + lane] : -INFINITY;
+    key[j] = on ? sortable(v[j]) : 0;  // below every product's
+    top = fmaxf(top, v[j]);
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+#pragma unroll
+  for (int j = 0; j < PER; j++) {
+    v[j] = expf(v[j] - top);
+    if (j * 32 + lane < a.experts) sum += v[j];
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+  float total = 0.f;
+  const bool tell = blockIdx.x == 0;
+  for (int r = 0; r < a.top; r++) {
+    uint32_t best = 0, at = 0;
+#pragma unroll
+    for (int j = PER - 1; j >= 0; j--)
+      if (key[j] >= best) best = key[j], at = j;
+    const uint32_t most = __reduce_max_sync(~0u, best);
+    const uint32_t e = __reduce_min_sync(~0u, best == most ? at * 32 + lane : ~0u);
+    float p = 0.f;
+#pragma unroll
+    for (int j = 0; j < PER; j++)
+      if (j * 32 + lane == e) p = v[j], key[j] = 0;
+    p = __shfl_sync(~0u, p, e & 31) / sum;
+    total += p;
+    if (lane == 0) {
+      L.chosen[t * a.top + r] = (uint16_t)e;
+      if (tell) a.e.ids[t * a.top + r] = (int)e, a.e.weights[t * a.top + r] = p;
+    }
+  }
+  if (tell && a.e.renormalize) {
+    __syncwarp();
+    for (int r = lane; r < a.top; r += 32) a.e.weights[t * a.top + r] /= total;
+  }
+}
 
 // Choose the experts of every token (every CTA does all of them: a barrier
 // would cost more) and list the slots of every expert.
-__device__ void route(const LayerArgs& a, int* chosen /* [slots] */, Lists& L, int* scratch) {
+template <int NT>
+__device__ __forceinline__ void route(const LayerArgs& a, Lists& L, int* scratch) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = (a.experts + 31) / 32;
   for (int t = warp; t < a.tokens; t += kWarps) {
-    const float* l = a.logits + (int64_t)t * a.experts;
-    float top = -INFINITY, sum = 0.f;
-    for (int j = 0; j < per; j++)
-      if (j * 32 + lane < a.experts) top = fmaxf(top, __ldcg(l + j * 32 + lane));
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    for (int j = 0; j < per; j++)
-      if (j * 32 + lane < a.experts) sum += expf(__ldcg(l + j * 32 + lane) - top);
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    uint32_t taken = 0;  // bit j: expert j * 32 + lane (at most 1024 experts)
-    float total = 0.f;
-    for (int r = 0; r < a.top; r++) {
-      unsigned long long best = 0;
-      for (int j = 0; j < per; j++) {
-        const int e = j * 32 + lane;
-        if (e >= a.experts || (taken >> j & 1)) continue;
-        const float f = __ldcg(l + e) + 0.f;  // -0 and 0 are equal
-        uint32_t u = __float_as_uint(f);
-        u = f != f ? 0xffffffffu : (u & 0x80000000u) ? ~u : u | 0x80000000u;  // NaN above all, as in a sort
-        best = max(best, (unsigned long long)u << 32 | (0xffffffffu - e));
-      }
-      for (int o = 16; o; o >>= 1) best = max(best, __shfl_xor_sync(~0u, best, o));
-      const int e = (int)(0xffffffffu - (uint32_t)best);
-      if ((e & 31) == lane) taken |= 1u << (e >> 5);
-      const float p = expf(__ldcg(l + e) - top) / sum;
-      total += p;
-      if (lane == 0) {
-        chosen[t * a.top + r] = e;
-        if (blockIdx.x == 0) a.e.ids[t * a.top + r] = e, a.e.weights[t * a.top + r] = p;
-      }
-    }
-    if (a.e.renormalize && blockIdx.x == 0) {
-      __syncwarp();
-      for (int r = lane; r < a.top; r += 32) a.e.weights[t * a.top + r] /= total;
-    }
+    if (a.experts <= 64)
+      choose<2>(a, t, L);
+    else if (a.experts <= 256)
+      choose<8>(a, t, L);
+    else
+      choose<32>(a, t, L);
   }
   __syncthreads();
-  // slots of each expert in order: count, scan, place
   const int slots = a.tokens * a.top;
   for (int e = warp; e < a.experts; e += kWarps) {
     int n = 0;
-    for (int s = 0; s < slots; s += 32) n += __popc(__ballot_sync(~0u, s + lane < slots && chosen[s + lane] == e));
+    for (int s = 0; s < slots; s += 32) n += __popc(__ballot_sync(~0u, s + lane < slots && L.chosen[s + lane] == e));
     if (lane == 0) scratch[e] = n;
   }
   __syncthreads();
   if (warp == 0) {
-    int at = 0, act = 0;
+    int at = 0, units = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const int e = e0 + lane, n = e < a.experts ? scratch[e] : 0;
-      int x = n;
+      const int e = e0 + lane, n = e < a.experts ? scratch[e] : 0, u = (n + 8 * NT - 1) / (8 * NT);
+      int x = n, y = u;
+#pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(~0u, x, o);
-        if (lane >= o) x += y;
+        const int p = __shfl_up_sync(~0u, x, o), q = __shfl_up_sync(~0u, y, o);
+        if (lane >= o) x += p, y += q;
       }
       if (e < a.experts) L.first[e] = at + x - n;
-      const unsigned on = __ballot_sync(~0u, n > 0);
-      if (n > 0) L.active[act + __popc(on & ((1u << lane) - 1))] = e;
-      act += __popc(on);
-      at += __shfl_sync(~0u, x, 31);
+      for (int k = 0; k < u; k++) {
+        L.unit_expert[units + y - u + k] = (uint16_t)e;
+        L.unit_first[units + y - u + k] = (uint16_t)(at + x - n + k * 8 * NT);
+      }
+      at += __shfl_sync(~0u, x, 31), units += __shfl_sync(~0u, y, 31);
     }
-    if (lane == 0) L.first[a.experts] = at, scratch[0] = act;
+    if (lane == 0) L.first[a.experts] = at, L.units = units;
   }
   __syncthreads();
-  L.n_active = scratch[0];
   for (int e = warp; e < a.experts; e += kWarps) {
     int at = L.first[e];
     if (L.first[e + 1] == at) continue;
     for (int s = 0; s < slots; s += 32) {
-      const bool on = s + lane < slots && chosen[s + lane] == e;
+      const bool on = s + lane < slots && L.chosen[s + lane] == e;
       const unsigned m = __ballot_sync(~0u, on);
-      if (on) L.slots[at + __popc(m & ((1u << lane) - 1))] = s + lane;
+      if (on) L.slots[at + __popc(m & ((1u << lane) - 1))] = (uint16_t)(s + lane);
       at += __popc(m);
     }
   }
   __syncthreads();
 }
 
-// W: the weights' type, M: the products' type, VEC: rows are whole 16-byte
-// vectors, NT: column tiles of 8 tokens that a product takes at a time.
-template <typename W, typename X, typename M, bool VEC, int NT>
-__global__ void __launch_bounds__(kThreads, 1) layer_kernel(const LayerArgs a) {
-  using S = Step<W, M>;
-  constexpr bool kScaled = sizeof(W) == 1;
-  constexpr int kBlock = kScaled ? 128 : S::kK;  // k that share a scale
-  __shared__ int chosen[kMaxSlots];
-  __shared__ int slot_list[kMaxSlots];
-  __shared__ int first[kMaxExperts + 1], active[kMaxExperts], scratch[kMaxExperts];
-  extern __shared__ __align__(16) float red[];  // [kWarps][NT][32][4]
+// Sums over the warp of 32 values a lane: lane l ends with the sum of value l.
+__device__ __forceinline__ float transpose_sum(float* v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 16; o; o >>= 1)
+#pragma unroll
+    for (int j = 0; j < o; j++) {
+      const bool up = lane & o;
+      const float give = up ? v[j] : v[j + o], keep = up ? v[j + o] : v[j];
+      v[j] = keep + __shfl_xor_sync(~0u, give, o);
+    }
+  return v[0];
+}
+
+// Router products: a CTA takes RE experts and up to 8 tokens.
+template <typename X, bool VEC, int RE>
+__device__ __forceinline__ void router(const LayerArgs& a, float* red) {
+  static_assert(RE * kGroup <= 32, "");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, q = lane & 3;  // row (and token) of the lane, quarter of k
-  cg::grid_group grid = cg::this_grid();
-
-  // ---- router: a CTA takes one expert and up to 8 tokens
-  {
-    const int groups = (a.tokens + kGroup - 1) / kGroup;
-    for (int u = blockIdx.x; u < a.experts * groups; u += gridDim.x) {
-      const int e = u % a.experts, t0 = u / a.experts * kGroup, nt = min(kGroup, a.tokens - t0);
-      float acc[kGroup] = {};
-      const X* r = (const X*)a.e.router + (int64_t)e * a.h;
-      const X* x = (const X*)a.e.x + (int64_t)t0 * a.e.ldx;
-      for (int k = threadIdx.x * 8; k < a.h; k += kThreads * 8) {
-        const uint4 rv = row16<X, VEC>(r, k, a.h, true);
-        const X* re = reinterpret_cast<const X*>(&rv);
+  const int groups = (a.tokens + kGroup - 1) / kGroup, es = (a.experts + RE - 1) / RE;
+  for (int u = blockIdx.x; u < es * groups; u += gridDim.x) {
+    const int e0 = u % es * RE, t0 = u / es * kGroup, nt = min(kGroup, a.tokens - t0), ne = min(RE, a.experts - e0);
+    float acc[32] = {};
+    const X* r = (const X*)a.e.router + (int64_t)e0 * a.h;
+    const X* x = (const X*)a.e.x + (int64_t)t0 * a.e.ldx;
+    for (int k = threadIdx.x * 8; k < a.h; k += kThreads * 8) {
+      uint4 rv[RE], xv[kGroup];
 #pragma unroll
-        for (int t = 0; t < kGroup; t++) {
-          const uint4 xv = row16<X, VEC>(x + t * a.e.ldx, k, a.h, t < nt);
-          const X* xe = reinterpret_cast<const X*>(&xv);
+      for (int j = 0; j < RE; j++) rv[j] = row16<X, VEC>(r + (int64_t)j * a.h, k, a.h, j < ne);
 #pragma unroll
-          for (int j = 0; j < 8; j++) acc[t] = fmaf(to_f32<X>(re[j]), to_f32<X>(xe[j]), acc[t]);
+      for (int t = 0; t < kGroup; t++) xv[t] = row16<X, VEC>(x + t * a.e.ldx, k, a.h, t < nt);
+#pragma unroll
+      for (int t = 0; t < kGroup; t++) {
+        if (t >= nt) break;
+        const X* xe = reinterpret_cast<const X*>(&xv[t]);
+#pragma unroll
+        for (int j = 0; j < RE; j++) {
+          const X* re = reinterpret_cast<const X*>(&rv[j]);
+#pragma unroll
+          for (int c = 0; c < 8; c++) acc[j * kGroup + t] = fmaf(to_f32<X>(re[c]), to_f32<X>(xe[c]), acc[j * kGroup + t]);
         }
-      }
-#pragma unroll
-      for (int t = 0; t < kGroup; t++)
-#pragma unroll
-        for (int o = 16; o; o >>= 1) acc[t] += __shfl_xor_sync(~0u, acc[t], o);
-      if (lane == 0)
-#pragma unroll
-        for (int t = 0; t < kGroup; t++) red[warp * kGroup + t] = acc[t];
-      __syncthreads();
-      if (threadIdx.x < nt) {
-        float s = 0.f;
-        for (int w = 0; w < kWarps; w++) s += red[w * kGroup + threadIdx.x];
-        a.logits[(int64_t)(t0 + threadIdx.x) * a.experts + e] = s;
-      }
-      __syncthreads();
-    }
-    for (int s = blockIdx.x * kThreads + threadIdx.x; s < a.tokens * a.top; s += gridDim.x * kThreads) a.bmax[s] = 0;
-  }
-  grid.sync();
-  Lists L{slot_list, first, active, 0};
-  route(a, chosen, L, scratch);
-
-  // ---- first product: tasks of 8 outputs (their gate and up rows) of one expert
-  {
-    const int tiles = (a.i + 7) / 8, blocks = (a.h + kBlock - 1) / kBlock;
-    const int kb0 = blocks * warp / kWarps, kb1 = blocks * (warp + 1) / kWarps;
-    for (int task = blockIdx.x; task < L.n_active * tiles; task += gridDim.x) {
-      const int e = L.active[task / tiles], i0 = task % tiles * 8;
-      const bool on = i0 + g < a.i;
-      const int ra = i0 + g, rb = a.i + i0 + g;
-      const W* wa = (const W*)a.e.w_in + ((int64_t)e * 2 * a.i + (on ? ra : 0)) * a.h;
-      const W* wb = (const W*)a.e.w_in + ((int64_t)e * 2 * a.i + (on ? rb : 0)) * a.h;
-      const int hb = (a.h + 127) / 128, rbs = (2 * a.i + 127) / 128;
-      const float* sa = kScaled ? a.e.in_scales + ((int64_t)e * rbs + (on ? ra : 0) / 128) * hb : nullptr;
-      const float* sb = kScaled ? a.e.in_scales + ((int64_t)e * rbs + (on ? rb : 0) / 128) * hb : nullptr;
-      for (int n0 = L.first[e]; n0 < L.first[e + 1]; n0 += NT * 8) {
-        const int n = min(NT * 8, L.first[e + 1] - n0);
-        const X* xr[NT];
-#pragma unroll
-        for (int j = 0; j < NT; j++) xr[j] = (const X*)a.e.x + (int64_t)(j * 8 + g < n ? L.slots[n0 + j * 8 + g] / a.top : 0) * a.e.ldx;
-        float acc[NT][4] = {};
-        for (int kb = kb0; kb < kb1; kb++) {
-          float part[NT][4] = {};
-#pragma unroll
-          for (int st = 0; st < kBlock / S::kK; st++) {
-            const int k = kb * kBlock + st * S::kK + q * S::kPerLane;
-            uint32_t pa[S::kPairs], pb[S::kPairs];
-            S::pairs(row16<W, VEC>(wa, k, a.h, on), pa);
-            S::pairs(row16<W, VEC>(wb, k, a.h, on), pb);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-              if (j * 8 >= n) break;
-              alignas(16) uint32_t px[S::kPairs];
-#pragma unroll
-              for (int v = 0; v < S::kPairs / 4; v++)
-                *reinterpret_cast<uint4*>(px + 4 * v) = row16<X, VEC>(xr[j], k + 8 * v, a.h, j * 8 + g < n);
-#pragma unroll
-              for (int v = 0; v < S::kPairs; v += 2) mma<M>(kScaled ? part[j] : acc[j], pa[v], pb[v], pa[v + 1], pb[v + 1], px[v], px[v + 1]);
-            }
-          }
-          if (kScaled) {
-            const float fa = sa[kb], fb = sb[kb];
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-              acc[j][0] = fmaf(part[j][0], fa, acc[j][0]), acc[j][1] = fmaf(part[j][1], fa, acc[j][1]);
-              acc[j][2] = fmaf(part[j][2], fb, acc[j][2]), acc[j][3] = fmaf(part[j][3], fb, acc[j][3]);
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-          *reinterpret_cast<float4*>(red + ((warp * NT + j) * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
-        __syncthreads();
-        // accumulator (row g: gate; row g + 8: up; columns 2 q, 2 q + 1) of column tile j
-        for (int o = threadIdx.x; o < NT * 64; o += kThreads) {
-          const int j = o >> 6, ln = o >> 1 & 31, half = o & 1;
-          const int col = j * 8 + (ln & 3) * 2 + half, row = i0 + (ln >> 2);
-          float ga = 0.f, up = 0.f;
-          for (int w = 0; w < kWarps; w++) {
-            const float* p = red + ((w * NT + j) * 32 + ln) * 4 + half;
-            ga += p[0], up += p[2];
-          }
-          if (col < n && row < a.i) {
-            const int slot = L.slots[n0 + col];
-            const float v = ga / (1.f + expf(-ga)) * up;
-            a.b[(int64_t)slot * a.i + row] = v;
-            if (std::is_same_v<M, __half>) atomicMax(a.bmax + slot, __float_as_uint(fabsf(v)));
-          }
-        }
-        __syncthreads();
       }
     }
-  }
-  grid.sync();
-
-  // ---- second product: tasks of 16 rows of one expert
-  {
-    const int tiles = (a.h + 15) / 16, blocks = (a.i + kBlock - 1) / kBlock;
-    const int kb0 = blocks * warp / kWarps, kb1 = blocks * (warp + 1) / kWarps;
-    for (int task = blockIdx.x; task < L.n_active * tiles; task += gridDim.x) {
-      const int e = L.active[task / tiles], r0 = task % tiles * 16;
-      const bool ona = r0 + g < a.h, onb = r0 + g + 8 < a.h;
-      const int ra = ona ? r0 + g : 0, rb = onb ? r0 + g + 8 : 0;
-      const W* wa = (const W*)a.e.w_out + ((int64_t)e * a.h + ra) * a.i;
-      const W* wb = (const W*)a.e.w_out + ((int64_t)e * a.h + rb) * a.i;
-      const int ib = (a.i + 127) / 128, rbs = (a.h + 127) / 128;
-      const float* sa = kScaled ? a.e.out_scales + ((int64_t)e * rbs + ra / 128) * ib : nullptr;
-      const float* sb = kScaled ? a.e.out_scales + ((int64_t)e * rbs + rb / 128) * ib : nullptr;
-      for (int n0 = L.first[e]; n0 < L.first[e + 1]; n0 += NT * 8) {
-        const int n = min(NT * 8, L.first[e + 1] - n0);
-        const float* br[NT];
-        float up[NT], down[NT][2];
+    red[warp * 32 + lane] = transpose_sum(acc);
+    __syncthreads();
+    if (warp == 0) {
+      float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-          const int slot = L.slots[n0 + min(j * 8 + g, n - 1)];
-          br[j] = a.b + (int64_t)slot * a.i;
-          up[j] = 1.f, down[j][0] = down[j][1] = 1.f;
-          if constexpr (std::is_same_v<M, __half>) {
-            // 2^-x of the slot's largest value, and back for the lane's two result columns
-            auto power = [&](int s, bool inverse) {
-              const int ex = (int)(__ldcg(a.bmax + s) >> 23) - 127;
-              const int c = ex < -100 || ex > 127 ? 0 : min(ex, 126);  // tiny, infinite or NaN: as it is
-              return __uint_as_float((uint32_t)(127 + (inverse ? c : -c)) << 23);
-            };
-            up[j] = power(slot, false);
-            for (int c = 0; c < 2; c++) down[j][c] = power(L.slots[n0 + min(j * 8 + 2 * q + c, n - 1)], true);
-          }
-        }
-        float acc[NT][4] = {};
-        for (int kb = kb0; kb < kb1; kb++) {
-          float part[NT][4] = {};
-#pragma unroll
-          for (int st = 0; st < kBlock / S::kK; st++) {
-            const int k = kb * kBlock + st * S::kK + q * S::kPerLane;
-            uint32_t pa[S::kPairs], pb[S::kPairs];
-            S::pairs(row16<W, VEC>(wa, k, a.i, ona), pa);
-            S::pairs(row16<W, VEC>(wb, k, a.i, onb), pb);
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-              if (j * 8 >= n) break;
-#pragma unroll
-              for (int v = 0; v < S::kPairs; v += 2) {
-                uint32_t hi[2], lo[2];
-#pragma unroll
-                for (int p = 0; p < 2; p++) {
-                  const int kk = k + 2 * (v + p);
-                  float f0 = 0.f, f1 = 0.f;
-                  if (j * 8 + g < n) {
-                    if (kk < a.i) f0 = __ldcg(br[j] + kk) * up[j];
-                    if (kk + 1 < a.i) f1 = __ldcg(br[j] + kk + 1) * up[j];
-                  }
-                  hi[p] = pack2<M>(f0, f1);
-                  const float2 h = unpack2<M>(hi[p]);
-                  // (an infinite high part stands alone: no inf - inf)
-                  lo[p] = pack2<M>(isinf(h.x) ? 0.f : f0 - h.x, isinf(h.y) ? 0.f : f1 - h.y);
-                }
-                mma<M>(kScaled ? part[j] : acc[j], pa[v], pb[v], pa[v + 1], pb[v + 1], hi[0], hi[1]);
-                mma<M>(kScaled ? part[j] : acc[j], pa[v], pb[v], pa[v + 1], pb[v + 1], lo[0], lo[1]);
-              }
-            }
-          }
-          if (kScaled) {
-            const float fa = sa[kb], fb = sb[kb];
-#pragma unroll
-            for (int j = 0; j < NT; j++) {
-              acc[j][0] = fmaf(part[j][0], fa, acc[j][0]), acc[j][1] = fmaf(part[j][1], fa, acc[j][1]);
-              acc[j][2] = fmaf(part[j][2], fb, acc[j][2]), acc[j][3] = fmaf(part[j][3], fb, acc[j][3]);
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-          *reinterpret_cast<float4*>(red + ((warp * NT + j) * 32 + lane) * 4) =
-              make_float4(acc[j][0] * down[j][0], acc[j][1] * down[j][1], acc[j][2] * down[j][0], acc[j][3] * down[j][1]);
-        __syncthreads();
-        for (int o = threadIdx.x; o < NT * 128; o += kThreads) {
-          const int j = o >> 7, c = o >> 5 & 3, ln = o & 31;
-          const int col = j * 8 + (ln & 3) * 2 + (c & 1), row = r0 + (ln >> 2) + (c & 2) * 4;
-          float s = 0.f;
-          for (int w = 0; w < kWarps; w++) s += red[((w * NT + j) * 32 + ln) * 4 + c];
-          if (col < n && row < a.h) a.o[(int64_t)L.slots[n0 + col] * a.h + row] = s;
-        }
-        __syncthreads();
-      }
+      for (int w = 0; w < kWarps; w++) s += red[w * 32 + lane];
+      const int j = lane / kGroup, t = lane % kGroup;
+      if (j < ne && t < nt) a.logits[(int64_t)(t0 + t) * a.experts + e0 + j] = s;
     }
-  }
-  grid.sync();
-
-  // ---- the tokens' sums over their experts, in the order of choice
-  for (int64_t u = blockIdx.x * (int64_t)kThreads + threadIdx.x; u < (int64_t)a.tokens * a.h; u += (int64_t)gridDim.x * kThreads) {
-    const int t = (int)(u / a.h), c = (int)(u - (int64_t)t * a.h);
-    float s = 0.f;
-    for (int r = 0; r < a.top; r++) s += __ldcg(a.e.weights + t * a.top + r) * __ldcg(a.o + ((int64_t)t * a.top + r) * a.h + c);
-    ((X*)a.e.y)[(int64_t)t * a.e.ldy + c] = from_f32<X>(s);
+    __syncthreads();
   }
 }
 
-template <typename W, typename X, typename M, bool VEC, int NT>
+// W: the weights' type, M: x's and the products' type, VEC: rows are whole
+// 16-byte vectors, NT: column tiles of 8 tokens that a product takes at a time.
+template <typename W, typename M, bool VEC, int NT>
+struct Layer {
+  using S = Step<W, M>;
+  static constexpr bool kScaled = sizeof(W) == 1;
+  static constexpr bool kHalf = std::is_same_v<M, __half>;
+  static constexpr int kRing = NT == 1 ? 8 : 6;          // steps in flight
+  static constexpr int kSlot = 2 * 512 + (kScaled ? 256 : 0);  // bytes of a warp's step: two rows, two scales a lane
+  static constexpr int kRed = kWarps * NT * 128;         // floats of a task's parts
+  static constexpr size_t kSmem = (size_t)kWarps * kRing * kSlot + 2 * kRed * 4;
+
+  // Where a lane's weights of a task are.  product 0: outputs 8 tile + g, their
+  // gate and up rows of w_in; product 1: rows 16 tile + g and + 8 of w_out.
+  struct Rows {
+    const W *a, *b;
+    const float *sa, *sb;
+    bool ona, onb;
+  };
+  __device__ static __forceinline__ Rows rows(const LayerArgs& a, int product, int expert, int tile, int g) {
+    Rows r;
+    const int ra = product == 0 ? tile * 8 + g : tile * 16 + g;
+    r.ona = ra < (product == 0 ? a.i : a.h);
+    r.onb = product == 0 ? r.ona : ra + 8 < a.h;
+    const int rb = !r.onb ? 0 : product == 0 ? a.i + ra : ra + 8;
+    const int qa = r.ona ? ra : 0;
+    const int64_t n = product == 0 ? 2 * a.i : a.h, k = product == 0 ? a.h : a.i;
+    const W* w = (const W*)(product == 0 ? a.e.w_in : a.e.w_out) + expert * n * k;
+    r.a = w + qa * k, r.b = w + rb * k;
+    if (kScaled) {
+      const int64_t kb = (k + 127) / 128;
+      const float* s = (product == 0 ? a.e.in_scales : a.e.out_scales) + expert * ((n + 127) / 128) * kb;
+      r.sa = s + qa / 128 * kb, r.sb = s + rb / 128 * kb;
+    }
+    return r;
+  }
+
+  // The stream of steps that a warp copies ahead of their use.
+  struct Feed {
+    int product, task, step, slot;
+    Rows r;
+  };
+
+  __device__ static void run(const LayerArgs& a, Lists& L, int* scratch, unsigned char* dyn) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, q = lane & 3;  // row (and token) of the lane, quarter of k
+    unsigned char* ring = dyn + (size_t)warp * kRing * kSlot;
+    float* red = reinterpret_cast<float*>(dyn + (size_t)kWarps * kRing * kSlot);
+    cg::grid_group grid = cg::this_grid();
+
+    if (a.tokens <= 8)
+      router<M, VEC, 1>(a, red);
+    else
+      router<M, VEC, 4>(a, red);
+    const int tiles0 = (a.i + 7) / 8, tiles1 = (a.h + 15) / 16;
+    for (int s = blockIdx.x * kThreads + threadIdx.x; s < max(a.tokens * a.top, tiles1); s += gridDim.x * kThreads) {
+      if (s < a.tokens * a.top) a.bmax[s] = 0;
+      if (s < tiles1) a.done[s] = 0;
+    }
+    grid.sync();
+    route<NT>(a, L, scratch);
+
+    // this warp's steps of k in each product, and the tasks
+    const int steps0 = (a.h + S::kK - 1) / S::kK, steps1 = (a.i + S::kK - 1) / S::kK;
+    const int lo0 = steps0 * warp / kWarps, hi0 = steps0 * (warp + 1) / kWarps;
+    const int lo1 = steps1 * warp / kWarps, hi1 = steps1 * (warp + 1) / kWarps;
+    const int tasks0 = L.units * tiles0, tasks1 = L.units * tiles1;
+
+    Feed f{0, (int)blockIdx.x, lo0, 0, {}};
+    auto settle = [&] {  // onto the next task that has steps for this warp
+      if (f.product == 0 && (f.task >= tasks0 || lo0 == hi0)) f.product = 1, f.task = blockIdx.x, f.step = lo1;
+      if (f.product == 1 && (f.task >= tasks1 || lo1 == hi1)) f.product = 2;
+      if (f.product < 2) {
+        const int tiles = f.product == 0 ? tiles0 : tiles1;
+        const int u = f.task / tiles;
+        f.r = rows(a, f.product, L.unit_expert[u], f.task - u * tiles, g);
+      }
+    };
+    auto feed = [&] {  // copy the next step; an empty group at the end of the stream
+      if (f.product < 2) {
+        unsigned char* at = ring + f.slot * kSlot + lane * 16;
+        const int n = f.product == 0 ? a.h : a.i, k = f.step * S::kK + q * S::kPerLane;
+        copy16<W, VEC>(at, f.r.a, k, n, f.r.ona);
+        copy16<W, VEC>(at + 512, f.r.b, k, n, f.r.onb);
+        if (kScaled) {
+          const int kb = f.step * S::kK / 128;
+          const uint32_t sc = smem_u32(ring + f.slot * kSlot + 1024 + lane * 8);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc), "l"(f.r.sa + kb) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 4), "l"(f.r.sb + kb) : "memory");
+        }
+        if (++f.slot == kRing) f.slot = 0;
+        if (++f.step == (f.product == 0 ? hi0 : hi1)) {
+          f.task += gridDim.x, f.step = f.product == 0 ? lo0 : lo1;
+          settle();
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    settle();
+    for (int p = 0; p < kRing - 1; p++) feed();
+    int slot = 0, parity = 0;
+    // take the oldest step: its two rows' pairs and scales
+    auto take = [&](uint32_t* pa, uint32_t* pb, float& fa, float& fb) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      const unsigned char* at = ring + slot * kSlot;
+      S::pairs(*reinterpret_cast<const uint4*>(at + lane * 16), pa);
+      S::pairs(*reinterpret_cast<const uint4*>(at + 512 + lane * 16), pb);
+      if (kScaled) {
+        const float2 sc = *reinterpret_cast<const float2*>(at + 1024 + lane * 8);
+        fa = sc.x, fb = sc.y;
+      }
+      if (++slot == kRing) slot = 0;
+      feed();
+    };
+    auto add_scaled = [&](float* acc, const float* part, float fa, float fb) {
+      acc[0] = fmaf(part[0], fa, acc[0]), acc[1] = fmaf(part[1], fa, acc[1]);
+      acc[2] = fmaf(part[2], fb, acc[2]), acc[3] = fmaf(part[3], fb, acc[3]);
+    };
+    auto park = [&](float (*acc)[4]) {  // this warp's part of the task, for the warps that finish it
+      float* at = red + parity * kRed;
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+        *reinterpret_cast<float4*>(at + ((warp * NT + j) * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+      __syncthreads();  // one barrier a task: the parts alternate between two buffers
+      parity ^= 1;
+      return at;
+    };
+
+    // ---- first product: tasks of 8 outputs of one expert
+    for (int task = blockIdx.x; task < tasks0; task += gridDim.x) {
+      const int u = task / tiles0, i0 = (task - u * tiles0) * 8;
+      const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(NT * 8, L.first[e + 1] - n0);
+      const M* xr[NT];
+#pragma unroll
+      for (int j = 0; j < NT; j++) xr[j] = (const M*)a.e.x + (int64_t)(j * 8 + g < n ? L.slots[n0 + j * 8 + g] / a.top : 0) * a.e.ldx;
+      float acc[NT][4] = {};
+      for (int s = lo0; s < hi0; s++) {
+        const int k = s * S::kK + q * S::kPerLane;
+        uint32_t pa[S::kPairs], pb[S::kPairs];
+        float fa, fb;
+        alignas(16) uint32_t px[NT][S::kPairs];
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+          if (j * 8 < n)
+#pragma unroll
+            for (int v = 0; v < S::kPairs / 4; v++)
+              *reinterpret_cast<uint4*>(px[j] + 4 * v) = row16<M, VEC>(xr[j], k + 8 * v, a.h, j * 8 + g < n);
+        take(pa, pb, fa, fb);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          if (j * 8 >= n) break;
+          float part[4] = {};
+          float* to = kScaled ? part : acc[j];
+#pragma unroll
+          for (int v = 0; v < S::kPairs; v += 2) mma<M>(to, pa[v], pb[v], pa[v + 1], pb[v + 1], px[j][v], px[j][v + 1]);
+          if (kScaled) add_scaled(acc[j], part, fa, fb);
+        }
+      }
+      const float* parts = park(acc);
+      // accumulator (row g: gate; row g + 8: up; columns 2 q, 2 q + 1) of column tile j
+      const int turn = (warp + kWarps - (task / gridDim.x * 2 * NT) % kWarps) % kWarps;  // which warps finish goes round
+      if (turn < 2 * NT) {
+        const int o = turn * 32 + lane, j = o >> 6, ln = o >> 1 & 31, half = o & 1;
+        const int col = j * 8 + (ln & 3) * 2 + half, row = i0 + (ln >> 2);
+        if (col < n) {
+          float ga = 0.f, up = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; w++) {
+            const float* p = parts + ((w * NT + j) * 32 + ln) * 4 + half;
+            ga += p[0], up += p[2];
+          }
+          const int64_t slot_row = L.slots[n0 + col];
+          const float v = ga / (1.f + expf(-ga)) * up;  // rows past i: 0, the padding of b
+          if constexpr (kHalf) {
+            ((float*)a.b)[slot_row * a.ip + row] = v;
+            atomicMax(a.bmax + slot_row, __float_as_uint(fabsf(v)));
+          } else {
+            const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+            const float hf = __bfloat162float(hi);
+            __nv_bfloat16* p = (__nv_bfloat16*)a.b + slot_row * 2 * a.ip + row;
+            p[0] = hi;
+            p[a.ip] = __float2bfloat16_rn(isinf(hf) ? 0.f : v - hf);  // an infinite high part stands alone
+          }
+        }
+      }
+    }
+    grid.sync();
+
+    // ---- second product: tasks of 16 rows of one expert
+    for (int task = blockIdx.x; task < tasks1; task += gridDim.x) {
+      const int u = task / tiles1, tile = task - u * tiles1, r0 = tile * 16;
+      const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(NT * 8, L.first[e + 1] - n0);
+      const char* br[NT];
+      float down[NT][2], up[NT];
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        const int sl = L.slots[n0 + min(j * 8 + g, n - 1)];
+        br[j] = (const char*)a.b + (int64_t)sl * a.ip * 4;
+        if constexpr (kHalf) {
+          // 2^-x of the slot's largest value, and back for the lane's two result columns
+          auto power = [&](int at, int sign) {
+            const int ex = (int)(a.bmax[at] >> 23) - 127;
+            const int c = ex < -100 || ex > 127 ? 0 : min(ex, 126);  // tiny, infinite or NaN: as it is
+            return __uint_as_float((uint32_t)(127 + sign * c) << 23);
+          };
+          up[j] = power(sl, -1);
+          for (int c = 0; c < 2; c++) down[j][c] = power(L.slots[n0 + min(j * 8 + 2 * q + c, n - 1)], 1);
+        }
+      }
+      float acc[NT][4] = {};
+      for (int s = lo1; s < hi1; s++) {
+        const int k = s * S::kK + q * S::kPerLane;
+        uint32_t pa[S::kPairs], pb[S::kPairs];
+        float fa, fb;
+        alignas(16) uint32_t hi[NT][S::kPairs], lo[NT][S::kPairs];
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          if (j * 8 >= n) break;
+#pragma unroll
+          for (int v = 0; v < S::kPairs / 4; v++) {
+            const int kk = k + 8 * v;
+            const bool on = j * 8 + g < n && kk < a.ip;
+            const uint4 zero = make_uint4(0, 0, 0, 0);
+            if constexpr (kHalf) {
+              const float4* p = reinterpret_cast<const float4*>((const float*)br[j] + kk);
+              const float4 f0 = on ? p[0] : make_float4(0, 0, 0, 0), f1 = on ? p[1] : make_float4(0, 0, 0, 0);
+              const float x[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
+#pragma unroll
+              for (int c = 0; c < 4; c++) {
+                const float y0 = x[2 * c] * up[j], y1 = x[2 * c + 1] * up[j];
+                hi[j][4 * v + c] = pack2<M>(y0, y1);
+                const float2 hf = unpack2<M>(hi[j][4 * v + c]);
+                // (an infinite high part stands alone: no inf - inf)
+                lo[j][4 * v + c] = pack2<M>(isinf(hf.x) ? 0.f : y0 - hf.x, isinf(hf.y) ? 0.f : y1 - hf.y);
+              }
+            } else {
+              const __nv_bfloat16* p = (const __nv_bfloat16*)br[j] + kk;
+              *reinterpret_cast<uint4*>(hi[j] + 4 * v) = on ? *reinterpret_cast<const uint4*>(p) : zero;
+              *reinterpret_cast<uint4*>(lo[j] + 4 * v) = on ? *reinterpret_cast<const uint4*>(p + a.ip) : zero;
+            }
+          }
+        }
+        take(pa, pb, fa, fb);
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          if (j * 8 >= n) break;
+          float part[4] = {};
+          float* to = kScaled ? part : acc[j];
+#pragma unroll
+          for (int v = 0; v < S::kPairs; v += 2) {
+            mma<M>(to, pa[v], pb[v], pa[v + 1], pb[v + 1], hi[j][v], hi[j][v + 1]);
+            mma<M>(to, pa[v], pb[v], pa[v + 1], pb[v + 1], lo[j][v], lo[j][v + 1]);
+          }
+          if (kScaled) add_scaled(acc[j], part, fa, fb);
+        }
+      }
+      if constexpr (kHalf) {
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+          for (int c = 0; c < 4; c++) acc[j][c] *= down[j][c & 1];
+      }
+      const float* parts = park(acc);
+      const int turn = (warp + kWarps - (task / gridDim.x * 4) % kWarps) % kWarps;
+      if (turn >= 4) continue;
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        const int col = j * 8 + (lane & 3) * 2 + (turn & 1), row = r0 + (lane >> 2) + (turn & 2) * 4;
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; w++) s += parts[((w * NT + j) * 32 + lane) * 4 + turn];
+        if (col < n && row < a.h) a.o[(int64_t)L.slots[n0 + col] * a.h + row] = s;
+      }
+      if (NT == 1) {
+        // the warp that finishes a row tile's last part (of 4 a unit) sums the tokens' experts there
+        __threadfence();
+        __syncwarp();
+        unsigned before = 0;
+        if (lane == 0) before = atomicAdd(a.done + tile, 1u);
+        before = __shfl_sync(~0u, before, 0);
+        if (before == 4u * L.units - 1) {
+          __threadfence();
+          for (int c = lane; c < a.tokens * 16; c += 32) combine(a, c >> 4, r0 + (c & 15));
+        }
+      }
+    }
+    if (NT > 1) {
+      grid.sync();
+      const int64_t all = (int64_t)a.tokens * a.h;
+      for (int64_t c = blockIdx.x * (int64_t)kThreads + threadIdx.x; c < all; c += (int64_t)gridDim.x * kThreads) {
+        const int t = (int)(c / a.h);
+        combine(a, t, (int)(c - (int64_t)t * a.h));
+      }
+    }
+  }
+
+  // A token's sum over its experts, in the order of choice.
+  __device__ static __forceinline__ void combine(const LayerArgs& a, int t, int row) {
+    if (row >= a.h) return;
+    float s = 0.f;
+#pragma unroll 4
+    for (int r = 0; r < a.top; r++) s += __ldcg(a.e.weights + t * a.top + r) * __ldcg(a.o + ((int64_t)t * a.top + r) * a.h + row);
+    ((M*)a.e.y)[(int64_t)t * a.e.ldy + row] = from_f32<M>(s);
+  }
+};
+
+template <typename W, typename M, bool VEC, int NT>
+__global__ void __launch_bounds__(kThreads, 1) layer_kernel(const LayerArgs a) {
+  __shared__ Lists lists;
+  __shared__ int scratch[kMaxExperts];
+  extern __shared__ __align__(16) unsigned char dyn[];
+  Layer<W, M, VEC, NT>::run(a, lists, scratch, dyn);
+}
+
+template <typename W, typename M, bool VEC, int NT>
 void launch(LayerArgs& a, cudaStream_t s) {
-  auto kern = layer_kernel<W, X, M, VEC, NT>;
-  const size_t smem = (size_t)kWarps * NT * 32 * 16;
+  auto kern = layer_kernel<W, M, VEC, NT>;
+  constexpr size_t smem = Layer<W, M, VEC, NT>::kSmem;
   ensure_dynamic_smem((const void*)kern, smem);
   void* args[] = {&a};
   NDT_CUDA(cudaLaunchCooperativeKernel((const void*)kern, dim3((unsigned)ctx().sm_count), dim3(kThreads), args, smem, s));
@@ -455,34 +647,36 @@ void launch(LayerArgs& a, cudaStream_t s) {
 
 void expert_layer(const ExpertArgs& e, cudaStream_t s) {
   if (e.tokens == 0 || e.h == 0) return;
-  if (e.experts > kMaxExperts) throw Error(ErrKind::InvalidArgument, "expert_layer: more than 1024 experts");
+  if (e.experts > kMaxExperts) throw Error(ErrKind::InvalidArgument, "more than 1024 experts");
   // a launch takes as many tokens as its lists hold; more tokens, more launches
   const int64_t step = std::max<int64_t>(1, std::min<int64_t>(kMaxTokens, kMaxSlots / e.top));
   const int64_t most = std::min(step, e.tokens);
-  const size_t xs = msize(e.xt);
-  Workspace ws((size_t)most * 4 * (e.experts + e.top * (e.i + e.h + 1)), s);
+  const int64_t ip = (e.i + 7) / 8 * 8;
+  const int64_t xs = msize(e.xt), ws_ = msize(e.wt);
+  // b first: its rows are read in 16-byte vectors
+  Workspace ws((size_t)4 * (most * (e.top * (ip + e.h + 1) + e.experts) + (e.h + 15) / 16), s);
   for (int64_t t0 = 0; t0 < e.tokens; t0 += step) {
     LayerArgs a{};
     a.e = e;
     a.tokens = (int)std::min(step, e.tokens - t0);
-    a.experts = (int)e.experts, a.top = (int)e.top, a.h = (int)e.h, a.i = (int)e.i;
+    a.experts = (int)e.experts, a.top = (int)e.top, a.h = (int)e.h, a.i = (int)e.i, a.ip = (int)ip;
     a.e.x = (const char*)e.x + t0 * e.ldx * xs;
     a.e.y = (char*)e.y + t0 * e.ldy * xs;
     a.e.ids = e.ids + t0 * e.top, a.e.weights = e.weights + t0 * e.top;
-    a.logits = (float*)ws.p;
-    a.b = a.logits + most * e.experts;
-    a.o = a.b + most * e.top * e.i;
-    a.bmax = (unsigned*)(a.o + most * e.top * e.h);
-    const int ws_ = msize(e.wt);
+    a.b = ws.p;
+    a.o = (float*)ws.p + most * e.top * ip;
+    a.logits = a.o + most * e.top * e.h;
+    a.bmax = (unsigned*)(a.logits + most * e.experts);
+    a.done = a.bmax + most * e.top;
     const bool vec = e.h * ws_ % 16 == 0 && e.i * ws_ % 16 == 0 && e.h % 8 == 0 && e.ldx % 8 == 0 &&
                      (((uintptr_t)a.e.x | (uintptr_t)e.router | (uintptr_t)e.w_in | (uintptr_t)e.w_out) % 16) == 0;
     auto go = [&](auto w, auto x) {
       using W = decltype(w);
-      using X = decltype(x);
+      using M = decltype(x);
       if (a.tokens <= 8)
-        vec ? launch<W, X, X, true, 1>(a, s) : launch<W, X, X, false, 1>(a, s);
+        vec ? launch<W, M, true, 1>(a, s) : launch<W, M, false, 1>(a, s);
       else
-        vec ? launch<W, X, X, true, 4>(a, s) : launch<W, X, X, false, 4>(a, s);
+        vec ? launch<W, M, true, 4>(a, s) : launch<W, M, false, 4>(a, s);
     };
     if (e.wt == MType::E4M3)
       e.xt == MType::BF16 ? go(__nv_fp8_e4m3{}, __nv_bfloat16{}) : go(__nv_fp8_e4m3{}, __half{});

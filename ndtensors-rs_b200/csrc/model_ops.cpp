@@ -24,9 +24,7 @@ int* wait_flag_device() {
     g_flag = (int*)p;
     *(volatile int*)g_flag = 0;
   }
-  void* d = nullptr;
-  NDT_CUDA(cudaHostGetDevicePointer(&d, g_flag, 0));
-  return (int*)d;
+  return g_flag;  // unified addressing: the device's pointer is the host's
 }
 bool wait_flag_raised() {
   std::lock_guard<std::mutex> lk(g_flag_mu);
@@ -108,6 +106,26 @@ void set_scales(ScaledOperand& o, const float* s, int block_rows, long rs, long 
   o.s = s, o.srs = rs, o.scs = cs, o.per_row = block_rows == 1;
 }
 
+// An 8-bit matrix in a workspace: values with rows on 16 bytes, then scales, a
+// column of them for each block of 128 along the rows (as the product reads them).
+struct Quantised {
+  MatView x;
+  int block_rows;
+  MType type;
+  int64_t ld, sld;
+  char* p = nullptr;
+  Quantised(const MatView& x_, int br, MType t)
+      : x(x_), block_rows(br), type(t), ld(up(x_.cols, 16)), sld(br == 1 ? up(x_.rows, 4) : (x_.rows + 127) / 128) {}
+  size_t bytes() const { return (size_t)(up(x.rows * ld, 256) + up((x.cols + 127) / 128 * sld * 4, 256)); }
+  void* place(void* at) {
+    p = (char*)at;
+    return p + bytes();
+  }
+  float* scales() const { return (float*)(p + up(x.rows * ld, 256)); }
+  QuantOut out() const { return QuantOut{p, ld, scales(), 1, sld}; }
+  ScaledOperand operand() const { return ScaledOperand{p, x.rows, ld, type, scales(), 1, sld, block_rows == 1}; }
+};
+
 void zero_rows(void* c, int64_t m, int64_t n, int64_t ldc, MType t, cudaStream_t s) {
   NDT_CUDA(cudaMemset2DAsync(c, ldc * msize(t), 0, n * msize(t), m, s));
 }
@@ -179,13 +197,70 @@ int ndt_b200_scaled_linear_dev(int x_type, const void* x, long tokens, long k, l
     if (!x || !w || !w_scales) bad("NULL pointer");
     Laid lw(wt, w, n, k, w_row_stride, w_col_stride, s);
     set_scales(lw.o, w_scales, 128, w_scale_row_stride, w_scale_col_stride, "w");
-    // 8-bit x and its scales (a column of them for each block of k)
-    const int64_t ld = up(k, 16), kb = (k + 127) / 128, st = up(tokens, 4);
-    Workspace ws((size_t)(tokens * ld + kb * st * 4), s);
-    float* sx = (float*)((char*)ws.p + tokens * ld);
-    quantize(xt, MatView{x, tokens, k, x_row_stride, x_col_stride}, 1, MType::E4M3, QuantOut{ws.p, ld, sx, 1, st}, QuantOut{}, s);
-    ScaledOperand ox{ws.p, tokens, ld, MType::E4M3, sx, 1, st, true};
-    scaled_gemm(ox, lw.o, k, yt, y, ldy, false, s);
+    Quantised qx(MatView{x, tokens, k, x_row_stride, x_col_stride}, 1, MType::E4M3);
+    Workspace ws(qx.bytes(), s);
+    qx.place(ws.p);
+    quantize(xt, qx.x, 1, MType::E4M3, qx.out(), QuantOut{}, s);
+    scaled_gemm(qx.operand(), lw.o, k, yt, y, ldy, false, s);
+  });
+}
+
+int ndt_b200_scaled_linear_fwd_dev(int x_type, const void* x, long tokens, long k, long x_row_stride, long x_col_stride,
+                                   int w_type, const void* w, long n, long w_row_stride, long w_col_stride, void* y,
+                                   long ldy, void* wt, long ldwt, float* wt_scales, void* stream) {
+  return entry("scaled_linear_fwd", [&] {
+    const MType xt = real_type(x_type, "x"), wtp = real_type(w_type, "w");
+    size_ok(tokens, "tokens"), size_ok(n, "outputs"), size_ok(k, "inputs");
+    cudaStream_t s = (cudaStream_t)stream;
+    if (ldy < n) bad("ldy is smaller than a row of y");
+    if ((tokens && n && !y) || (k && ((tokens && !x) || (n && !w))) || (wt && !wt_scales)) bad("NULL pointer");
+    if (wt && (ldwt < up(n, 16) || ldwt % 16 || (uintptr_t)wt % 16)) bad("wt needs a 16-byte aligned base and a leading dimension to match");
+    if (n == 0) return;
+    if (k == 0) {
+      if (tokens) zero_rows(y, tokens, n, ldy, xt, s);
+      return;
+    }
+    Quantised qw(MatView{w, n, k, w_row_stride, w_col_stride}, 128, MType::E4M3),
+        qx(MatView{x, tokens, k, x_row_stride, x_col_stride}, 1, MType::E4M3);
+    Workspace ws(qw.bytes() + qx.bytes(), s);
+    qx.place(qw.place(ws.p));
+    const QuantOut t{wt, ldwt, wt_scales, 1, (k + 127) / 128};
+    quantize(wtp, qw.x, 128, MType::E4M3, qw.out(), wt ? t : QuantOut{}, s);
+    if (tokens == 0) return;
+    quantize(xt, qx.x, 1, MType::E4M3, qx.out(), QuantOut{}, s);
+    scaled_gemm(qx.operand(), qw.operand(), k, xt, y, ldy, false, s);
+  });
+}
+
+int ndt_b200_scaled_linear_vjp_dev(int x_type, const void* dy, long tokens, long n, long dy_row_stride, long dy_col_stride,
+                                   const void* x, long k, long x_row_stride, long x_col_stride, const void* wt, long ldwt,
+                                   const float* wt_scales, int grad8_type, void* dx, long lddx, int dw_type, void* dw,
+                                   long lddw, void* stream) {
+  return entry("scaled_linear_vjp", [&] {
+    const MType xt = real_type(x_type, "x"), g8 = type8(grad8_type, "the gradient's 8-bit type");
+    const MType dwt = dw ? real_type(dw_type, "dw") : MType::F32;
+    size_ok(tokens, "tokens"), size_ok(n, "outputs"), size_ok(k, "inputs");
+    cudaStream_t s = (cudaStream_t)stream;
+    if ((dx && lddx < k) || (dw && lddw < k)) bad("a leading dimension is smaller than a row");
+    if (k == 0 || (!dx && !dw)) return;
+    if (dx && n == 0 && tokens) zero_rows(dx, tokens, k, lddx, xt, s);
+    if (dw && tokens == 0 && n) zero_rows(dw, n, k, lddw, dwt, s);
+    if (n == 0 || tokens == 0) return;
+    if (!dy || (dx && (!wt || !wt_scales)) || (dw && !x)) bad("NULL pointer");
+    const MatView g{dy, tokens, n, dy_row_stride, dy_col_stride}, gt{dy, n, tokens, dy_col_stride, dy_row_stride},
+        xtr{x, k, tokens, x_col_stride, x_row_stride};
+    Quantised qg(g, 1, g8), qgt(gt, 1, g8), qxt(xtr, 1, MType::E4M3);
+    Workspace ws((dx ? qg.bytes() : 0) + (dw ? qgt.bytes() + qxt.bytes() : 0), s);
+    void* p = ws.p;
+    if (dx) p = qg.place(p);
+    if (dw) qxt.place(qgt.place(p));
+    quantize(xt, g, 1, g8, dx ? qg.out() : QuantOut{}, dw ? qgt.out() : QuantOut{}, s);
+    if (dw) quantize(xt, MatView{x, tokens, k, x_row_stride, x_col_stride}, 1, MType::E4M3, QuantOut{}, qxt.out(), s);
+    if (dx) {
+      ScaledOperand ow{wt, k, ldwt, MType::E4M3, wt_scales, 1, (k + 127) / 128, false};
+      scaled_gemm(qg.operand(), ow, n, xt, dx, lddx, false, s);
+    }
+    if (dw) scaled_gemm(qgt.operand(), qxt.operand(), tokens, dwt, dw, lddw, false, s);
   });
 }
 

@@ -9,16 +9,17 @@
 // accumulators in registers, in 32 bits.  Two TMEM buffers let the tensor
 // core work on block kb + 1 meanwhile.
 //
-// Roles (11 warps): 0 loads the operand tiles by TMA into a ring of 128-byte
+// Roles (12 warps): 0 loads the operand tiles by TMA into a ring of 128-byte
 // swizzled stages, 1 issues the MMAs, 2 loads the scales into a ring of its
-// own (cp.async), 3 - 10 scale and sum (a thread holds one row and half the
+// own (cp.async), 4 - 11 scale and sum (a thread holds one row and half the
 // tile's columns).
 //
 // Two forms.  CTAS = 1: one CTA computes a 128 x BN tile; where there are few
 // tiles a cluster of CTAs splits k and adds its parts through distributed
-// shared memory, in rank order (no workspace, no atomics).  CTAS = 2: a CTA
-// pair computes 256 x 256 with cta_group::2 MMAs, each CTA staging its half of
-// both operands; persistent.
+// shared memory, in rank order (no workspace, no atomics).  With few rows of A
+// (a decoding batch) the operands trade places, so that B's rows fill the 128
+// lanes and A's few the columns.  CTAS = 2: a CTA pair computes 256 x 256 with
+// cta_group::2 MMAs, each CTA staging its half of both operands; persistent.
 //
 // sa * sb is formed in 32 bits: it stays finite while the product of two
 // blocks' largest values is below 2^127.
@@ -32,8 +33,8 @@ namespace ndt {
 namespace {
 
 constexpr int kBK = 128;     // one scale block, one swizzled row
-constexpr int kThreads = 352;
-constexpr int kEpiWarp0 = 3;
+constexpr int kThreads = 384;
+constexpr int kEpiWarp0 = 4;  // the epilogue is two whole warpgroups (setmaxnreg)
 constexpr int kEpiWarps = 8;
 constexpr int kSlots = 8;    // scale ring
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
@@ -43,15 +44,15 @@ struct GemmArgs {
   const float* sb;
   int64_t sa_rs, sa_cs, sb_rs, sb_cs;
   void* c;
-  int64_t ldc;
+  int64_t crs, ccs;  // strides of C's rows and columns (one of them is 1)
   int m, n, kblocks;
   int tiles_m, tiles_n;
   int ksplit;
   uint32_t idesc;
-  int a_row;       // a scale for each row of A (else for each 128)
+  int a_row, b_row;  // a scale for each row of A / B (else for each 128)
   int ctype;       // MType of C
   int accumulate;
-  int vec;         // 16-byte stores are aligned
+  int vec;         // rows of C are contiguous and their 16-byte stores aligned
   int* flag;       // set when a bounded wait ran out
 };
 
@@ -66,8 +67,11 @@ __device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// In another CTA of the cluster.  (What it reports, that TMEM has been read, is
+// ordered by the tcgen05 fences; a release at cluster scope would add a memory
+// barrier to every k block.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
   uint32_t r;
@@ -77,7 +81,7 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
       : "=r"(ok)
       : "r"(bar), "r"(parity)
       : "memory");
@@ -90,7 +94,7 @@ __device__ __forceinline__ uint64_t now_ns() {
 }
 // A wait that ends: after two seconds, or once another wait of this CTA has
 // given up, it raises the flags and returns false.
-__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
   const uint64_t t0 = now_ns();
   while (true) {
     for (int i = 0; i < 32; i++)
@@ -159,14 +163,45 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
         "h"((uint16_t)3)
         : "memory");
 }
-__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(addr));
+// N columns of the warp's 32 lanes.
+template <int N>
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t* r) {
+  static_assert(N == 8 || N == 16 || N == 32, "columns of one load");
+  if constexpr (N == 8)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr));
+  if constexpr (N == 16)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(addr));
+  if constexpr (N == 32)
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+                 : "r"(addr));
 }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t pair(uint32_t a, uint32_t b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void cluster_sync() {
@@ -218,16 +253,19 @@ struct Shape {
   static constexpr int kBRows = BN / CTAS;           // rows of B that one CTA stages
   static constexpr int kABytes = kBM * kBK, kBBytes = kBRows * kBK;
   static constexpr int kStage = kABytes + kBBytes;
-  static constexpr int kStages = (192 * 1024) / kStage;
-  static constexpr int kScaleFloats = kBM + BN;      // a slot of the scale ring
+  // narrow tiles leave room for two CTAs on an SM: twice the loads in flight
+  static constexpr int kResident = BN <= 64 ? 2 : 1;
+  static constexpr int kStages = (kResident == 2 ? 100 : 192) * 1024 / kStage;
+  static constexpr int kScaleFloats = kBM + (BN + 31) / 32 * 32;  // a slot of the scale ring
   static constexpr int kTmemCols = 2 * BN;
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + (size_t)kSlots * kScaleFloats * 4;
-  static_assert(kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns");
+  static_assert(kTmemCols >= 32 && kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns");
   static_assert((size_t)BN * 129 * 4 <= (size_t)kStages * kStage || CTAS == 2, "the split's buffer reuses the stages");
+  static_assert(kStage % 1024 == 0, "swizzled tiles start on 1024 bytes");
 };
 
 template <int CTAS, int BN, bool BROW>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
     scaled_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                        const GemmArgs g) {
   using S = Shape<CTAS, BN>;
@@ -277,7 +315,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kb0 = CTAS == 1 ? (int)((int64_t)g.kblocks * split / g.ksplit) : 0;
   const int kb1 = CTAS == 1 ? (int)((int64_t)g.kblocks * (split + 1) / g.ksplit) : g.kblocks;
 
+  // wide tiles: the block's 384 x 168 registers, 40 a thread for the loading
+  // warpgroup and 232 for the two that sum (40 x 128 + 232 x 256 is their sum)
+  auto fewer = [] { if (BN == 256) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;"); };
+  auto more = [] { if (BN == 256) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;"); };
   if (warp == 0) {
+    fewer();
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
@@ -303,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
+    fewer();
     if (rank == 0 && lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
@@ -326,6 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     __syncwarp();
   } else if (warp == 2) {
+    fewer();
     uint32_t it = 0;
     bool ok = true;
     for (int t = unit; t < ntiles && ok; t += units) {
@@ -341,14 +386,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         va[j] = r < g.m;
         pa[j] = g.sa + (va[j] ? (int64_t)(g.a_row ? r : r >> 7) * g.sa_rs : 0);
       }
-      constexpr int kNB = BROW ? BN / 32 : 1;
+      constexpr int kNB = BROW ? (BN + 31) / 32 : 1;
       const float* pb[kNB];
       bool vb[kNB];
 #pragma unroll
       for (int j = 0; j < kNB; j++) {
         const int r = BROW ? row_b + lane + 32 * j : row_b + lane * 128;
-        vb[j] = r < g.n && (BROW || lane < (BN + 127) / 128);
-        pb[j] = g.sb + (vb[j] ? (int64_t)(BROW ? r : r >> 7) * g.sb_rs : 0);
+        vb[j] = r < g.n && (BROW ? lane + 32 * j < BN : lane < (BN + 127) / 128);
+        pb[j] = g.sb + (vb[j] ? (int64_t)(BROW && g.b_row ? r : r >> 7) * g.sb_rs : 0);
       }
       for (int kb = kb0; kb < kb1; kb++, it++) {
         const uint32_t slot = it % kSlots, ph = (it / kSlots) & 1;
@@ -364,72 +409,85 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     __syncwarp();
+  } else if (warp == 3) {
+    fewer();
   } else {
+    more();
     const int quad = warp & 3, half = (warp - kEpiWarp0) >> 2;
     const int row = quad * 32 + lane;
     const uint32_t tmem_row = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
     const uint32_t tempty_leader = CTAS == 2 ? mapa(tempty, 0) : tempty;
+    constexpr int kLd = kHalf < 16 ? kHalf : 16, kLoads = kHalf / kLd, kFly = kLoads < 4 ? kLoads : 4;
     uint32_t it = 0;
     bool ok = true;
     for (int t = unit; t < ntiles && ok; t += units) {
       int tm, tn;
       tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
-      float acc[kHalf];
+      uint64_t acc[kHalf / 2];
 #pragma unroll
-      for (int j = 0; j < kHalf; j++) acc[j] = 0.f;
+      for (int j = 0; j < kHalf / 2; j++) acc[j] = 0;
       for (int kb = kb0; kb < kb1; kb++, it++) {
         const uint32_t slot = it % kSlots, sph = (it / kSlots) & 1, buf = it & 1, ph = (it >> 1) & 1;
         if (!(ok = warp_wait(sfull + 8 * slot, sph, gave_up, g.flag))) break;
         const float* sc = scale_ring + slot * S::kScaleFloats;
         const float sa = sc[row];
         const float sab = BROW ? sa : sa * sc[128 + (BN == 256 ? half : 0)];
+        const uint64_t s2 = pair(sab, sab);
         if (!(ok = warp_wait(tfull + 8 * buf, ph, gave_up, g.flag))) break;
         fence_after();
-        uint32_t d[2][16];
-        tmem_ld16(tmem_row + buf * BN, d[0]);
+        // kFly loads at a time, so that their latency is paid once
+        uint32_t d[kFly][kLd];
 #pragma unroll
-        for (int q = 0; q < kHalf / 16; q++) {
-          tmem_ld_wait();
-          if (q + 1 < kHalf / 16) tmem_ld16(tmem_row + buf * BN + (q + 1) * 16, d[(q + 1) & 1]);
-          if (BROW) {
+        for (int q = 0; q < kFly; q++) tmem_ld<kLd>(tmem_row + buf * BN + q * kLd, d[q]);
 #pragma unroll
-            for (int j = 0; j < 16; j += 4) {
-              const float4 b = *reinterpret_cast<const float4*>(sc + 128 + half * kHalf + q * 16 + j);
-              acc[q * 16 + j] = fmaf(__uint_as_float(d[q & 1][j]), sab * b.x, acc[q * 16 + j]);
-              acc[q * 16 + j + 1] = fmaf(__uint_as_float(d[q & 1][j + 1]), sab * b.y, acc[q * 16 + j + 1]);
-              acc[q * 16 + j + 2] = fmaf(__uint_as_float(d[q & 1][j + 2]), sab * b.z, acc[q * 16 + j + 2]);
-              acc[q * 16 + j + 3] = fmaf(__uint_as_float(d[q & 1][j + 3]), sab * b.w, acc[q * 16 + j + 3]);
+        for (int q = 0; q < kLoads; q++) {
+          if (q % kFly == 0) {
+            tmem_ld_wait();
+            if (q + kFly >= kLoads) {  // the last column is in registers: the tensor core may have the buffer
+              fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                if (CTAS == 2)
+                  mbar_arrive_cluster(tempty_leader + 8 * buf);
+                else
+                  mbar_arrive(tempty + 8 * buf);
+              }
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; j++) acc[q * 16 + j] = fmaf(__uint_as_float(d[q & 1][j]), sab, acc[q * 16 + j]);
           }
+          uint32_t* w = d[q % kFly];
+#pragma unroll
+          for (int j = 0; j < kLd; j += 4) {
+            uint64_t f0 = s2, f1 = s2;
+            if (BROW) {
+              const float4 b = *reinterpret_cast<const float4*>(sc + 128 + half * kHalf + q * kLd + j);
+              f0 = mul2(s2, pair(b.x, b.y)), f1 = mul2(s2, pair(b.z, b.w));
+            }
+            uint64_t& a0 = acc[(q * kLd + j) / 2];
+            uint64_t& a1 = acc[(q * kLd + j) / 2 + 1];
+            a0 = fma2(pair(w[j], w[j + 1]), f0, a0);
+            a1 = fma2(pair(w[j + 2], w[j + 3]), f1, a1);
+          }
+          if (q + kFly < kLoads) tmem_ld<kLd>(tmem_row + buf * BN + (q + kFly) * kLd, w);
         }
-        fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (CTAS == 2)
-            mbar_arrive_cluster(tempty_leader + 8 * buf);
-          else
-            mbar_arrive(tempty + 8 * buf);
-          mbar_arrive(sempty + 8 * slot);
-        }
+        if (lane == 0) mbar_arrive(sempty + 8 * slot);
       }
       if (!ok) break;
+      auto at = [&](int j) { return __uint_as_float((uint32_t)(acc[j / 2] >> (j & 1) * 32)); };
       const int row_c = tm * 128 * CTAS + rank * 128 + row, col_c = tn * BN + half * kHalf;
       if (CTAS == 1 && g.ksplit > 1) {
         // this CTA's part, column-major with an odd pitch, over the stages (all consumed)
         float* part = reinterpret_cast<float*>(raw + (stage0 - smem_u32(raw)));
 #pragma unroll
-        for (int j = 0; j < kHalf; j++) part[(half * kHalf + j) * 129 + row] = acc[j];
+        for (int j = 0; j < kHalf; j++) part[(half * kHalf + j) * 129 + row] = at(j);
       } else if (row_c < g.m) {
-        const int64_t base = (int64_t)row_c * g.ldc + col_c;
+        const int64_t base = row_c * g.crs + col_c * g.ccs;
         const int cols = min(kHalf, g.n - col_c);
         if (g.vec && cols == kHalf && !g.accumulate) {
           if (g.ctype == (int)MType::F32) {
             float4* p = reinterpret_cast<float4*>((float*)g.c + base);
 #pragma unroll
-            for (int j = 0; j < kHalf / 4; j++) p[j] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+            for (int j = 0; j < kHalf / 4; j++) p[j] = make_float4(at(4 * j), at(4 * j + 1), at(4 * j + 2), at(4 * j + 3));
           } else {
             uint4* p = reinterpret_cast<uint4*>((uint16_t*)g.c + base);
 #pragma unroll
@@ -438,10 +496,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int i = 0; i < 4; i++) {
                 if (g.ctype == (int)MType::BF16) {
-                  const __nv_bfloat162 h = __floats2bfloat162_rn(acc[8 * j + 2 * i], acc[8 * j + 2 * i + 1]);
+                  const __nv_bfloat162 h = __floats2bfloat162_rn(at(8 * j + 2 * i), at(8 * j + 2 * i + 1));
                   w[i] = *reinterpret_cast<const uint32_t*>(&h);
                 } else {
-                  const __half2 h = __floats2half2_rn(acc[8 * j + 2 * i], acc[8 * j + 2 * i + 1]);
+                  const __half2 h = __floats2half2_rn(at(8 * j + 2 * i), at(8 * j + 2 * i + 1));
                   w[i] = *reinterpret_cast<const uint32_t*>(&h);
                 }
               }
@@ -452,9 +510,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < kHalf; j++)
             if (j < cols) {
-              float v = acc[j];
-              if (g.accumulate) v += load_c(g.c, base + j, g.ctype);
-              store_c(g.c, base + j, g.ctype, v);
+              float v = at(j);
+              if (g.accumulate) v += load_c(g.c, base + j * g.ccs, g.ctype);
+              store_c(g.c, base + j * g.ccs, g.ctype, v);
             }
         }
       }
@@ -466,22 +524,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   if (CTAS == 1 && g.ksplit > 1) {
     cluster_sync();
-    // each CTA adds its share of the tile's columns over all parts, in rank order
+    // each CTA adds its share of the tile over all parts, in rank order; neighbouring threads take neighbours in C
     int tm, tn;
     tile_at(unit, g.tiles_m, g.tiles_n, tm, tn);
-    const int rows = min(128, g.m - tm * 128), cols = BN / g.ksplit;
-    const uint32_t part = stage0;
-    for (int e = threadIdx.x; e < rows * cols; e += kThreads) {
-      const int r = e / cols, j = split * cols + e % cols;
-      const uint32_t at = part + (uint32_t)(j * 129 + r) * 4;
+    const int rows = min(128, g.m - tm * 128), cols = min(BN, g.n - tn * BN);
+    const bool by_row = g.crs == 1;
+    const int fast = by_row ? rows : cols, total = rows * cols;
+    for (int e = total * split / g.ksplit + threadIdx.x; e < total * (split + 1) / g.ksplit; e += kThreads) {
+      const int lo = e % fast, hi = e / fast;
+      const int r = by_row ? lo : hi, j = by_row ? hi : lo;
+      const uint32_t at = stage0 + (uint32_t)(j * 129 + r) * 4;
       float v = 0.f;
       for (int p = 0; p < g.ksplit; p++) v += ld_cluster(mapa(at, p));
-      const int col = tn * BN + j;
-      if (col < g.n && !*gave_up) {
-        const int64_t i = (int64_t)(tm * 128 + r) * g.ldc + col;
-        if (g.accumulate) v += load_c(g.c, i, g.ctype);
-        store_c(g.c, i, g.ctype, v);
-      }
+      if (*gave_up) continue;
+      const int64_t i = (tm * 128 + r) * g.crs + (tn * BN + j) * g.ccs;
+      if (g.accumulate) v += load_c(g.c, i, g.ctype);
+      store_c(g.c, i, g.ctype, v);
     }
     cluster_sync();
   } else if (CTAS == 2) {
@@ -549,16 +607,19 @@ void launch(const ScaledOperand& a, const ScaledOperand& b, int64_t k, GemmArgs 
 
 }  // namespace
 
-void scaled_gemm(const ScaledOperand& a, const ScaledOperand& b, int64_t k, MType ct, void* c, int64_t ldc,
+void scaled_gemm(const ScaledOperand& a_, const ScaledOperand& b_, int64_t k, MType ct, void* c, int64_t ldc,
                  bool accumulate, cudaStream_t s) {
+  // Up to 64 rows of A: B's rows on the 128 lanes, A's as 16 to 64 columns.
+  const bool swap = a_.rows <= 64;
+  const ScaledOperand &a = swap ? b_ : a_, &b = swap ? a_ : b_;
   GemmArgs g{};
   g.sa = a.s, g.sa_rs = a.srs, g.sa_cs = a.scs;
   g.sb = b.s, g.sb_rs = b.srs, g.sb_cs = b.scs;
-  g.c = c, g.ldc = ldc;
+  g.c = c, g.crs = swap ? 1 : ldc, g.ccs = swap ? ldc : 1;
   g.m = (int)a.rows, g.n = (int)b.rows;
   g.kblocks = (int)((k + kBK - 1) / kBK);
-  g.a_row = a.per_row, g.ctype = (int)ct, g.accumulate = accumulate;
-  g.vec = (uintptr_t)c % 16 == 0 && ldc * msize(ct) % 16 == 0;
+  g.a_row = a.per_row, g.b_row = b.per_row, g.ctype = (int)ct, g.accumulate = accumulate;
+  g.vec = !swap && (uintptr_t)c % 16 == 0 && ldc * msize(ct) % 16 == 0;
   g.flag = wait_flag_device();
   g.ksplit = 1;
   const int sms = ctx().sm_count;
@@ -570,7 +631,7 @@ void scaled_gemm(const ScaledOperand& a, const ScaledOperand& b, int64_t k, MTyp
            (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
   };
   const int pair_tiles = cdiv(g.m, 256) * cdiv(g.n, 256);
-  if (pair_tiles * 2 >= sms / 2) {
+  if (!swap && pair_tiles * 2 >= sms / 2) {
     g.tiles_m = cdiv(g.m, 256), g.tiles_n = cdiv(g.n, 256);
     g.idesc = idesc(256, 256);
     const int grid = 2 * std::min(pair_tiles, sms / 2);
@@ -580,16 +641,21 @@ void scaled_gemm(const ScaledOperand& a, const ScaledOperand& b, int64_t k, MTyp
       launch<2, 256, false>(a, b, k, g, grid, 2, s);
     return;
   }
-  g.tiles_m = cdiv(g.m, 128), g.tiles_n = cdiv(g.n, 128);
-  g.idesc = idesc(128, 128);
-  int split = 1;
-  while (split < 8 && g.tiles_m * g.tiles_n * split * 2 <= sms && g.kblocks >= 4 * split) split *= 2;
-  g.ksplit = split;
-  const int grid = g.tiles_m * g.tiles_n * split;
-  if (b.per_row)
-    launch<1, 128, true>(a, b, k, g, grid, split, s);
+  const int bn = !swap ? 128 : g.n <= 16 ? 16 : g.n <= 32 ? 32 : 64;
+  g.tiles_m = cdiv(g.m, 128), g.tiles_n = cdiv(g.n, bn);
+  g.idesc = idesc(128, bn);
+  // k is split while the CTAs fit the GPU at once and keep at least 4 blocks each
+  const int room = sms * (swap ? 2 : 1), tiles = g.tiles_m * g.tiles_n;
+  g.ksplit = std::max(1, std::min({8, room / tiles, g.kblocks / 4}));
+  const int grid = tiles * g.ksplit;
+  if (!swap)
+    b.per_row ? launch<1, 128, true>(a, b, k, g, grid, g.ksplit, s) : launch<1, 128, false>(a, b, k, g, grid, g.ksplit, s);
+  else if (bn == 16)
+    launch<1, 16, true>(a, b, k, g, grid, g.ksplit, s);
+  else if (bn == 32)
+    launch<1, 32, true>(a, b, k, g, grid, g.ksplit, s);
   else
-    launch<1, 128, false>(a, b, k, g, grid, split, s);
+    launch<1, 64, true>(a, b, k, g, grid, g.ksplit, s);
 }
 
 }  // namespace ndt

@@ -174,6 +174,10 @@ SIGNATURES = [
      [cl, cl, cl, ci, vp, cl, cl, ci, vp, cl, cl, ci, vp, cl, cl, ci, vp, cl, cl, ci, vp, cl, ci, vp]),
     ("ndt_b200_scaled_linear_dev", ctypes.c_int,
      [ci, vp, cl, cl, cl, cl, ci, vp, cl, cl, cl, vp, cl, cl, ci, vp, cl, vp]),
+    ("ndt_b200_scaled_linear_fwd_dev", ctypes.c_int,
+     [ci, vp, cl, cl, cl, cl, ci, vp, cl, cl, cl, vp, cl, vp, cl, vp, vp]),
+    ("ndt_b200_scaled_linear_vjp_dev", ctypes.c_int,
+     [ci, vp, cl, cl, cl, cl, vp, cl, cl, cl, vp, cl, vp, ci, vp, cl, ci, vp, cl, vp]),
     ("ndt_b200_embedding_dev", ctypes.c_int, [ci, vp, cl, cl, cl, vp, ci, cl, cl, cf, vp, cl, vp]),
     ("ndt_b200_embedding_grad_dev", ctypes.c_int, [ci, vp, cl, vp, ci, cl, cl, cl, cl, cf, ci, vp, cl, ci, vp]),
     ("ndt_b200_expert_layer_dev", ctypes.c_int,

@@ -1,8 +1,10 @@
-"""What the language-model operators share: element types, streams, checks."""
+"""What the language-model operators share: element types, streams, checks.
+
+A call for a few tokens costs the host more than the GPU, so the wrappers read
+each attribute of a tensor once and leave the messages to the failing path.
+"""
 
 from __future__ import annotations
-
-import contextlib
 
 import torch
 
@@ -10,17 +12,25 @@ from ._lib import get_lib, last_error
 from .tensor import NDTensorsError, StatusCode
 
 #: element type codes of the C ABI
-CODES = {torch.float32: 2, torch.bfloat16: 3, torch.float16: 4, torch.float8_e4m3fn: 5, torch.float8_e5m2: 6}
-REAL = (torch.float32, torch.bfloat16, torch.float16)
-FLOAT8 = (torch.float8_e4m3fn, torch.float8_e5m2)
+REAL = {torch.float32: 2, torch.bfloat16: 3, torch.float16: 4}
+FLOAT8 = {torch.float8_e4m3fn: 5, torch.float8_e5m2: 6}
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
-_here = contextlib.nullcontext()
+_current_device = torch._C._cuda_getDevice
+_entries: dict = {}
 
 
-def call(name: str, *args) -> None:
-    """Call a C entry point; raise its error (ValueError for sizes that do not fit)."""
-    status = getattr(get_lib(), name)(*args)
+def launch(name: str, device: int, *args) -> None:
+    """Call the C entry point with the device current, its current stream as the last argument; raise its error
+    (ValueError for sizes that do not fit)."""
+    f = _entries.get(name)
+    if f is None:
+        f = _entries[name] = getattr(get_lib(), name)
+    if device == _current_device():
+        status = f(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = f(*args, _raw_stream(device))
     if status == 0:
         return
     if status == StatusCode.SHAPE_MISMATCH:
@@ -28,38 +38,39 @@ def call(name: str, *args) -> None:
     raise NDTensorsError(f"{last_error()} (status {status})")
 
 
-def on(device):
-    """The context in which `device` is current, and its current stream's handle."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        return _here, _raw_stream(index)
-    return torch.cuda.device(index), _raw_stream(index)
-
-
-def check_cuda(what: str, first, *others) -> None:
-    """Every tensor given is a CUDA tensor of one device."""
-    if not first.is_cuda:
+def device_of(what: str, first, *others) -> int:
+    """The CUDA device that every tensor given is on."""
+    device = first.get_device()
+    if device < 0:
         raise NDTensorsError(f"{what}: the tensors must be CUDA tensors (there is no CPU compute path)")
     for t in others:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != device:
             raise NDTensorsError(f"{what}: the tensors must be on one device")
+    return device
 
 
-def check_type(what: str, name: str, dtype, allowed) -> None:
-    if dtype not in allowed:
+def code_of(what: str, name: str, dtype, allowed) -> int:
+    """The C ABI's code of an element type, one of those allowed."""
+    code = allowed.get(dtype)
+    if code is None:
         raise TypeError(f"{what}: {name} must be one of {', '.join(str(d)[6:] for d in allowed)}, got {str(dtype)[6:]}")
+    return code
 
 
 def rows_of(x):
     """x as a matrix of its last axis (a view where its strides allow)."""
-    return x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    if x.dim() == 2:
+        return x
+    lead = 1
+    for n in x.shape[:-1]:
+        lead *= n
+    return x.reshape(lead, x.shape[-1])
 
 
 def unit_rows(x):
-    """x with unit stride along its last axis and rows that do not overlap, copied only where it has not."""
-    if x.dim() == 2 and x.stride(1) == 1 and x.stride(0) >= x.shape[1]:
-        return x
-    return x.contiguous()
+    """The matrix x with unit stride along its rows and rows that do not overlap, copied only where it has not."""
+    rs, cs = x.stride()
+    return x if cs == 1 and rs >= x.shape[1] else x.contiguous()
 
 
-__all__ = ["CODES", "REAL", "FLOAT8", "call", "on", "check_cuda", "check_type", "rows_of", "unit_rows"]
+__all__ = ["REAL", "FLOAT8", "launch", "device_of", "code_of", "rows_of", "unit_rows"]

@@ -5,9 +5,11 @@ from __future__ import annotations
 
 import torch
 
-from ._model import CODES, call, check_cuda, check_type, on, rows_of, unit_rows
+from ._model import code_of, device_of, launch, rows_of, unit_rows
 
 E4M3 = torch.float8_e4m3fn
+_HALF = {torch.bfloat16: 3, torch.float16: 4}
+_F32 = {torch.float32: 2}
 
 
 def expert_layer(x, router, w_in, w_out, top: int, in_scales=None, out_scales=None, renormalize: bool = True):
@@ -28,11 +30,11 @@ def expert_layer(x, router, w_in, w_out, top: int, in_scales=None, out_scales=No
     [..., top].  Made for at most about a hundred tokens (a decoding batch);
     more are right, but each 8 to 32 tokens of an expert read its weights anew.
     """
-    check_cuda("expert_layer", x, router, w_in, w_out, in_scales, out_scales)
-    check_type("expert_layer", "x", x.dtype, (torch.bfloat16, torch.float16))
-    check_type("expert_layer", "router", router.dtype, (x.dtype,))
-    check_type("expert_layer", "w_in", w_in.dtype, (x.dtype, E4M3))
-    check_type("expert_layer", "w_out", w_out.dtype, (w_in.dtype,))
+    device = device_of("expert_layer", x, router, w_in, w_out, in_scales, out_scales)
+    xt = code_of("expert_layer", "x", x.dtype, _HALF)
+    code_of("expert_layer", "router", router.dtype, {x.dtype: xt})
+    wt = code_of("expert_layer", "w_in", w_in.dtype, {x.dtype: xt, E4M3: 5})
+    code_of("expert_layer", "w_out", w_out.dtype, {w_in.dtype: wt})
     if router.dim() != 2 or w_in.dim() != 3 or w_out.dim() != 3 or x.dim() < 1:
         raise ValueError("expert_layer: router is a matrix, w_in and w_out have three axes")
     e, h = router.shape
@@ -47,23 +49,20 @@ def expert_layer(x, router, w_in, w_out, top: int, in_scales=None, out_scales=No
         hb, ib, jb = (h + 127) // 128, (i + 127) // 128, (2 * i + 127) // 128
         if in_scales.shape != (e, jb, hb) or out_scales.shape != (e, hb, ib):
             raise ValueError("expert_layer: scales do not fit the weights' 128 x 128 blocks")
-        check_type("expert_layer", "in_scales", in_scales.dtype, (torch.float32,))
-        check_type("expert_layer", "out_scales", out_scales.dtype, (torch.float32,))
+        code_of("expert_layer", "in_scales", in_scales.dtype, _F32)
+        code_of("expert_layer", "out_scales", out_scales.dtype, _F32)
         in_scales, out_scales = in_scales.contiguous(), out_scales.contiguous()
     elif in_scales is not None or out_scales is not None:
         raise ValueError("expert_layer: scales are for float8 weights")
     x2 = unit_rows(rows_of(x))
     router, w_in, w_out = router.contiguous(), w_in.contiguous(), w_out.contiguous()
     t = x2.shape[0]
-    y = torch.empty((t, h), dtype=x.dtype, device=x.device)
-    ids = torch.empty((t, top), dtype=torch.int32, device=x.device)
-    weights = torch.empty((t, top), dtype=torch.float32, device=x.device)
-    ctx, stream = on(x.device)
-    with ctx:
-        call("ndt_b200_expert_layer_dev", CODES[x.dtype], x2.data_ptr(), t, h, max(h, x2.stride(0)), router.data_ptr(), e,
-             CODES[w_in.dtype], w_in.data_ptr(), None if in_scales is None else in_scales.data_ptr(), w_out.data_ptr(),
-             None if out_scales is None else out_scales.data_ptr(), i, top, renormalize, y.data_ptr(), h,
-             ids.data_ptr(), weights.data_ptr(), stream)
+    y = x.new_empty((t, h))
+    ids, weights = x.new_empty((t, top), dtype=torch.int32), x.new_empty((t, top), dtype=torch.float32)
+    launch("ndt_b200_expert_layer_dev", device, xt, x2.data_ptr(), t, h, max(h, x2.stride(0)), router.data_ptr(), e, wt,
+           w_in.data_ptr(), None if in_scales is None else in_scales.data_ptr(), w_out.data_ptr(),
+           None if out_scales is None else out_scales.data_ptr(), i, top, renormalize, y.data_ptr(), h, ids.data_ptr(),
+           weights.data_ptr())
     lead = x.shape[:-1]
     return (y, ids, weights) if x.dim() == 2 else (y.view(x.shape), ids.view(lead + (top,)), weights.view(lead + (top,)))
 

@@ -15,8 +15,7 @@ from __future__ import annotations
 import torch
 from torch.autograd import Function
 
-from ._model import CODES, FLOAT8, REAL, call, check_cuda, check_type, on, rows_of
-from .tensor import NDTensorsError
+from ._model import FLOAT8, REAL, code_of, device_of, launch, rows_of
 
 E4M3 = torch.float8_e4m3fn
 
@@ -46,9 +45,8 @@ def quantize_blocks(x, block_rows: int = 1, dtype=E4M3, transposed: bool = False
     qt being the 8-bit form of x's transpose from the same pass over x (and
     with ``values=False`` only ``(qt, scales_t)``).
     """
-    check_cuda("quantize_blocks", x)
-    check_type("quantize_blocks", "x", x.dtype, REAL)
-    check_type("quantize_blocks", "dtype", dtype, FLOAT8)
+    device = device_of("quantize_blocks", x)
+    xt, qt8 = code_of("quantize_blocks", "x", x.dtype, REAL), code_of("quantize_blocks", "dtype", dtype, FLOAT8)
     if x.dim() != 2:
         raise ValueError("quantize_blocks: x must be a matrix")
     if block_rows not in (1, 128):
@@ -64,23 +62,20 @@ def quantize_blocks(x, block_rows: int = 1, dtype=E4M3, transposed: bool = False
     if transposed:
         t, u = _empty8(c, r, dtype, x.device), _empty_scales(c, r, block_rows, x.device)
         ta = (t.data_ptr(), max(16, t.stride(0)), u.data_ptr(), u.stride(0), u.stride(1))
-    ctx, stream = on(x.device)
-    with ctx:
-        call("ndt_b200_quantize_dev", CODES[x.dtype], x.data_ptr(), r, c, x.stride(0), x.stride(1), block_rows, CODES[dtype],
-             *qa, *ta, stream)
+    launch("ndt_b200_quantize_dev", device, xt, x.data_ptr(), r, c, x.stride(0), x.stride(1), block_rows, qt8, *qa, *ta)
     return ((q, s) if values else ()) + ((t, u) if transposed else ())
 
 
-def _block_rows(what: str, q, s):
+def _block_rows(what: str, q, s) -> int:
     """Whether the scales are for single rows (1) or for 128 rows."""
-    check_type(what, "an 8-bit operand", q.dtype, FLOAT8)
     if q.dim() != 2 or s.dim() != 2 or s.dtype != torch.float32:
         raise ValueError(f"{what}: an operand is a float8 matrix with a float32 matrix of scales")
-    r, kb = q.shape[0], (q.shape[1] + 127) // 128
-    if s.shape[1] == kb:
-        if s.shape[0] == (r + 127) // 128:
+    r, c = q.shape
+    rb, kb = s.shape
+    if kb == (c + 127) // 128:
+        if rb == (r + 127) // 128:
             return 128
-        if s.shape[0] == r:
+        if rb == r:
             return 1
     raise ValueError(f"{what}: scales of shape {tuple(s.shape)} do not fit an operand of shape {tuple(q.shape)}")
 
@@ -93,7 +88,8 @@ def scaled_gemm(a, a_scales, b, b_scales, out_dtype=torch.bfloat16, out=None, ac
     ``accumulate``.  Any strides are taken; rows that do not start on 16 bytes
     cost a copy.
     """
-    check_cuda("scaled_gemm", a, a_scales, b, b_scales, out)
+    device = device_of("scaled_gemm", a, a_scales, b, b_scales, out)
+    at, bt = code_of("scaled_gemm", "a", a.dtype, FLOAT8), code_of("scaled_gemm", "b", b.dtype, FLOAT8)
     ra, rb = _block_rows("scaled_gemm", a, a_scales), _block_rows("scaled_gemm", b, b_scales)
     m, k = a.shape
     n = b.shape[0]
@@ -102,18 +98,15 @@ def scaled_gemm(a, a_scales, b, b_scales, out_dtype=torch.bfloat16, out=None, ac
     if out is None:
         if accumulate:
             raise ValueError("scaled_gemm: accumulate needs out")
-        check_type("scaled_gemm", "out_dtype", out_dtype, REAL)
-        out = torch.empty((m, n), dtype=out_dtype, device=a.device)
+        ct = code_of("scaled_gemm", "out_dtype", out_dtype, REAL)
+        out = a.new_empty((m, n), dtype=out_dtype)
     else:
-        check_type("scaled_gemm", "out", out.dtype, REAL)
+        ct = code_of("scaled_gemm", "out", out.dtype, REAL)
         if out.shape != (m, n) or (n > 1 and out.stride(1) != 1) or (m > 1 and out.stride(0) < n):
             raise ValueError("scaled_gemm: out must be [m, n] with unit stride along n")
-    ctx, stream = on(a.device)
-    with ctx:
-        call("ndt_b200_scaled_gemm_dev", m, n, k, CODES[a.dtype], a.data_ptr(), a.stride(0), a.stride(1), ra,
-             a_scales.data_ptr(), a_scales.stride(0), a_scales.stride(1), CODES[b.dtype], b.data_ptr(), b.stride(0),
-             b.stride(1), rb, b_scales.data_ptr(), b_scales.stride(0), b_scales.stride(1), CODES[out.dtype],
-             out.data_ptr(), max(n, out.stride(0)), int(accumulate), stream)
+    launch("ndt_b200_scaled_gemm_dev", device, m, n, k, at, a.data_ptr(), *a.stride(), ra, a_scales.data_ptr(),
+           *a_scales.stride(), bt, b.data_ptr(), *b.stride(), rb, b_scales.data_ptr(), *b_scales.stride(), ct,
+           out.data_ptr(), max(n, out.stride(0)), accumulate)
     return out
 
 
@@ -124,23 +117,20 @@ def scaled_linear(x, weight, weight_scales, out_dtype=None):
     in the call (e4m3, a scale for each row and 128 columns).  ``out_dtype``
     defaults to x's type.
     """
-    check_cuda("scaled_linear", x, weight, weight_scales)
-    check_type("scaled_linear", "x", x.dtype, REAL)
+    device = device_of("scaled_linear", x, weight, weight_scales)
+    xt = code_of("scaled_linear", "x", x.dtype, REAL)
+    wt = code_of("scaled_linear", "weight", weight.dtype, FLOAT8)
     if _block_rows("scaled_linear", weight, weight_scales) != 128:
         raise ValueError("scaled_linear: the weights' scales must be those of 128 x 128 blocks")
     n, k = weight.shape
     if x.dim() < 1 or x.shape[-1] != k:
         raise ValueError("scaled_linear: the last axis of x does not fit the weights")
-    out_dtype = out_dtype or x.dtype
-    check_type("scaled_linear", "out_dtype", out_dtype, REAL)
+    yt = xt if out_dtype is None else code_of("scaled_linear", "out_dtype", out_dtype, REAL)
     x2 = rows_of(x)
     t = x2.shape[0]
-    y = torch.empty((t, n), dtype=out_dtype, device=x.device)
-    ctx, stream = on(x.device)
-    with ctx:
-        call("ndt_b200_scaled_linear_dev", CODES[x.dtype], x2.data_ptr(), t, k, x2.stride(0), x2.stride(1),
-             CODES[weight.dtype], weight.data_ptr(), n, weight.stride(0), weight.stride(1), weight_scales.data_ptr(),
-             weight_scales.stride(0), weight_scales.stride(1), CODES[out_dtype], y.data_ptr(), n, stream)
+    y = x.new_empty((t, n), dtype=out_dtype or x.dtype)
+    launch("ndt_b200_scaled_linear_dev", device, xt, x2.data_ptr(), t, k, *x2.stride(), wt, weight.data_ptr(), n,
+           *weight.stride(), weight_scales.data_ptr(), *weight_scales.stride(), yt, y.data_ptr(), n)
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
 
 
@@ -150,36 +140,37 @@ class _ScaledLinear(Function):
 
     @staticmethod
     def forward(ctx, x, weight, grad_dtype):
+        device, xt, wt = x.get_device(), REAL[x.dtype], REAL[weight.dtype]
+        n, k = weight.shape
         x2 = rows_of(x)
-        xq, xs = quantize_blocks(x2)
-        ctx.needs = ctx.needs_input_grad
-        if ctx.needs[0]:
-            wq, ws, wt, wu = quantize_blocks(weight, 128, transposed=True)
-        else:
-            (wq, ws), wt, wu = quantize_blocks(weight, 128), None, None
-        ctx.save_for_backward(x2 if ctx.needs[1] else None, wt, wu)
-        ctx.grad_dtype, ctx.x_shape, ctx.types = grad_dtype, x.shape, (x.dtype, weight.dtype)
-        y = scaled_gemm(xq, xs, wq, ws, out_dtype=x.dtype)
-        return y if x.dim() == 2 else y.view(x.shape[:-1] + (weight.shape[0],))
+        t = x2.shape[0]
+        y = x.new_empty((t, n))
+        need_x, need_w, _ = ctx.needs_input_grad
+        # the weights' 8-bit transpose, kept for x's gradient: values and scales in one buffer
+        ld, kb, nb = (n + 15) // 16 * 16, (k + 127) // 128, (n + 127) // 128
+        kept = x.new_empty(k * ld + 4 * kb * nb, dtype=torch.uint8) if need_x else None
+        at = kept.data_ptr() if need_x else 0
+        launch("ndt_b200_scaled_linear_fwd_dev", device, xt, x2.data_ptr(), t, k, *x2.stride(), wt, weight.data_ptr(), n,
+               *weight.stride(), y.data_ptr(), max(1, n), at or None, ld, at + k * ld if need_x else None)
+        ctx.save_for_backward(x2 if need_w else None, kept)
+        ctx.args = device, xt, FLOAT8[grad_dtype], x.shape, weight.shape, weight.dtype, x.dtype
+        return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
 
     @staticmethod
     def backward(ctx, dy):
-        x2, wt, wu = ctx.saved_tensors
-        dx = dw = None
+        x2, kept = ctx.saved_tensors
+        device, xt, g8, x_shape, (n, k), w_dtype, x_dtype = ctx.args
+        need_x, need_w, _ = ctx.needs_input_grad
         dy2 = rows_of(dy)
-        if ctx.needs[0] and ctx.needs[1]:
-            gq, gs, gt, gu = quantize_blocks(dy2, 1, ctx.grad_dtype, transposed=True)
-        elif ctx.needs[0]:
-            gq, gs = quantize_blocks(dy2, 1, ctx.grad_dtype)
-        elif ctx.needs[1]:
-            gt, gu = quantize_blocks(dy2, 1, ctx.grad_dtype, transposed=True, values=False)
-        if ctx.needs[0]:
-            dx = scaled_gemm(gq, gs, wt, wu, out_dtype=ctx.types[0])
-            dx = dx if len(ctx.x_shape) == 2 else dx.view(ctx.x_shape)
-        if ctx.needs[1]:
-            xt, xu = quantize_blocks(x2, transposed=True, values=False)
-            dw = scaled_gemm(gt, gu, xt, xu, out_dtype=ctx.types[1])
-        return dx, dw, None
+        t = dy2.shape[0]
+        ld = (n + 15) // 16 * 16
+        dx = dy.new_empty((t, k), dtype=x_dtype) if need_x else None
+        dw = dy.new_empty((n, k), dtype=w_dtype) if need_w else None
+        launch("ndt_b200_scaled_linear_vjp_dev", device, xt, dy2.data_ptr(), t, n, *dy2.stride(),
+               x2.data_ptr() if need_w else None, k, *(x2.stride() if need_w else (0, 0)),
+               kept.data_ptr() if need_x else None, ld, kept.data_ptr() + k * ld if need_x else None, g8,
+               dx.data_ptr() if need_x else None, max(1, k), REAL[w_dtype], dw.data_ptr() if need_w else None, max(1, k))
+        return dx if dx is None or len(x_shape) == 2 else dx.view(x_shape), dw, None
 
 
 def torch_scaled_linear(x, weight, grad_dtype=E4M3):
@@ -191,13 +182,13 @@ def torch_scaled_linear(x, weight, grad_dtype=E4M3):
     ``grad_dtype`` is the 8-bit type of the output's gradient (e4m3 or e5m2).
     The result has x's type, the gradients their tensors' types.
     """
-    check_cuda("torch_scaled_linear", x, weight)
-    check_type("torch_scaled_linear", "x", x.dtype, REAL)
-    check_type("torch_scaled_linear", "weight", weight.dtype, REAL)
-    check_type("torch_scaled_linear", "grad_dtype", grad_dtype, FLOAT8)
+    device_of("torch_scaled_linear", x, weight)
+    code_of("torch_scaled_linear", "x", x.dtype, REAL)
+    code_of("torch_scaled_linear", "weight", weight.dtype, REAL)
+    code_of("torch_scaled_linear", "grad_dtype", grad_dtype, FLOAT8)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError("torch_scaled_linear: the last axis of x does not fit the weights")
     return _ScaledLinear.apply(x, weight, grad_dtype)
 
 
-__all__ = ["quantize_blocks", "scaled_gemm", "scaled_linear", "torch_scaled_linear", "NDTensorsError"]
+__all__ = ["quantize_blocks", "scaled_gemm", "scaled_linear", "torch_scaled_linear"]
