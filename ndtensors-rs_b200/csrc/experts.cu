@@ -17,7 +17,9 @@
 // bytes are its operand fragments as they are (the tokens' fragments are
 // loaded with the same order).  In the first product the two rows are the gate
 // and the up row of the same output, so silu(gate) * up needs no exchange.
-// The warps of a CTA split k and add their parts through shared memory.
+// Four warps share a tile of 16 rows, split its k and add their parts through
+// shared memory (with all 16 warps on a tile the barrier and the sums cost as
+// much as the product).
 //
 // The weights stream through a ring of cp.async copies in shared memory, each
 // lane reading back only what it copied itself, so no barrier stands between a
@@ -41,6 +43,8 @@ namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kTeam = 4;             // warps that share a tile
+constexpr int kTeams = kWarps / kTeam;
 constexpr int kMaxSlots = 4096;    // (token, chosen expert) pairs of one launch
 constexpr int kMaxTokens = 256;
 constexpr int kMaxExperts = 1024;
@@ -112,16 +116,15 @@ __device__ __forceinline__ uint4 row16(const T* row, int k, int n, bool on) {
   }
 }
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// The same into shared memory: an asynchronous copy where rows are whole vectors.
+// 16 bytes from p, of which n elements are the row's, into shared memory: an
+// asynchronous copy where rows are whole vectors.
 template <typename T, bool VEC>
-__device__ __forceinline__ void copy16(void* dst, const T* row, int k, int n, bool on) {
+__device__ __forceinline__ void copy16(void* dst, const T* p, int n, bool on) {
   if constexpr (VEC) {
-    const bool in = on && k < n;
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(in ? row + k : row),
-                 "r"(in ? 16 : 0)
-                 : "memory");
+    const bool in = on && n > 0;
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(p), "r"(in ? 16 : 0) : "memory");
   } else {
-    *reinterpret_cast<uint4*>(dst) = row16<T, false>(row, k, n, on);
+    *reinterpret_cast<uint4*>(dst) = row16<T, false>(p, 0, n, on);
   }
 }
 
@@ -327,43 +330,23 @@ struct Layer {
   static constexpr bool kScaled = sizeof(W) == 1;
   static constexpr bool kHalf = std::is_same_v<M, __half>;
   static constexpr int kRing = NT == 1 ? 8 : 6;          // steps in flight
-  static constexpr int kSlot = 2 * 512 + (kScaled ? 256 : 0);  // bytes of a warp's step: two rows, two scales a lane
-  static constexpr int kRed = kWarps * NT * 128;         // floats of a task's parts
+  static constexpr int kSlot = 2 * 512 + (kScaled ? 64 : 0);  // bytes of a warp's step: two rows a lane, two scales a row
+  static constexpr int kRed = kWarps * NT * 128;         // floats of the teams' parts
   static constexpr size_t kSmem = (size_t)kWarps * kRing * kSlot + 2 * kRed * 4;
 
-  // Where a lane's weights of a task are.  product 0: outputs 8 tile + g, their
-  // gate and up rows of w_in; product 1: rows 16 tile + g and + 8 of w_out.
-  struct Rows {
-    const W *a, *b;
-    const float *sa, *sb;
-    bool ona, onb;
-  };
-  __device__ static __forceinline__ Rows rows(const LayerArgs& a, int product, int expert, int tile, int g) {
-    Rows r;
-    const int ra = product == 0 ? tile * 8 + g : tile * 16 + g;
-    r.ona = ra < (product == 0 ? a.i : a.h);
-    r.onb = product == 0 ? r.ona : ra + 8 < a.h;
-    const int rb = !r.onb ? 0 : product == 0 ? a.i + ra : ra + 8;
-    const int qa = r.ona ? ra : 0;
-    const int64_t n = product == 0 ? 2 * a.i : a.h, k = product == 0 ? a.h : a.i;
-    const W* w = (const W*)(product == 0 ? a.e.w_in : a.e.w_out) + expert * n * k;
-    r.a = w + qa * k, r.b = w + rb * k;
-    if (kScaled) {
-      const int64_t kb = (k + 127) / 128;
-      const float* s = (product == 0 ? a.e.in_scales : a.e.out_scales) + expert * ((n + 127) / 128) * kb;
-      r.sa = s + qa / 128 * kb, r.sb = s + rb / 128 * kb;
-    }
-    return r;
-  }
-
-  // The stream of steps that a warp copies ahead of their use.
+  // The stream of steps that a warp copies ahead of their use.  product 0:
+  // outputs 8 tile + g, their gate and up rows of w_in; product 1: rows
+  // 16 tile + g and + 8 of w_out.
   struct Feed {
     int product, task, step, slot;
-    Rows r;
+    const W *a, *b;  // the lane's two rows
+    const float *sa, *sb;
+    bool ona, onb;
   };
 
   __device__ static void run(const LayerArgs& a, Lists& L, int* scratch, unsigned char* dyn) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int team = warp / kTeam, part = warp % kTeam;
     const int g = lane >> 2, q = lane & 3;  // row (and token) of the lane, quarter of k
     unsigned char* ring = dyn + (size_t)warp * kRing * kSlot;
     float* red = reinterpret_cast<float*>(dyn + (size_t)kWarps * kRing * kSlot);
@@ -381,37 +364,53 @@ struct Layer {
     grid.sync();
     route<NT>(a, L, scratch);
 
-    // this warp's steps of k in each product, and the tasks
+    // this warp's steps of k in each product; the tiles are dealt to the CTAs in even runs, to their teams in turn
     const int steps0 = (a.h + S::kK - 1) / S::kK, steps1 = (a.i + S::kK - 1) / S::kK;
-    const int lo0 = steps0 * warp / kWarps, hi0 = steps0 * (warp + 1) / kWarps;
-    const int lo1 = steps1 * warp / kWarps, hi1 = steps1 * (warp + 1) / kWarps;
+    const int lo0 = steps0 * part / kTeam, hi0 = steps0 * (part + 1) / kTeam;
+    const int lo1 = steps1 * part / kTeam, hi1 = steps1 * (part + 1) / kTeam;
+    auto share = [&](int tasks, int cta) { return (int)((int64_t)tasks * cta / gridDim.x); };
     const int tasks0 = L.units * tiles0, tasks1 = L.units * tiles1;
+    const int first0 = share(tasks0, blockIdx.x) + team, end0 = share(tasks0, blockIdx.x + 1);
+    const int first1 = share(tasks1, blockIdx.x) + team, end1 = share(tasks1, blockIdx.x + 1);
 
-    Feed f{0, (int)blockIdx.x, lo0, 0, {}};
+    Feed f;
+    f.product = 0, f.task = first0, f.slot = 0;
     auto settle = [&] {  // onto the next task that has steps for this warp
-      if (f.product == 0 && (f.task >= tasks0 || lo0 == hi0)) f.product = 1, f.task = blockIdx.x, f.step = lo1;
-      if (f.product == 1 && (f.task >= tasks1 || lo1 == hi1)) f.product = 2;
-      if (f.product < 2) {
-        const int tiles = f.product == 0 ? tiles0 : tiles1;
-        const int u = f.task / tiles;
-        f.r = rows(a, f.product, L.unit_expert[u], f.task - u * tiles, g);
+      if (f.product == 0 && (f.task >= end0 || lo0 == hi0)) f.product = 1, f.task = first1;
+      if (f.product == 1 && (f.task >= end1 || lo1 == hi1)) f.product = 2;
+      if (f.product == 2) return;
+      const bool p0 = f.product == 0;
+      f.step = p0 ? lo0 : lo1;
+      const int tiles = p0 ? tiles0 : tiles1, u = f.task / tiles, tile = f.task - u * tiles;
+      const int64_t expert = L.unit_expert[u];
+      const int ra = p0 ? tile * 8 + g : tile * 16 + g, n = p0 ? 2 * a.i : a.h, k = p0 ? a.h : a.i;
+      f.ona = ra < (p0 ? a.i : a.h);
+      f.onb = p0 ? f.ona : ra + 8 < a.h;
+      const int qa = f.ona ? ra : 0, qb = !f.onb ? 0 : p0 ? a.i + ra : ra + 8;
+      const W* w = (const W*)(p0 ? a.e.w_in : a.e.w_out) + expert * n * k + f.step * S::kK + q * S::kPerLane;
+      f.a = w + (int64_t)qa * k, f.b = w + (int64_t)qb * k;
+      if (kScaled) {
+        const int kb = (k + 127) / 128;
+        const float* sc = (p0 ? a.e.in_scales : a.e.out_scales) + expert * ((n + 127) / 128) * kb;
+        f.sa = sc + (qa >> 7) * kb, f.sb = sc + (qb >> 7) * kb;
       }
     };
     auto feed = [&] {  // copy the next step; an empty group at the end of the stream
       if (f.product < 2) {
         unsigned char* at = ring + f.slot * kSlot + lane * 16;
-        const int n = f.product == 0 ? a.h : a.i, k = f.step * S::kK + q * S::kPerLane;
-        copy16<W, VEC>(at, f.r.a, k, n, f.r.ona);
-        copy16<W, VEC>(at + 512, f.r.b, k, n, f.r.onb);
-        if (kScaled) {
+        const int n = (f.product == 0 ? a.h : a.i) - (f.step * S::kK + q * S::kPerLane);  // elements from here to the row's end
+        copy16<W, VEC>(at, f.a, n, f.ona);
+        copy16<W, VEC>(at + 512, f.b, n, f.onb);
+        f.a += S::kK, f.b += S::kK;
+        if (kScaled && q == 0) {
           const int kb = f.step * S::kK / 128;
-          const uint32_t sc = smem_u32(ring + f.slot * kSlot + 1024 + lane * 8);
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc), "l"(f.r.sa + kb) : "memory");
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 4), "l"(f.r.sb + kb) : "memory");
+          const uint32_t sc = smem_u32(ring + f.slot * kSlot + 1024 + g * 8);
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc), "l"(f.sa + kb) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 4), "l"(f.sb + kb) : "memory");
         }
         if (++f.slot == kRing) f.slot = 0;
         if (++f.step == (f.product == 0 ? hi0 : hi1)) {
-          f.task += gridDim.x, f.step = f.product == 0 ? lo0 : lo1;
+          f.task += kTeams;
           settle();
         }
       }
@@ -423,11 +422,12 @@ struct Layer {
     // take the oldest step: its two rows' pairs and scales
     auto take = [&](uint32_t* pa, uint32_t* pb, float& fa, float& fb) {
       asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      if (kScaled) __syncwarp();  // the scales were copied by the row's first lane (and the last ones have been read)
       const unsigned char* at = ring + slot * kSlot;
       S::pairs(*reinterpret_cast<const uint4*>(at + lane * 16), pa);
       S::pairs(*reinterpret_cast<const uint4*>(at + 512 + lane * 16), pb);
       if (kScaled) {
-        const float2 sc = *reinterpret_cast<const float2*>(at + 1024 + lane * 8);
+        const float2 sc = *reinterpret_cast<const float2*>(at + 1024 + g * 8);
         fa = sc.x, fb = sc.y;
       }
       if (++slot == kRing) slot = 0;
@@ -437,18 +437,18 @@ struct Layer {
       acc[0] = fmaf(part[0], fa, acc[0]), acc[1] = fmaf(part[1], fa, acc[1]);
       acc[2] = fmaf(part[2], fb, acc[2]), acc[3] = fmaf(part[3], fb, acc[3]);
     };
-    auto park = [&](float (*acc)[4]) {  // this warp's part of the task, for the warps that finish it
-      float* at = red + parity * kRed;
+    auto park = [&](float (*acc)[4]) {  // this warp's part of the tile, for its team
+      float* at = red + parity * kRed + team * kTeam * NT * 128;
 #pragma unroll
       for (int j = 0; j < NT; j++)
-        *reinterpret_cast<float4*>(at + ((warp * NT + j) * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
-      __syncthreads();  // one barrier a task: the parts alternate between two buffers
+        *reinterpret_cast<float4*>(at + ((part * NT + j) * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kTeam * 32) : "memory");  // one a tile: two buffers alternate
       parity ^= 1;
-      return at;
+      return (const float*)at;
     };
 
-    // ---- first product: tasks of 8 outputs of one expert
-    for (int task = blockIdx.x; task < tasks0; task += gridDim.x) {
+    // ---- first product: tiles of 8 outputs of one expert
+    for (int task = first0; task < end0; task += kTeams) {
       const int u = task / tiles0, i0 = (task - u * tiles0) * 8;
       const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(NT * 8, L.first[e + 1] - n0);
       const M* xr[NT];
@@ -459,56 +459,51 @@ struct Layer {
         const int k = s * S::kK + q * S::kPerLane;
         uint32_t pa[S::kPairs], pb[S::kPairs];
         float fa, fb;
-        alignas(16) uint32_t px[NT][S::kPairs];
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-          if (j * 8 < n)
-#pragma unroll
-            for (int v = 0; v < S::kPairs / 4; v++)
-              *reinterpret_cast<uint4*>(px[j] + 4 * v) = row16<M, VEC>(xr[j], k + 8 * v, a.h, j * 8 + g < n);
         take(pa, pb, fa, fb);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
           if (j * 8 >= n) break;
-          float part[4] = {};
-          float* to = kScaled ? part : acc[j];
+          alignas(16) uint32_t px[S::kPairs];
 #pragma unroll
-          for (int v = 0; v < S::kPairs; v += 2) mma<M>(to, pa[v], pb[v], pa[v + 1], pb[v + 1], px[j][v], px[j][v + 1]);
-          if (kScaled) add_scaled(acc[j], part, fa, fb);
+          for (int v = 0; v < S::kPairs / 4; v++)
+            *reinterpret_cast<uint4*>(px + 4 * v) = row16<M, VEC>(xr[j], k + 8 * v, a.h, j * 8 + g < n);
+          float sum[4] = {};
+          float* to = kScaled ? sum : acc[j];
+#pragma unroll
+          for (int v = 0; v < S::kPairs; v += 2) mma<M>(to, pa[v], pb[v], pa[v + 1], pb[v + 1], px[v], px[v + 1]);
+          if (kScaled) add_scaled(acc[j], sum, fa, fb);
         }
       }
       const float* parts = park(acc);
       // accumulator (row g: gate; row g + 8: up; columns 2 q, 2 q + 1) of column tile j
-      const int turn = (warp + kWarps - (task / gridDim.x * 2 * NT) % kWarps) % kWarps;  // which warps finish goes round
-      if (turn < 2 * NT) {
-        const int o = turn * 32 + lane, j = o >> 6, ln = o >> 1 & 31, half = o & 1;
+      for (int o = part * 32 + lane; o < NT * 64; o += kTeam * 32) {
+        const int j = o >> 6, ln = o >> 1 & 31, half = o & 1;
         const int col = j * 8 + (ln & 3) * 2 + half, row = i0 + (ln >> 2);
-        if (col < n) {
-          float ga = 0.f, up = 0.f;
+        if (col >= n) continue;
+        float ga = 0.f, up = 0.f;
 #pragma unroll
-          for (int w = 0; w < kWarps; w++) {
-            const float* p = parts + ((w * NT + j) * 32 + ln) * 4 + half;
-            ga += p[0], up += p[2];
-          }
-          const int64_t slot_row = L.slots[n0 + col];
-          const float v = ga / (1.f + expf(-ga)) * up;  // rows past i: 0, the padding of b
-          if constexpr (kHalf) {
-            ((float*)a.b)[slot_row * a.ip + row] = v;
-            atomicMax(a.bmax + slot_row, __float_as_uint(fabsf(v)));
-          } else {
-            const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-            const float hf = __bfloat162float(hi);
-            __nv_bfloat16* p = (__nv_bfloat16*)a.b + slot_row * 2 * a.ip + row;
-            p[0] = hi;
-            p[a.ip] = __float2bfloat16_rn(isinf(hf) ? 0.f : v - hf);  // an infinite high part stands alone
-          }
+        for (int w = 0; w < kTeam; w++) {
+          const float* p = parts + ((w * NT + j) * 32 + ln) * 4 + half;
+          ga += p[0], up += p[2];
+        }
+        const int64_t slot_row = L.slots[n0 + col];
+        const float v = ga / (1.f + expf(-ga)) * up;  // rows past i: 0, the padding of b
+        if constexpr (kHalf) {
+          ((float*)a.b)[slot_row * a.ip + row] = v;
+          atomicMax(a.bmax + slot_row, __float_as_uint(fabsf(v)));
+        } else {
+          const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+          const float hf = __bfloat162float(hi);
+          __nv_bfloat16* p = (__nv_bfloat16*)a.b + slot_row * 2 * a.ip + row;
+          p[0] = hi;
+          p[a.ip] = __float2bfloat16_rn(isinf(hf) ? 0.f : v - hf);  // an infinite high part stands alone
         }
       }
     }
     grid.sync();
 
-    // ---- second product: tasks of 16 rows of one expert
-    for (int task = blockIdx.x; task < tasks1; task += gridDim.x) {
+    // ---- second product: tiles of 16 rows of one expert
+    for (int task = first1; task < end1; task += kTeams) {
       const int u = task / tiles1, tile = task - u * tiles1, r0 = tile * 16;
       const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(NT * 8, L.first[e + 1] - n0);
       const char* br[NT];
@@ -533,15 +528,17 @@ struct Layer {
         const int k = s * S::kK + q * S::kPerLane;
         uint32_t pa[S::kPairs], pb[S::kPairs];
         float fa, fb;
-        alignas(16) uint32_t hi[NT][S::kPairs], lo[NT][S::kPairs];
+        take(pa, pb, fa, fb);
 #pragma unroll
         for (int j = 0; j < NT; j++) {
           if (j * 8 >= n) break;
+          float sum[4] = {};
+          float* to = kScaled ? sum : acc[j];
 #pragma unroll
           for (int v = 0; v < S::kPairs / 4; v++) {
             const int kk = k + 8 * v;
             const bool on = j * 8 + g < n && kk < a.ip;
-            const uint4 zero = make_uint4(0, 0, 0, 0);
+            alignas(16) uint32_t hi[4] = {}, lo[4] = {};
             if constexpr (kHalf) {
               const float4* p = reinterpret_cast<const float4*>((const float*)br[j] + kk);
               const float4 f0 = on ? p[0] : make_float4(0, 0, 0, 0), f1 = on ? p[1] : make_float4(0, 0, 0, 0);
@@ -549,30 +546,24 @@ struct Layer {
 #pragma unroll
               for (int c = 0; c < 4; c++) {
                 const float y0 = x[2 * c] * up[j], y1 = x[2 * c + 1] * up[j];
-                hi[j][4 * v + c] = pack2<M>(y0, y1);
-                const float2 hf = unpack2<M>(hi[j][4 * v + c]);
+                hi[c] = pack2<M>(y0, y1);
+                const float2 hf = unpack2<M>(hi[c]);
                 // (an infinite high part stands alone: no inf - inf)
-                lo[j][4 * v + c] = pack2<M>(isinf(hf.x) ? 0.f : y0 - hf.x, isinf(hf.y) ? 0.f : y1 - hf.y);
+                lo[c] = pack2<M>(isinf(hf.x) ? 0.f : y0 - hf.x, isinf(hf.y) ? 0.f : y1 - hf.y);
               }
-            } else {
+            } else if (on) {
               const __nv_bfloat16* p = (const __nv_bfloat16*)br[j] + kk;
-              *reinterpret_cast<uint4*>(hi[j] + 4 * v) = on ? *reinterpret_cast<const uint4*>(p) : zero;
-              *reinterpret_cast<uint4*>(lo[j] + 4 * v) = on ? *reinterpret_cast<const uint4*>(p + a.ip) : zero;
+              *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(p);
+              *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(p + a.ip);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+              const int m = 4 * v + c;
+              mma<M>(to, pa[m], pb[m], pa[m + 1], pb[m + 1], hi[c], hi[c + 1]);
+              mma<M>(to, pa[m], pb[m], pa[m + 1], pb[m + 1], lo[c], lo[c + 1]);
             }
           }
-        }
-        take(pa, pb, fa, fb);
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-          if (j * 8 >= n) break;
-          float part[4] = {};
-          float* to = kScaled ? part : acc[j];
-#pragma unroll
-          for (int v = 0; v < S::kPairs; v += 2) {
-            mma<M>(to, pa[v], pb[v], pa[v + 1], pb[v + 1], hi[j][v], hi[j][v + 1]);
-            mma<M>(to, pa[v], pb[v], pa[v + 1], pb[v + 1], lo[j][v], lo[j][v + 1]);
-          }
-          if (kScaled) add_scaled(acc[j], part, fa, fb);
+          if (kScaled) add_scaled(acc[j], sum, fa, fb);
         }
       }
       if constexpr (kHalf) {
@@ -582,24 +573,23 @@ struct Layer {
           for (int c = 0; c < 4; c++) acc[j][c] *= down[j][c & 1];
       }
       const float* parts = park(acc);
-      const int turn = (warp + kWarps - (task / gridDim.x * 4) % kWarps) % kWarps;
-      if (turn >= 4) continue;
+      // warp `part` finishes accumulator `part` of every lane
 #pragma unroll
       for (int j = 0; j < NT; j++) {
-        const int col = j * 8 + (lane & 3) * 2 + (turn & 1), row = r0 + (lane >> 2) + (turn & 2) * 4;
+        const int col = j * 8 + (lane & 3) * 2 + (part & 1), row = r0 + (lane >> 2) + (part & 2) * 4;
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; w++) s += parts[((w * NT + j) * 32 + lane) * 4 + turn];
+        for (int w = 0; w < kTeam; w++) s += parts[((w * NT + j) * 32 + lane) * 4 + part];
         if (col < n && row < a.h) a.o[(int64_t)L.slots[n0 + col] * a.h + row] = s;
       }
       if (NT == 1) {
-        // the warp that finishes a row tile's last part (of 4 a unit) sums the tokens' experts there
+        // the warp that finishes a row tile's last part (of kTeam a unit) sums the tokens' experts there
         __threadfence();
         __syncwarp();
         unsigned before = 0;
         if (lane == 0) before = atomicAdd(a.done + tile, 1u);
         before = __shfl_sync(~0u, before, 0);
-        if (before == 4u * L.units - 1) {
+        if (before == (unsigned)(kTeam * L.units - 1)) {
           __threadfence();
           for (int c = lane; c < a.tokens * 16; c += 32) combine(a, c >> 4, r0 + (c & 15));
         }
