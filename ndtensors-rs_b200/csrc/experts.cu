@@ -11,65 +11,82 @@
 // a launch's latency overlap saves) and every phase spreads its rows over all
 // SMs.
 //
-// Products run on the warp-level tensor cores with the weights as the 16-row
-// operand and up to 8 tokens a column tile: a lane copies 16 contiguous bytes
-// of two weight rows, and since the order of k within a product is free, those
-// bytes are its operand fragments as they are (the tokens' fragments are
-// loaded with the same order).  In the first product the two rows are the gate
-// and the up row of the same output, so silu(gate) * up needs no exchange.
-// Four warps share a tile of 16 rows, split its k and add their parts through
-// shared memory (with all 16 warps on a tile the barrier and the sums cost as
-// much as the product).
+// Products run on the warp-level tensor cores (mma.sync) with the weights as
+// the 16-row operand and up to 8 tokens a column tile: with so few columns the
+// tensor core is never what is waited for.  In the first product a tile is 8
+// gate rows and the 8 up rows of the same outputs, so silu(gate) * up needs no
+// exchange.
 //
-// The weights stream through a ring of cp.async copies in shared memory, each
-// lane reading back only what it copied itself, so no barrier stands between a
-// copy and its use.  The ring runs across tasks, and from the first product
-// into the second before the grid barrier between them.
+// The weights stream through a ring of stages in shared memory, 16 rows x 2 KB
+// each; 16 warps split a stage's k and add their parts through shared memory
+// at a tile's end.  The ring runs across tiles, and from the first product
+// into the second before the grid barrier between them.  One warp fills it.
+// Rows that are multiples of 128 bytes come as two tensor copies a stage (8
+// rows x 16 pieces of 128 bytes, swizzled so that ldmatrix meets no bank
+// conflict); others of whole 16-byte vectors as 16 bulk copies of 2 KB, rows
+// 2064 bytes apart, which the copy engine takes at 70 - 85 ns each, below the
+// rate of HBM; the rest by plain loads of four warps.  Lanes that copied their
+// own fragments (cp.async) spent 110 instructions on each KB: 3.2 TB/s.
 //
 // All sums are in 32 bits.  The activations b enter the second product as the
 // sum of two 16-bit numbers (16 or 22 bits of mantissa), so it loses nothing
 // against a 32-bit b; for float16 each row of b is scaled by a power of two
-// first, since b may be out of that type's range.
+// first, since b may be out of that type's range.  8-bit weights multiply in
+// float16, x scaled likewise.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 
-#include "model_ops.h"
+#include "mbarrier.h"
 
 namespace ndt {
 namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
-constexpr int kWarps = kThreads / 32;
-constexpr int kTeam = 4;             // warps that share a tile
-constexpr int kTeams = kWarps / kTeam;
-constexpr int kMaxSlots = 4096;    // (token, chosen expert) pairs of one launch
+constexpr int kConsumers = 16;       // warps that multiply
+constexpr int kMaxWarps = kConsumers + 4;
+enum Copy { kPlain, kBulk, kTensor };  // how rows come: by element, in 16-byte vectors, in 128-byte pieces
+__host__ __device__ constexpr int warps_of(int copy) { return kConsumers + (copy == kPlain ? 4 : 1); }
+constexpr int kMaxSlots = 2048;      // (token, chosen expert) pairs of one launch
 constexpr int kMaxTokens = 256;
 constexpr int kMaxExperts = 1024;
-constexpr int kGroup = 8;          // tokens of one router product
-constexpr int kMaxUnits = kMaxExperts + kMaxSlots / 32;
+constexpr int kGroup = 8;            // tokens of one router product
+constexpr int kRowBytes = 2048;      // of a row in one stage
+constexpr int kRowPitch = kRowBytes + 16;
+constexpr int kStageBytes = 33 * 1024;  // 16 rows of either pitch, a multiple of the swizzle's 1024
+static_assert(16 * kRowPitch <= kStageBytes, "");
+constexpr int kMaxStages = 6;
 
 struct LayerArgs {
   ExpertArgs e;
   int tokens, experts, top, h, i;
   int ip;           // i rounded up to 8: the pitch of b's rows
+  int unit;         // tokens of an expert that a CTA takes at a time
+  int stages;
+  int xpitch, bpitch;  // bytes of a token's row of x / of b's parts in shared memory
+  int op_bytes;     // shared memory for either
   float* logits;    // [tokens, experts]
-  void* b;          // [slots, 2, ip] bf16 high and low parts, or [slots, ip] floats (float16 layers)
+  float* b;         // [slots, ip]
   float* o;         // [slots, h]
   unsigned* bmax;   // [slots] bits of max |b|
-  unsigned* done;   // [row tiles of w_out] parts of a tile that are finished
+  unsigned* xmax;   // [tokens] bits of max |x| (8-bit layers)
+  unsigned* arrived;  // CTAs whose part of b is written
+  int* flag;        // set when a bounded wait ran out
+};
+
+struct Maps {
+  CUtensorMap m[2];  // w_in and w_out
 };
 
 template <typename M>
 __device__ __forceinline__ void mma(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same_v<M, __half>)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -90,13 +107,10 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
   else
     return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
 }
-// Two 8-bit weights (the low 16 bits of w) as a pair of M: exact in both types.
-template <typename M>
+// Two 8-bit weights (the low 16 bits of w) as a pair of float16: exact.
 __device__ __forceinline__ uint32_t widen(uint32_t w) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
-  if constexpr (std::is_same_v<M, __half>) return *reinterpret_cast<const uint32_t*>(&h);
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  return pack2<__nv_bfloat16>(f.x, f.y);
+  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 // 16 bytes of a row of n elements from element k; zeros outside it.
@@ -115,43 +129,30 @@ __device__ __forceinline__ uint4 row16(const T* row, int k, int n, bool on) {
     return v;
   }
 }
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 bytes from p, of which n elements are the row's, into shared memory: an
-// asynchronous copy where rows are whole vectors.
-template <typename T, bool VEC>
-__device__ __forceinline__ void copy16(void* dst, const T* p, int n, bool on) {
-  if constexpr (VEC) {
-    const bool in = on && n > 0;
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(p), "r"(in ? 16 : 0) : "memory");
-  } else {
-    *reinterpret_cast<uint4*>(dst) = row16<T, false>(p, 0, n, on);
-  }
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, int bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes),
+               "r"(bar)
+               : "memory");
 }
-
-// The weights' side of one step of k: a lane's 16 bytes of a row as pairs of M.
-template <typename W, typename M>
-struct Step {
-  static constexpr int kPerLane = 16 / sizeof(W);  // k of a lane
-  static constexpr int kK = 4 * kPerLane;          // k of the warp
-  static constexpr int kPairs = kPerLane / 2;
-  __device__ static __forceinline__ void pairs(const uint4& v, uint32_t* p) {
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    if constexpr (sizeof(W) == 2) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) p[j] = w[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++) p[2 * j] = widen<M>(w[j] & 0xffff), p[2 * j + 1] = widen<M>(w[j] >> 16);
-    }
-  }
-};
+// 8 rows x 16 pieces of 128 bytes, piece by piece, 128-byte swizzle.
+__device__ __forceinline__ void tensor_copy(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int piece) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(0), "r"(row), "r"(piece)
+      : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
 
 struct Lists {
   uint16_t chosen[kMaxSlots];     // the expert of each slot (token * top + place)
   uint16_t slots[kMaxSlots];      // slots expert by expert, in order
-  int first[kMaxExperts + 1];     // where an expert's slots start
-  uint16_t unit_expert[kMaxUnits];  // an expert with up to 8 NT of its slots
-  uint16_t unit_first[kMaxUnits];   // ... from this place of `slots` on
+  int first[kMaxExperts + 1];     // where an expert's slots start (with few slots only [e + 1] of its experts)
+  uint16_t unit_expert[kMaxSlots];  // an expert with up to `unit` of its slots
+  uint16_t unit_first[kMaxSlots];   // ... from this place of `slots` on
   int units;
 };
 
@@ -164,9 +165,8 @@ __device__ __forceinline__ uint32_t sortable(float f) {
 
 // One token's choice, by a warp that holds PER of its products a lane.
 template <int PER>
-__device__ __forceinline__ void choose(const LayerArgs& a, int t, Lists& L) {
+__device__ __forceinline__ void choose(const LayerArgs& a, const float* l, int t, Lists& L) {
   const int lane = threadIdx.x & 31;
-  const float* l = a.logits + (int64_t)t * a.experts;
   float v[PER];
   uint32_t key[PER];
   float top = -INFINITY, sum = 0.f;
@@ -214,19 +214,54 @@ __device__ __forceinline__ void choose(const LayerArgs& a, int t, Lists& L) {
 
 // Choose the experts of every token (every CTA does all of them: a barrier
 // would cost more) and list the slots of every expert.
-template <int NT>
-__device__ __forceinline__ void route(const LayerArgs& a, Lists& L, int* scratch) {
+template <int kWarps>
+__device__ __forceinline__ void route(const LayerArgs& a, Lists& L, int* scratch, float* space, int space_bytes) {
+  constexpr int kThreads = kWarps * 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // all products at once where they fit: a load for each token in turn waits for L2 each time
+  const int all = a.tokens * a.experts;
+  const float* l = a.logits;
+  if (all * 4 <= space_bytes) {
+#pragma unroll 4
+    for (int c = threadIdx.x; c < all; c += kThreads) space[c] = __ldcg(a.logits + c);
+    __syncthreads();
+    l = space;
+  }
   for (int t = warp; t < a.tokens; t += kWarps) {
+    const float* lt = l + t * a.experts;
     if (a.experts <= 64)
-      choose<2>(a, t, L);
+      choose<2>(a, lt, t, L);
     else if (a.experts <= 256)
-      choose<8>(a, t, L);
+      choose<8>(a, lt, t, L);
     else
-      choose<32>(a, t, L);
+      choose<32>(a, lt, t, L);
   }
   __syncthreads();
   const int slots = a.tokens * a.top;
+  if (slots <= 32) {  // one warp: a slot's place is the number of slots before it by (expert, slot)
+    if (warp == 0) {
+      const int e = lane < slots ? L.chosen[lane] : 0xffff;
+      const unsigned same = __match_any_sync(~0u, e);
+      const int rank = __popc(same & ((1u << lane) - 1));
+      int before = 0, units = 0;  // slots, and units, of lower experts
+      for (int s = 0; s < slots; s++) {
+        const int f = __shfl_sync(~0u, e, s), r = __shfl_sync(~0u, rank, s);
+        if (f < e) before++, units += r % a.unit == 0;
+      }
+      const int place = before + rank;
+      if (lane < slots) {
+        L.slots[place] = (uint16_t)lane;
+        if (rank % a.unit == 0) {
+          L.unit_expert[units + rank / a.unit] = (uint16_t)e, L.unit_first[units + rank / a.unit] = (uint16_t)place;
+          if (rank == 0) L.first[e + 1] = before + __popc(same);
+        }
+      }
+      const int all = __popc(__ballot_sync(~0u, lane < slots && rank % a.unit == 0));
+      if (lane == 0) L.units = all;
+    }
+    __syncthreads();
+    return;
+  }
   for (int e = warp; e < a.experts; e += kWarps) {
     int n = 0;
     for (int s = 0; s < slots; s += 32) n += __popc(__ballot_sync(~0u, s + lane < slots && L.chosen[s + lane] == e));
@@ -236,7 +271,7 @@ __device__ __forceinline__ void route(const LayerArgs& a, Lists& L, int* scratch
   if (warp == 0) {
     int at = 0, units = 0;
     for (int e0 = 0; e0 < a.experts; e0 += 32) {
-      const int e = e0 + lane, n = e < a.experts ? scratch[e] : 0, u = (n + 8 * NT - 1) / (8 * NT);
+      const int e = e0 + lane, n = e < a.experts ? scratch[e] : 0, u = (n + a.unit - 1) / a.unit;
       int x = n, y = u;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -246,7 +281,7 @@ __device__ __forceinline__ void route(const LayerArgs& a, Lists& L, int* scratch
       if (e < a.experts) L.first[e] = at + x - n;
       for (int k = 0; k < u; k++) {
         L.unit_expert[units + y - u + k] = (uint16_t)e;
-        L.unit_first[units + y - u + k] = (uint16_t)(at + x - n + k * 8 * NT);
+        L.unit_first[units + y - u + k] = (uint16_t)(at + x - n + k * a.unit);
       }
       at += __shfl_sync(~0u, x, 31), units += __shfl_sync(~0u, y, 31);
     }
@@ -280,15 +315,19 @@ __device__ __forceinline__ float transpose_sum(float* v) {
   return v[0];
 }
 
-// Router products: a CTA takes RE experts and up to 8 tokens.
-template <typename X, bool VEC, int RE>
+// Router products: a CTA takes RE experts and up to 8 tokens (MAX: and their
+// largest magnitudes).
+template <typename X, int COPY, bool MAX, int RE>
 __device__ __forceinline__ void router(const LayerArgs& a, float* red) {
   static_assert(RE * kGroup <= 32, "");
+  constexpr int kWarps = warps_of(COPY), kThreads = kWarps * 32;
+  constexpr bool VEC = COPY != kPlain;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = (a.tokens + kGroup - 1) / kGroup, es = (a.experts + RE - 1) / RE;
   for (int u = blockIdx.x; u < es * groups; u += gridDim.x) {
     const int e0 = u % es * RE, t0 = u / es * kGroup, nt = min(kGroup, a.tokens - t0), ne = min(RE, a.experts - e0);
     float acc[32] = {};
+    unsigned top[kGroup] = {};
     const X* r = (const X*)a.e.router + (int64_t)e0 * a.h;
     const X* x = (const X*)a.e.x + (int64_t)t0 * a.e.ldx;
     for (int k = threadIdx.x * 8; k < a.h; k += kThreads * 8) {
@@ -301,6 +340,9 @@ __device__ __forceinline__ void router(const LayerArgs& a, float* red) {
       for (int t = 0; t < kGroup; t++) {
         if (t >= nt) break;
         const X* xe = reinterpret_cast<const X*>(&xv[t]);
+        if (MAX)
+#pragma unroll
+          for (int c = 0; c < 8; c++) top[t] = max(top[t], __float_as_uint(fabsf(to_f32<X>(xe[c]))));
 #pragma unroll
         for (int j = 0; j < RE; j++) {
           const X* re = reinterpret_cast<const X*>(&rv[j]);
@@ -310,6 +352,13 @@ __device__ __forceinline__ void router(const LayerArgs& a, float* red) {
       }
     }
     red[warp * 32 + lane] = transpose_sum(acc);
+    if (MAX && e0 == 0) {
+#pragma unroll
+      for (int t = 0; t < kGroup; t++) {
+        const unsigned m = __reduce_max_sync(~0u, top[t]);
+        if (lane == 0) red[(kMaxWarps + t) * 32 + warp] = __uint_as_float(m);
+      }
+    }
     __syncthreads();
     if (warp == 0) {
       float s = 0.f;
@@ -318,318 +367,442 @@ __device__ __forceinline__ void router(const LayerArgs& a, float* red) {
       const int j = lane / kGroup, t = lane % kGroup;
       if (j < ne && t < nt) a.logits[(int64_t)(t0 + t) * a.experts + e0 + j] = s;
     }
+    if (MAX && e0 == 0 && threadIdx.x < nt) {
+      unsigned m = 0;
+      for (int w = 0; w < kWarps; w++) m = max(m, __float_as_uint(red[(kMaxWarps + threadIdx.x) * 32 + w]));
+      a.xmax[t0 + threadIdx.x] = m;
+    }
     __syncthreads();
   }
 }
 
-// W: the weights' type, M: x's and the products' type, VEC: rows are whole
-// 16-byte vectors, NT: column tiles of 8 tokens that a product takes at a time.
-template <typename W, typename M, bool VEC, int NT>
+// W: the weights' type, X: x's and y's, M: the products', COPY: how rows come,
+// NT: column tiles of 8 tokens that a product takes at a time.
+template <typename W, typename X, typename M, int COPY, int NT>
 struct Layer {
-  using S = Step<W, M>;
+  static constexpr bool VEC = COPY != kPlain;
+  static constexpr int kWarps = warps_of(COPY), kThreads = kWarps * 32;
   static constexpr bool kScaled = sizeof(W) == 1;
   static constexpr bool kHalf = std::is_same_v<M, __half>;
-  static constexpr int kRing = NT == 1 ? 8 : 6;          // steps in flight
-  static constexpr int kSlot = 2 * 512 + (kScaled ? 64 : 0);  // bytes of a warp's step: two rows a lane, two scales a row
-  static constexpr int kRed = kWarps * NT * 128;         // floats of the teams' parts
-  static constexpr size_t kSmem = (size_t)kWarps * kRing * kSlot + 2 * kRed * 4;
+  static constexpr int kRowK = kRowBytes / (int)sizeof(W);    // k of a stage
+  static constexpr int kStepK = kScaled ? 128 : 32;           // k of a warp's step: one scale, or two MMAs
+  static constexpr int kStepBytes = kStepK * (int)sizeof(W);
+  static constexpr int kRed = kConsumers * NT * 128;          // floats of a tile's parts
 
-  // The stream of steps that a warp copies ahead of their use.  product 0:
-  // outputs 8 tile + g, their gate and up rows of w_in; product 1: rows
-  // 16 tile + g and + 8 of w_out.
-  struct Feed {
-    int product, task, step, slot;
-    const W *a, *b;  // the lane's two rows
-    const float *sa, *sb;
-    bool ona, onb;
-  };
+  // What brings a row whose largest value is at `most` into float16's range,
+  // 2^-x, or (sign 1) what takes it back.
+  __device__ static __forceinline__ float power(const unsigned* most, int sign) {
+    const int ex = (int)(__ldcg(most) >> 23) - 127;
+    const int c = ex < -100 || ex > 127 ? 0 : min(ex, 126);  // tiny, infinite or NaN: as it is
+    return __uint_as_float((uint32_t)(127 + sign * c) << 23);
+  }
 
-  __device__ static void run(const LayerArgs& a, Lists& L, int* scratch, unsigned char* dyn) {
+  __device__ static void run(const LayerArgs& a, const CUtensorMap* maps, Lists& L, int* scratch, uint64_t* bars, volatile int* gave_up,
+                             unsigned char* dyn) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int team = warp / kTeam, part = warp % kTeam;
-    const int g = lane >> 2, q = lane & 3;  // row (and token) of the lane, quarter of k
-    unsigned char* ring = dyn + (size_t)warp * kRing * kSlot;
-    float* red = reinterpret_cast<float*>(dyn + (size_t)kWarps * kRing * kSlot);
+    const int g = lane >> 2;
+    unsigned char* op = dyn;                                        // x, then b, of the unit's tokens
+    float* red = reinterpret_cast<float*>(dyn + a.op_bytes);        // two buffers of parts
+    unsigned char* ring = dyn + a.op_bytes + 2 * kRed * 4;
+    ring += (1024 - (smem_u32(ring) & 1023)) & 1023;
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages;
+    __shared__ float back[NT * 8];  // what takes a token's results back from float16's range
     cg::grid_group grid = cg::this_grid();
 
+    if (threadIdx.x == 0) {
+      *gave_up = 0;
+      for (int st = 0; st < a.stages; st++) {
+        mbar_init(full + 8 * st, VEC ? 1 : kWarps - kConsumers);
+        mbar_init(empty + 8 * st, kConsumers);
+      }
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     if (a.tokens <= 8)
-      router<M, VEC, 1>(a, red);
+      router<X, COPY, kScaled, 1>(a, red);
     else
-      router<M, VEC, 4>(a, red);
+      router<X, COPY, kScaled, 4>(a, red);
     const int tiles0 = (a.i + 7) / 8, tiles1 = (a.h + 15) / 16;
-    for (int s = blockIdx.x * kThreads + threadIdx.x; s < max(a.tokens * a.top, tiles1); s += gridDim.x * kThreads) {
-      if (s < a.tokens * a.top) a.bmax[s] = 0;
-      if (s < tiles1) a.done[s] = 0;
-    }
+    if (kHalf)
+      for (int s = blockIdx.x * kThreads + threadIdx.x; s < a.tokens * a.top; s += gridDim.x * kThreads) a.bmax[s] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.arrived = 0;
     grid.sync();
-    route<NT>(a, L, scratch);
+    route<kWarps>(a, L, scratch, reinterpret_cast<float*>(ring), a.stages * kStageBytes);
+    // (plain writes to the ring before its first copies)
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
 
-    // this warp's steps of k in each product; the tiles are dealt to the CTAs in even runs, to their teams in turn
-    const int steps0 = (a.h + S::kK - 1) / S::kK, steps1 = (a.i + S::kK - 1) / S::kK;
-    const int lo0 = steps0 * part / kTeam, hi0 = steps0 * (part + 1) / kTeam;
-    const int lo1 = steps1 * part / kTeam, hi1 = steps1 * (part + 1) / kTeam;
+    // the tiles are dealt to the CTAs in even runs
     auto share = [&](int tasks, int cta) { return (int)((int64_t)tasks * cta / gridDim.x); };
-    const int tasks0 = L.units * tiles0, tasks1 = L.units * tiles1;
-    const int first0 = share(tasks0, blockIdx.x) + team, end0 = share(tasks0, blockIdx.x + 1);
-    const int first1 = share(tasks1, blockIdx.x) + team, end1 = share(tasks1, blockIdx.x + 1);
+    const int first0 = share(L.units * tiles0, blockIdx.x), end0 = share(L.units * tiles0, blockIdx.x + 1);
+    const int first1 = share(L.units * tiles1, blockIdx.x), end1 = share(L.units * tiles1, blockIdx.x + 1);
 
-    Feed f;
-    f.product = 0, f.task = first0, f.slot = 0;
-    auto settle = [&] {  // onto the next task that has steps for this warp
-      if (f.product == 0 && (f.task >= end0 || lo0 == hi0)) f.product = 1, f.task = first1;
-      if (f.product == 1 && (f.task >= end1 || lo1 == hi1)) f.product = 2;
-      if (f.product == 2) return;
-      const bool p0 = f.product == 0;
-      f.step = p0 ? lo0 : lo1;
-      const int tiles = p0 ? tiles0 : tiles1, u = f.task / tiles, tile = f.task - u * tiles;
-      const int64_t expert = L.unit_expert[u];
-      const int ra = p0 ? tile * 8 + g : tile * 16 + g, n = p0 ? 2 * a.i : a.h, k = p0 ? a.h : a.i;
-      f.ona = ra < (p0 ? a.i : a.h);
-      f.onb = p0 ? f.ona : ra + 8 < a.h;
-      const int qa = f.ona ? ra : 0, qb = !f.onb ? 0 : p0 ? a.i + ra : ra + 8;
-      const W* w = (const W*)(p0 ? a.e.w_in : a.e.w_out) + expert * n * k + f.step * S::kK + q * S::kPerLane;
-      f.a = w + (int64_t)qa * k, f.b = w + (int64_t)qb * k;
-      if (kScaled) {
-        const int kb = (k + 127) / 128;
-        const float* sc = (p0 ? a.e.in_scales : a.e.out_scales) + expert * ((n + 127) / 128) * kb;
-        f.sa = sc + (qa >> 7) * kb, f.sb = sc + (qb >> 7) * kb;
+    if (warp >= kConsumers) {
+      if (!VEC || warp == kConsumers) {
+        int stage = 0;
+        uint32_t phase = 0;
+        copy_tiles<0>(a, maps, L, first0, end0, tiles0, ring, full, empty, stage, phase, gave_up);
+        copy_tiles<1>(a, maps + 1, L, first1, end1, tiles1, ring, full, empty, stage, phase, gave_up);
+        // after a wait that gave up: let the copies in flight land before the CTA's memory goes
+        if (*gave_up)
+          for (int n = 0; n < 1000; n++) __nanosleep(1000);
+        __syncwarp();
       }
-    };
-    auto feed = [&] {  // copy the next step; an empty group at the end of the stream
-      if (f.product < 2) {
-        unsigned char* at = ring + f.slot * kSlot + lane * 16;
-        const int n = (f.product == 0 ? a.h : a.i) - (f.step * S::kK + q * S::kPerLane);  // elements from here to the row's end
-        copy16<W, VEC>(at, f.a, n, f.ona);
-        copy16<W, VEC>(at + 512, f.b, n, f.onb);
-        f.a += S::kK, f.b += S::kK;
-        if (kScaled && q == 0) {
-          const int kb = f.step * S::kK / 128;
-          const uint32_t sc = smem_u32(ring + f.slot * kSlot + 1024 + g * 8);
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc), "l"(f.sa + kb) : "memory");
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sc + 4), "l"(f.sb + kb) : "memory");
-        }
-        if (++f.slot == kRing) f.slot = 0;
-        if (++f.step == (f.product == 0 ? hi0 : hi1)) {
-          f.task += kTeams;
-          settle();
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
-    settle();
-    for (int p = 0; p < kRing - 1; p++) feed();
-    int slot = 0, parity = 0;
-    // take the oldest step: its two rows' pairs and scales
-    auto take = [&](uint32_t* pa, uint32_t* pb, float& fa, float& fb) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
-      if (kScaled) __syncwarp();  // the scales were copied by the row's first lane (and the last ones have been read)
-      const unsigned char* at = ring + slot * kSlot;
-      S::pairs(*reinterpret_cast<const uint4*>(at + lane * 16), pa);
-      S::pairs(*reinterpret_cast<const uint4*>(at + 512 + lane * 16), pb);
-      if (kScaled) {
-        const float2 sc = *reinterpret_cast<const float2*>(at + 1024 + g * 8);
-        fa = sc.x, fb = sc.y;
-      }
-      if (++slot == kRing) slot = 0;
-      feed();
-    };
-    auto add_scaled = [&](float* acc, const float* part, float fa, float fb) {
-      acc[0] = fmaf(part[0], fa, acc[0]), acc[1] = fmaf(part[1], fa, acc[1]);
-      acc[2] = fmaf(part[2], fb, acc[2]), acc[3] = fmaf(part[3], fb, acc[3]);
-    };
-    auto park = [&](float (*acc)[4]) {  // this warp's part of the tile, for its team
-      float* at = red + parity * kRed + team * kTeam * NT * 128;
-#pragma unroll
-      for (int j = 0; j < NT; j++)
-        *reinterpret_cast<float4*>(at + ((part * NT + j) * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
-      asm volatile("bar.sync %0, %1;" ::"r"(team + 1), "n"(kTeam * 32) : "memory");  // one a tile: two buffers alternate
-      parity ^= 1;
-      return (const float*)at;
-    };
-
-    // ---- first product: tiles of 8 outputs of one expert
-    for (int task = first0; task < end0; task += kTeams) {
-      const int u = task / tiles0, i0 = (task - u * tiles0) * 8;
-      const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(NT * 8, L.first[e + 1] - n0);
-      const M* xr[NT];
-#pragma unroll
-      for (int j = 0; j < NT; j++) xr[j] = (const M*)a.e.x + (int64_t)(j * 8 + g < n ? L.slots[n0 + j * 8 + g] / a.top : 0) * a.e.ldx;
-      float acc[NT][4] = {};
-      for (int s = lo0; s < hi0; s++) {
-        const int k = s * S::kK + q * S::kPerLane;
-        uint32_t pa[S::kPairs], pb[S::kPairs];
-        float fa, fb;
-        take(pa, pb, fa, fb);
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-          if (j * 8 >= n) break;
-          alignas(16) uint32_t px[S::kPairs];
-#pragma unroll
-          for (int v = 0; v < S::kPairs / 4; v++)
-            *reinterpret_cast<uint4*>(px + 4 * v) = row16<M, VEC>(xr[j], k + 8 * v, a.h, j * 8 + g < n);
-          float sum[4] = {};
-          float* to = kScaled ? sum : acc[j];
-#pragma unroll
-          for (int v = 0; v < S::kPairs; v += 2) mma<M>(to, pa[v], pb[v], pa[v + 1], pb[v + 1], px[v], px[v + 1]);
-          if (kScaled) add_scaled(acc[j], sum, fa, fb);
-        }
-      }
-      const float* parts = park(acc);
-      // accumulator (row g: gate; row g + 8: up; columns 2 q, 2 q + 1) of column tile j
-      for (int o = part * 32 + lane; o < NT * 64; o += kTeam * 32) {
-        const int j = o >> 6, ln = o >> 1 & 31, half = o & 1;
-        const int col = j * 8 + (ln & 3) * 2 + half, row = i0 + (ln >> 2);
-        if (col >= n) continue;
-        float ga = 0.f, up = 0.f;
-#pragma unroll
-        for (int w = 0; w < kTeam; w++) {
-          const float* p = parts + ((w * NT + j) * 32 + ln) * 4 + half;
-          ga += p[0], up += p[2];
-        }
-        const int64_t slot_row = L.slots[n0 + col];
-        const float v = ga / (1.f + expf(-ga)) * up;  // rows past i: 0, the padding of b
-        if constexpr (kHalf) {
-          ((float*)a.b)[slot_row * a.ip + row] = v;
-          atomicMax(a.bmax + slot_row, __float_as_uint(fabsf(v)));
-        } else {
-          const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-          const float hf = __bfloat162float(hi);
-          __nv_bfloat16* p = (__nv_bfloat16*)a.b + slot_row * 2 * a.ip + row;
-          p[0] = hi;
-          p[a.ip] = __float2bfloat16_rn(isinf(hf) ? 0.f : v - hf);  // an infinite high part stands alone
-        }
-      }
-    }
-    grid.sync();
-
-    // ---- second product: tiles of 16 rows of one expert
-    for (int task = first1; task < end1; task += kTeams) {
-      const int u = task / tiles1, tile = task - u * tiles1, r0 = tile * 16;
-      const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(NT * 8, L.first[e + 1] - n0);
-      const char* br[NT];
-      float down[NT][2], up[NT];
-#pragma unroll
-      for (int j = 0; j < NT; j++) {
-        const int sl = L.slots[n0 + min(j * 8 + g, n - 1)];
-        br[j] = (const char*)a.b + (int64_t)sl * a.ip * 4;
-        if constexpr (kHalf) {
-          // 2^-x of the slot's largest value, and back for the lane's two result columns
-          auto power = [&](int at, int sign) {
-            const int ex = (int)(a.bmax[at] >> 23) - 127;
-            const int c = ex < -100 || ex > 127 ? 0 : min(ex, 126);  // tiny, infinite or NaN: as it is
-            return __uint_as_float((uint32_t)(127 + sign * c) << 23);
-          };
-          up[j] = power(sl, -1);
-          for (int c = 0; c < 2; c++) down[j][c] = power(L.slots[n0 + min(j * 8 + 2 * q + c, n - 1)], 1);
-        }
-      }
-      float acc[NT][4] = {};
-      for (int s = lo1; s < hi1; s++) {
-        const int k = s * S::kK + q * S::kPerLane;
-        uint32_t pa[S::kPairs], pb[S::kPairs];
-        float fa, fb;
-        take(pa, pb, fa, fb);
-#pragma unroll
-        for (int j = 0; j < NT; j++) {
-          if (j * 8 >= n) break;
-          float sum[4] = {};
-          float* to = kScaled ? sum : acc[j];
-#pragma unroll
-          for (int v = 0; v < S::kPairs / 4; v++) {
-            const int kk = k + 8 * v;
-            const bool on = j * 8 + g < n && kk < a.ip;
-            alignas(16) uint32_t hi[4] = {}, lo[4] = {};
-            if constexpr (kHalf) {
-              const float4* p = reinterpret_cast<const float4*>((const float*)br[j] + kk);
-              const float4 f0 = on ? p[0] : make_float4(0, 0, 0, 0), f1 = on ? p[1] : make_float4(0, 0, 0, 0);
-              const float x[8] = {f0.x, f0.y, f0.z, f0.w, f1.x, f1.y, f1.z, f1.w};
-#pragma unroll
-              for (int c = 0; c < 4; c++) {
-                const float y0 = x[2 * c] * up[j], y1 = x[2 * c + 1] * up[j];
-                hi[c] = pack2<M>(y0, y1);
-                const float2 hf = unpack2<M>(hi[c]);
-                // (an infinite high part stands alone: no inf - inf)
-                lo[c] = pack2<M>(isinf(hf.x) ? 0.f : y0 - hf.x, isinf(hf.y) ? 0.f : y1 - hf.y);
-              }
-            } else if (on) {
-              const __nv_bfloat16* p = (const __nv_bfloat16*)br[j] + kk;
-              *reinterpret_cast<uint4*>(hi) = *reinterpret_cast<const uint4*>(p);
-              *reinterpret_cast<uint4*>(lo) = *reinterpret_cast<const uint4*>(p + a.ip);
-            }
-#pragma unroll
-            for (int c = 0; c < 4; c += 2) {
-              const int m = 4 * v + c;
-              mma<M>(to, pa[m], pb[m], pa[m + 1], pb[m + 1], hi[c], hi[c + 1]);
-              mma<M>(to, pa[m], pb[m], pa[m + 1], pb[m + 1], lo[c], lo[c + 1]);
-            }
-          }
-          if (kScaled) add_scaled(acc[j], sum, fa, fb);
-        }
-      }
-      if constexpr (kHalf) {
+    } else {
+      int stage = 0, parity = 0;
+      uint32_t phase = 0;
+      auto park = [&](float (*acc)[4]) {  // this warp's part of the tile, for the warps that finish it
+        float* at = red + parity * kRed;
 #pragma unroll
         for (int j = 0; j < NT; j++)
+          *reinterpret_cast<float4*>(at + ((warp * NT + j) * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+        consumers_sync();  // one a tile: two buffers alternate
+        parity ^= 1;
+        return (const float*)at;
+      };
+
+      // ---- first product: tiles of 8 outputs of one expert
+      int unit = -1;
+      for (int task = first0; task < end0; task++) {
+        const int u = task / tiles0, i0 = (task - u * tiles0) * 8;
+        const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(a.unit, L.first[e + 1] - n0);
+        if (u != unit) {
+          if (unit < 0 || a.tokens > 1) stage_x(a, L, n0, n, op, back);
+          unit = u;
+        }
+        float acc[NT][4] = {};
+        const int row_a = min(i0 + g, a.i - 1);
+        multiply<0>(a, acc, e, row_a, a.i + row_a, n, op, ring, full, empty, stage, phase, gave_up);
+        const float* parts = park(acc);
+        // accumulator (row g: gate; row g + 8: up; columns 2 q, 2 q + 1) of column tile j; which warps finish goes round
+        for (int o = ((warp + kConsumers - (task * 2 * NT) % kConsumers) % kConsumers) * 32 + lane; o < NT * 64; o += kConsumers * 32) {
+          const int j = o >> 6, ln = o >> 1 & 31, half = o & 1;
+          const int col = j * 8 + (ln & 3) * 2 + half, row = i0 + (ln >> 2);
+          if (col >= n || row >= a.i) continue;
+          float ga = 0.f, up = 0.f;
 #pragma unroll
-          for (int c = 0; c < 4; c++) acc[j][c] *= down[j][c & 1];
+          for (int w = 0; w < kConsumers; w++) {
+            const float* p = parts + ((w * NT + j) * 32 + ln) * 4 + half;
+            ga += p[0], up += p[2];
+          }
+          const int64_t slot = L.slots[n0 + col];
+          if (kScaled) ga *= back[col], up *= back[col];
+          const float v = ga / (1.f + expf(-ga)) * up;
+          a.b[slot * a.ip + row] = v;
+          if (kHalf) atomicMax(a.bmax + slot, __float_as_uint(fabsf(v)));
+        }
       }
-      const float* parts = park(acc);
-      // warp `part` finishes accumulator `part` of every lane
+      all_consumers_sync(a, gave_up);
+
+      // ---- second product: tiles of 16 rows of one expert
+      unit = -1;
+      for (int task = first1; task < end1; task++) {
+        const int u = task / tiles1, tile = task - u * tiles1, r0 = tile * 16;
+        const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(a.unit, L.first[e + 1] - n0);
+        if (u != unit) {
+          stage_b(a, L, n0, n, op, back);
+          unit = u;
+        }
+        float acc[NT][4] = {};
+        multiply<1>(a, acc, e, min(r0 + g, a.h - 1), min(r0 + g + 8, a.h - 1), n, op, ring, full, empty, stage, phase, gave_up);
+        const float* parts = park(acc);
+        // a warp finishes accumulator `turn` of every lane
+        const int turn = (warp + kConsumers - (task & 3) * 4) % kConsumers;
+        if (turn >= 4) continue;
 #pragma unroll
-      for (int j = 0; j < NT; j++) {
-        const int col = j * 8 + (lane & 3) * 2 + (part & 1), row = r0 + (lane >> 2) + (part & 2) * 4;
-        float s = 0.f;
+        for (int j = 0; j < NT; j++) {
+          const int col = j * 8 + (lane & 3) * 2 + (turn & 1), row = r0 + (lane >> 2) + (turn & 2) * 4;
+          if (col >= n || row >= a.h) continue;
+          float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kTeam; w++) s += parts[((w * NT + j) * 32 + lane) * 4 + part];
-        if (col < n && row < a.h) a.o[(int64_t)L.slots[n0 + col] * a.h + row] = s;
-      }
-      if (NT == 1) {
-        // the warp that finishes a row tile's last part (of kTeam a unit) sums the tokens' experts there
-        __threadfence();
-        __syncwarp();
-        unsigned before = 0;
-        if (lane == 0) before = atomicAdd(a.done + tile, 1u);
-        before = __shfl_sync(~0u, before, 0);
-        if (before == (unsigned)(kTeam * L.units - 1)) {
-          __threadfence();
-          for (int c = lane; c < a.tokens * 16; c += 32) combine(a, c >> 4, r0 + (c & 15));
+          for (int w = 0; w < kConsumers; w++) s += parts[((w * NT + j) * 32 + lane) * 4 + turn];
+          const int slot = L.slots[n0 + col];
+          a.o[(int64_t)slot * a.h + row] = kHalf ? s * back[col] : s;
         }
       }
     }
-    if (NT > 1) {
-      grid.sync();
-      const int64_t all = (int64_t)a.tokens * a.h;
-      for (int64_t c = blockIdx.x * (int64_t)kThreads + threadIdx.x; c < all; c += (int64_t)gridDim.x * kThreads) {
-        const int t = (int)(c / a.h);
-        combine(a, t, (int)(c - (int64_t)t * a.h));
+    // ---- the tokens' sums over their experts, in the order of choice
+    // (A counter a tile, whose last part sums it, saves this barrier; its
+    // fence in every tile cost four times as much.)
+    grid.sync();
+    const int64_t all = (int64_t)a.tokens * a.h;
+    for (int64_t c = blockIdx.x * (int64_t)kThreads + threadIdx.x; c < all; c += (int64_t)gridDim.x * kThreads) {
+      const int t = (int)(c / a.h), row = (int)(c - (int64_t)t * a.h);
+      float s = 0.f;
+#pragma unroll 8
+      for (int r = 0; r < a.top; r++) s += __ldcg(a.e.weights + t * a.top + r) * __ldcg(a.o + ((int64_t)t * a.top + r) * a.h + row);
+      ((X*)a.e.y)[(int64_t)t * a.e.ldy + row] = from_f32<X>(s);
+    }
+  }
+
+  __device__ static __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
+
+  // A barrier of the multiplying warps of all CTAs (the grid is resident as a
+  // whole).  The copying warps stay out of it: they may be waiting for room in
+  // the ring, which only the second product makes.
+  __device__ static __forceinline__ void all_consumers_sync(const LayerArgs& a, volatile int* gave_up) {
+    consumers_sync();
+    if (threadIdx.x == 0) {
+      __threadfence();
+      atomicAdd(a.arrived, 1u);
+      const long long t0 = clock64();
+      unsigned n;
+      do {
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(n) : "l"(a.arrived) : "memory");
+        if (clock64() - t0 > kWaitLimit) {
+          *gave_up = 1;
+          atomicExch_system(a.flag, 1);
+          break;
+        }
+      } while (n < gridDim.x);
+      __threadfence();
+    }
+    consumers_sync();
+  }
+
+  // Fill the ring with the tiles' rows.  PRODUCT 0: outputs 8 tile + r, their
+  // gate rows of w_in in stage rows 0 - 7, their up rows in 8 - 15; 1: rows
+  // 16 tile + r of w_out.  Rows past the end are others or zeros (not used).
+  template <int PRODUCT>
+  __device__ static __forceinline__ void copy_tiles(const LayerArgs& a, const CUtensorMap* map, const Lists& L, int first, int end, int tiles,
+                                                    unsigned char* ring, uint32_t full, uint32_t empty, int& stage,
+                                                    uint32_t& phase, volatile int* gave_up) {
+    const int lane = threadIdx.x & 31, copier = (threadIdx.x >> 5) - kConsumers;
+    const int k = PRODUCT == 0 ? a.h : a.i;
+    const int64_t rows = PRODUCT == 0 ? 2 * (int64_t)a.i : a.h;
+    const W* w = (const W*)(PRODUCT == 0 ? a.e.w_in : a.e.w_out);
+    auto row_of = [&](int tile, int r) {
+      return PRODUCT == 0 ? min(tile * 8 + (r & 7), a.i - 1) + (r >= 8 ? a.i : 0) : min(tile * 16 + r, a.h - 1);
+    };
+    for (int task = first; task < end; task++) {
+      const int u = task / tiles, tile = task - u * tiles;
+      const int64_t expert = L.unit_expert[u];
+      for (int k0 = 0; k0 < k; k0 += kRowK) {
+        mbar_wait(empty + 8 * stage, phase ^ 1, gave_up, a.flag);
+        __syncwarp();
+        unsigned char* dst = ring + stage * kStageBytes;
+        if constexpr (COPY == kTensor) {
+          if (lane == 0) {
+            const int bar = full + 8 * stage, piece = k0 * (int)sizeof(W) / 128;
+            mbar_expect_tx(bar, 16 * kRowBytes);  // whole boxes: what is outside the tensor comes as zeros
+            tensor_copy(smem_u32(dst), map, bar, (int)(expert * rows) + (PRODUCT == 0 ? tile * 8 : tile * 16), piece);
+            tensor_copy(smem_u32(dst) + 8 * kRowBytes, map, bar, (int)(expert * rows) + (PRODUCT == 0 ? a.i + tile * 8 : tile * 16 + 8), piece);
+          }
+          __syncwarp();
+        } else if constexpr (COPY == kBulk) {
+          const int bytes = min(kRowBytes, (k - k0) * (int)sizeof(W));
+          if (lane == 0) mbar_expect_tx(full + 8 * stage, 16 * bytes);
+          __syncwarp();
+          if (lane < 16) bulk_copy(smem_u32(dst + lane * kRowPitch), w + (expert * rows + row_of(tile, lane)) * k + k0, bytes, full + 8 * stage);
+        } else {
+          const int m = min(kRowK, k - k0);
+          for (int r = copier; r < 16; r += kWarps - kConsumers) {
+            const W* src = w + (expert * rows + row_of(tile, r)) * k + k0;
+            for (int c = lane * 16 / (int)sizeof(W); c < m; c += 512 / (int)sizeof(W))
+              *reinterpret_cast<uint4*>(dst + r * kRowPitch + c * sizeof(W)) = row16<W, false>(src, c, m, true);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(full + 8 * stage);
+        }
+        if (++stage == a.stages) stage = 0, phase ^= 1;
       }
     }
   }
 
-  // A token's sum over its experts, in the order of choice.
-  __device__ static __forceinline__ void combine(const LayerArgs& a, int t, int row) {
-    if (row >= a.h) return;
-    float s = 0.f;
-#pragma unroll 4
-    for (int r = 0; r < a.top; r++) s += __ldcg(a.e.weights + t * a.top + r) * __ldcg(a.o + ((int64_t)t * a.top + r) * a.h + row);
-    ((M*)a.e.y)[(int64_t)t * a.e.ldy + row] = from_f32<M>(s);
+  // The unit's tokens of x as rows of `op`, zeros up to a multiple of 128.  8-bit
+  // weights are exact in float16 (one instruction for two), so x goes there too.
+  __device__ static __forceinline__ void stage_x(const LayerArgs& a, const Lists& L, int n0, int n, unsigned char* op, float* back) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    consumers_sync();
+    if (kScaled && threadIdx.x < n) back[threadIdx.x] = power(a.xmax + L.slots[n0 + threadIdx.x] / a.top, 1);
+    const int padded = (a.h + 127) / 128 * 128;
+    for (int c = warp * 32 + lane; c < n * (padded / 8); c += kConsumers * 32) {
+      const int t = c / (padded / 8), k = (c - t * (padded / 8)) * 8;
+      const int token = L.slots[n0 + t] / a.top;
+      uint4 v = row16<X, VEC>((const X*)a.e.x + (int64_t)token * a.e.ldx, k, a.h, true);
+      if (kScaled) {
+        const float f = power(a.xmax + token, -1);
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const float2 x = unpack2<X>(w[j]);
+          w[j] = pack2<M>(x.x * f, x.y * f);
+        }
+      }
+      *reinterpret_cast<uint4*>(op + t * a.xpitch + k * 2) = v;
+    }
+    consumers_sync();
+  }
+  // The unit's rows of b as high parts, then low parts.
+  __device__ static __forceinline__ void stage_b(const LayerArgs& a, const Lists& L, int n0, int n, unsigned char* op, float* back) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    consumers_sync();
+    if (kHalf && threadIdx.x < n) back[threadIdx.x] = power(a.bmax + L.slots[n0 + threadIdx.x], 1);
+    const int padded = (a.i + 127) / 128 * 128;
+    for (int c = warp * 32 + lane; c < n * (padded / 4); c += kConsumers * 32) {
+      const int t = c / (padded / 4), k = (c - t * (padded / 4)) * 4;
+      const int slot = L.slots[n0 + t];
+      const float scale = kHalf ? power(a.bmax + slot, -1) : 1.f;
+      float4 f = make_float4(0, 0, 0, 0);
+      if (k < a.i) f = __ldcg(reinterpret_cast<const float4*>(a.b + (int64_t)slot * a.ip + k));
+      float v[4] = {f.x, f.y, f.z, f.w};
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = k + j < a.i ? v[j] * scale : 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        hi[j] = pack2<M>(v[2 * j], v[2 * j + 1]);
+        const float2 h = unpack2<M>(hi[j]);
+        // (an infinite high part stands alone: no inf - inf)
+        lo[j] = pack2<M>(isinf(h.x) ? 0.f : v[2 * j] - h.x, isinf(h.y) ? 0.f : v[2 * j + 1] - h.y);
+      }
+      *reinterpret_cast<uint2*>(op + t * a.bpitch + k * 2) = make_uint2(hi[0], hi[1]);
+      *reinterpret_cast<uint2*>(op + (a.unit + t) * a.bpitch + k * 2) = make_uint2(lo[0], lo[1]);
+    }
+    consumers_sync();
+  }
+
+  // This warp's part of one tile: its steps of every stage of the tile.
+  template <int PRODUCT>
+  __device__ static __forceinline__ void multiply(const LayerArgs& a, float (*acc)[4], int expert, int row_a, int row_b, int n,
+                                                  const unsigned char* op, const unsigned char* ring, uint32_t full,
+                                                  uint32_t empty, int& stage, uint32_t& phase, volatile int* gave_up) {
+    constexpr int kParts = PRODUCT == 0 ? 1 : 2;  // b comes in two parts
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, q = lane & 3;
+    const int k = PRODUCT == 0 ? a.h : a.i;
+    const int pitch = PRODUCT == 0 ? a.xpitch : a.bpitch;
+    const float *sa = nullptr, *sb = nullptr;
+    if (kScaled) {
+      const int64_t kb = (k + 127) / 128, rb = ((PRODUCT == 0 ? 2 * a.i : a.h) + 127) / 128;
+      const float* s = (PRODUCT == 0 ? a.e.in_scales : a.e.out_scales) + expert * rb * kb;
+      sa = s + (row_a >> 7) * kb, sb = s + (row_b >> 7) * kb;
+    }
+    // the lane's row of the weights' 8 x 16 byte pieces: rows 0 - 7, 8 - 15, the same of the next 16 bytes
+    const uint32_t wrow = smem_u32(ring) + (COPY == kTensor ? (lane >> 3 & 1) * 8 * kRowBytes + (lane & 7) * 128
+                                                            : (lane & 15) * kRowPitch + (lane >> 4) * 16);
+    auto piece = [&](int byte) {  // of the stage's row, a multiple of 32
+      return COPY == kTensor ? (byte >> 7) * 1024 + ((((byte >> 4 & 7) + (lane >> 4)) ^ (lane & 7)) << 4) : byte;
+    };
+    // 16-bit weights: the lane's token and piece of k of the tokens' four 8 x 16 byte pieces
+    const uint32_t ops = smem_u32(op);
+    float odd[NT][4] = {};  // every second MMA's sums: a chain of dependent ones is half as long
+    for (int k0 = 0; k0 < k; k0 += kRowK) {
+      // bytes of a row in this stage, whole 16-byte pieces (zeros past the row's end)
+      const int bytes = min(kRowBytes, ((k - k0) * (int)sizeof(W) + 15) / 16 * 16);
+      float fa = 0.f, fb = 0.f;  // a warp has one block of 128 of a stage
+      static_assert(!kScaled || kRowBytes / kStepBytes == kConsumers, "");
+      if (kScaled && warp * 128 < bytes) fa = __ldg(sa + k0 / 128 + warp), fb = __ldg(sb + k0 / 128 + warp);
+      mbar_wait(full + 8 * stage, phase, gave_up, a.flag);
+      __syncwarp();
+      const uint32_t at = wrow + stage * kStageBytes;
+#pragma unroll 2
+      for (int st = 0; st < kRowBytes / kStepBytes / kConsumers; st++) {
+        const int byte = (st * kConsumers + warp) * kStepBytes;  // of the stage's row
+        if (byte >= bytes) break;
+        const int kk = k0 + byte / (int)sizeof(W);
+        if constexpr (!kScaled) {
+          uint32_t w[8];
+          ldmatrix4(at + piece(byte), w);
+          if (byte + 16 >= bytes) w[2] = w[3] = 0;
+          if (byte + 32 < bytes) ldmatrix4(at + piece(byte + 32), w + 4);
+          else w[4] = w[5] = w[6] = w[7] = 0;
+          if (byte + 48 >= bytes) w[6] = w[7] = 0;
+#pragma unroll
+          for (int j = 0; j < NT; j++) {
+            if (j * 8 >= n) break;
+#pragma unroll
+            for (int p = 0; p < kParts; p++) {
+              uint32_t b[4];
+              ldmatrix4(ops + (min(j * 8 + (lane & 7), n - 1) + p * a.unit) * pitch + kk * 2 + (lane >> 3) * 16, b);
+              mma<M>(acc[j], w[0], w[1], w[2], w[3], b[0], b[1]);
+              mma<M>(odd[j], w[4], w[5], w[6], w[7], b[2], b[3]);
+            }
+          }
+        } else {
+          float sum[NT][2][4] = {};
+          uint32_t w[4][4];  // 32 bytes of k each: two pieces of 16
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            if (byte + c * 32 < bytes) ldmatrix4(at + piece(byte + c * 32), w[c]);
+            else w[c][0] = w[c][1] = w[c][2] = w[c][3] = 0;
+            if (byte + c * 32 + 16 >= bytes) w[c][2] = w[c][3] = 0;
+          }
+#pragma unroll
+          for (int c = 0; c < 4; c++) {
+            uint32_t m[8];  // lane q has k 4 q .. 4 q + 3 of a piece: its MMA takes them as 2 q, 2 q + 1 and + 8
+#pragma unroll
+            for (int r = 0; r < 4; r++) m[2 * r] = widen(w[c][r] & 0xffff), m[2 * r + 1] = widen(w[c][r] >> 16);
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+              if (j * 8 >= n) break;
+#pragma unroll
+              for (int p = 0; p < kParts; p++) {
+                const unsigned char* b = op + (min(j * 8 + g, n - 1) + p * a.unit) * pitch + (kk + c * 32) * 2 + q * 8;
+                const uint2 b0 = *reinterpret_cast<const uint2*>(b), b1 = *reinterpret_cast<const uint2*>(b + 32);
+                mma<M>(sum[j][0], m[0], m[2], m[1], m[3], b0.x, b0.y);
+                mma<M>(sum[j][1], m[4], m[6], m[5], m[7], b1.x, b1.y);
+              }
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < NT; j++) {
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[j][c] = fmaf(sum[j][0][c] + sum[j][1][c], c < 2 ? fa : fb, acc[j][c]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + 8 * stage);
+      if (++stage == a.stages) stage = 0, phase ^= 1;
+    }
+    if (!kScaled)
+#pragma unroll
+      for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int c = 0; c < 4; c++) acc[j][c] += odd[j][c];
   }
 };
 
-template <typename W, typename M, bool VEC, int NT>
-__global__ void __launch_bounds__(kThreads, 1) layer_kernel(const LayerArgs a) {
+template <typename W, typename X, typename M, int COPY, int NT>
+__global__ void __launch_bounds__(warps_of(COPY) * 32, 1)
+    layer_kernel(const __grid_constant__ LayerArgs a, const __grid_constant__ Maps maps) {
   __shared__ Lists lists;
   __shared__ int scratch[kMaxExperts];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages];
+  __shared__ int gave_up;
   extern __shared__ __align__(16) unsigned char dyn[];
-  Layer<W, M, VEC, NT>::run(a, lists, scratch, dyn);
+  Layer<W, X, M, COPY, NT>::run(a, maps.m, lists, scratch, bars, &gave_up, dyn);
 }
 
-template <typename W, typename M, bool VEC, int NT>
-void launch(LayerArgs& a, cudaStream_t s) {
-  auto kern = layer_kernel<W, M, VEC, NT>;
-  constexpr size_t smem = Layer<W, M, VEC, NT>::kSmem;
+constexpr int red_bytes(int nt) { return 2 * kConsumers * nt * 128 * 4; }
+// Shared memory for the tokens of a unit and the ring.
+int room(int nt) { return (int)ctx().smem_optin - (int)sizeof(Lists) - kMaxExperts * 4 - 2048 - red_bytes(nt); }
+
+// Rows of `bytes` as [piece of 128 bytes][row][byte].
+CUtensorMap weight_map(const void* w, int64_t rows, int64_t bytes) {
+  const cuuint64_t dims[3] = {128, (cuuint64_t)rows, (cuuint64_t)(bytes / 128)}, strides[2] = {(cuuint64_t)bytes, 128};
+  const cuuint32_t box[3] = {128, 8, kRowBytes / 128};
+  return byte_map(w, 3, dims, strides, box);
+}
+
+template <typename W, typename X, typename M, int COPY, int NT>
+void launch(LayerArgs& a, int64_t row, cudaStream_t s) {
+  auto kern = layer_kernel<W, X, M, COPY, NT>;
+  // as many tokens as fit beside three stages (at least one, beside two), and stages for the rest
+  const int space = room(NT);
+  if (row > space - 2 * kStageBytes) throw Error(ErrKind::InvalidArgument, "h or i is too large for a token's row to fit shared memory");
+  a.unit = (int)std::max<int64_t>(1, std::min<int64_t>({NT * 8, a.tokens, (space - 3 * kStageBytes) / row}));
+  a.op_bytes = (int)(a.unit * row);
+  a.stages = std::min(kMaxStages, (space - a.op_bytes) / kStageBytes);
+  const size_t smem = (size_t)a.op_bytes + red_bytes(NT) + 1024 + (size_t)a.stages * kStageBytes;
   ensure_dynamic_smem((const void*)kern, smem);
-  void* args[] = {&a};
-  NDT_CUDA(cudaLaunchCooperativeKernel((const void*)kern, dim3((unsigned)ctx().sm_count), dim3(kThreads), args, smem, s));
+  Maps maps{};
+  if (COPY == kTensor) {
+    maps.m[0] = weight_map(a.e.w_in, 2 * a.e.experts * a.e.i, a.e.h * sizeof(W));
+    maps.m[1] = weight_map(a.e.w_out, a.e.experts * a.e.h, a.e.i * sizeof(W));
+  }
+  void* args[] = {&a, &maps};
+  NDT_CUDA(cudaLaunchCooperativeKernel((const void*)kern, dim3((unsigned)ctx().sm_count), dim3(warps_of(COPY) * 32), args, smem, s));
   count_launch();
 }
 
@@ -644,7 +817,7 @@ void expert_layer(const ExpertArgs& e, cudaStream_t s) {
   const int64_t ip = (e.i + 7) / 8 * 8;
   const int64_t xs = msize(e.xt), ws_ = msize(e.wt);
   // b first: its rows are read in 16-byte vectors
-  Workspace ws((size_t)4 * (most * (e.top * (ip + e.h + 1) + e.experts) + (e.h + 15) / 16), s);
+  Workspace ws((size_t)4 * (most * (e.top * (ip + e.h + 1) + e.experts) + most + 1), s);
   for (int64_t t0 = 0; t0 < e.tokens; t0 += step) {
     LayerArgs a{};
     a.e = e;
@@ -653,27 +826,42 @@ void expert_layer(const ExpertArgs& e, cudaStream_t s) {
     a.e.x = (const char*)e.x + t0 * e.ldx * xs;
     a.e.y = (char*)e.y + t0 * e.ldy * xs;
     a.e.ids = e.ids + t0 * e.top, a.e.weights = e.weights + t0 * e.top;
-    a.b = ws.p;
-    a.o = (float*)ws.p + most * e.top * ip;
+    a.b = (float*)ws.p;
+    a.o = a.b + most * e.top * ip;
     a.logits = a.o + most * e.top * e.h;
     a.bmax = (unsigned*)(a.logits + most * e.experts);
-    a.done = a.bmax + most * e.top;
+    a.xmax = a.bmax + most * e.top;
+    a.arrived = a.xmax + most;
+    a.flag = wait_flag_device();
     const bool vec = e.h * ws_ % 16 == 0 && e.i * ws_ % 16 == 0 && e.h % 8 == 0 && e.ldx % 8 == 0 &&
                      (((uintptr_t)a.e.x | (uintptr_t)e.router | (uintptr_t)e.w_in | (uintptr_t)e.w_out) % 16) == 0;
-    auto go = [&](auto w, auto x) {
+    const bool pieces = vec && e.h * ws_ % 128 == 0 && e.i * ws_ % 128 == 0 && 2 * e.experts * std::max(e.h, e.i) <= INT32_MAX;
+    // tokens' rows start on different banks
+    const int pad = e.wt == MType::E4M3 ? 32 : 16;
+    a.xpitch = (a.h + 127) / 128 * 256 + pad, a.bpitch = (a.i + 127) / 128 * 256 + pad;
+    const int64_t row = std::max((int64_t)a.xpitch, 2 * (int64_t)a.bpitch);
+    // An expert's second unit of tokens reads its weights again (from L2): more
+    // columns where an expert gets more than 6 tokens on average and 16 fit.
+    const bool many = a.tokens * e.top > 6 * e.experts && a.tokens > 8 && 16 * row <= room(2) - 3 * kStageBytes;
+    auto go = [&](auto w, auto x, auto m) {
       using W = decltype(w);
-      using M = decltype(x);
-      if (a.tokens <= 8)
-        vec ? launch<W, M, true, 1>(a, s) : launch<W, M, false, 1>(a, s);
+      using X = decltype(x);
+      using M = decltype(m);
+      if (!vec)
+        many ? launch<W, X, M, kPlain, 2>(a, row, s) : launch<W, X, M, kPlain, 1>(a, row, s);
+      else if (!pieces)
+        many ? launch<W, X, M, kBulk, 2>(a, row, s) : launch<W, X, M, kBulk, 1>(a, row, s);
       else
-        vec ? launch<W, M, true, 4>(a, s) : launch<W, M, false, 4>(a, s);
+        many ? launch<W, X, M, kTensor, 2>(a, row, s) : launch<W, X, M, kTensor, 1>(a, row, s);
     };
+    const __nv_bfloat16 bf{};
+    const __half hf{};
     if (e.wt == MType::E4M3)
-      e.xt == MType::BF16 ? go(__nv_fp8_e4m3{}, __nv_bfloat16{}) : go(__nv_fp8_e4m3{}, __half{});
+      e.xt == MType::BF16 ? go(__nv_fp8_e4m3{}, bf, hf) : go(__nv_fp8_e4m3{}, hf, hf);
     else if (e.xt == MType::BF16)
-      go(__nv_bfloat16{}, __nv_bfloat16{});
+      go(bf, bf, bf);
     else
-      go(__half{}, __half{});
+      go(hf, hf, hf);
   }
 }
 

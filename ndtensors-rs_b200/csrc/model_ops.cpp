@@ -7,7 +7,7 @@
 #include <string>
 
 #include "../../include/ndtensors_capi.h"
-#include "model_ops.h"
+#include "mbarrier.h"
 
 namespace ndt {
 
@@ -31,6 +31,27 @@ bool wait_flag_raised() {
   if (!g_flag || !*(volatile int*)g_flag) return false;
   *(volatile int*)g_flag = 0;
   return true;
+}
+
+
+CUtensorMap byte_map(const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+  using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    NDT_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r));
+    if (!p || r != cudaDriverEntryPointSuccess) throw Error(ErrKind::Cuda, "cuTensorMapEncodeTiled is not in this driver");
+    return (Encode)p;
+  }();
+  CUtensorMap m;
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = encode(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, one,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw Error(ErrKind::Cuda, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return m;
 }
 
 }  // namespace ndt

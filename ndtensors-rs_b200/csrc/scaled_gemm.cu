@@ -23,11 +23,9 @@
 //
 // sa * sb is formed in 32 bits: it stays finite while the product of two
 // blocks' largest values is below 2^127.
-#include <cuda.h>
-
 #include <algorithm>
 
-#include "model_ops.h"
+#include "mbarrier.h"
 
 namespace ndt {
 namespace {
@@ -37,7 +35,6 @@ constexpr int kThreads = 384;
 constexpr int kEpiWarp0 = 4;  // the epilogue is two whole warpgroups (setmaxnreg)
 constexpr int kEpiWarps = 8;
 constexpr int kSlots = 8;    // scale ring
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 struct GemmArgs {
   const float* sa;
@@ -57,16 +54,6 @@ struct GemmArgs {
 };
 
 // ------------------------------------------------------------- PTX pieces
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 // In another CTA of the cluster.  (What it reports, that TMEM has been read, is
 // ordered by the tcgen05 fences; a release at cluster scope would add a memory
 // barrier to every k block.)
@@ -78,44 +65,6 @@ __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok;
-}
-__device__ __forceinline__ uint64_t now_ns() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-// A wait that ends: after two seconds, or once another wait of this CTA has
-// given up, it raises the flags and returns false.
-__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
-  const uint64_t t0 = now_ns();
-  while (true) {
-    for (int i = 0; i < 32; i++)
-      if (mbar_try(bar, parity)) return true;
-    if (*gave_up) return false;
-    if (now_ns() - t0 > kWaitLimitNs) {
-      *gave_up = 1;
-      atomicExch_system(flag, 1);
-      return false;
-    }
-  }
-}
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
-  if (mbar_try(bar, parity)) return true;
-  return mbar_wait_slow(bar, parity, gave_up, flag);
-}
-// For a whole warp: all lanes go on, or none.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
-  return __all_sync(~0u, mbar_wait(bar, parity, gave_up, flag));
-}
-
 template <int CTAS>
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
   if constexpr (CTAS == 1)
@@ -555,31 +504,11 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
 }
 
 // ------------------------------------------------------------------- host
-using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult r;
-    NDT_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &r));
-    if (!p || r != cudaDriverEntryPointSuccess) throw Error(ErrKind::Cuda, "cuTensorMapEncodeTiled is not in this driver");
-    return (EncodeFn)p;
-  }();
-  return fn;
-}
 // Boxes of box_rows x 128 bytes; bytes outside the matrix read as zeros (0.0 in both 8-bit types).
 CUtensorMap operand_map(const ScaledOperand& o, int64_t k, int box_rows) {
-  CUtensorMap m;
-  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)o.rows};
-  const cuuint64_t strides[1] = {(cuuint64_t)o.ld};
+  const cuuint64_t dims[2] = {(cuuint64_t)k, (cuuint64_t)o.rows}, strides[1] = {(cuuint64_t)o.ld};
   const cuuint32_t box[2] = {kBK, (cuuint32_t)box_rows};
-  const cuuint32_t one[2] = {1, 1};
-  const CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(o.p), dims, strides, box, one,
-                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) throw Error(ErrKind::Cuda, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
-  return m;
+  return byte_map(o.p, 2, dims, strides, box);
 }
 
 template <int CTAS, int BN, bool BROW>
