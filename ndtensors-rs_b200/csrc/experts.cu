@@ -17,13 +17,16 @@
 // gate rows and the 8 up rows of the same outputs, so silu(gate) * up needs no
 // exchange.
 //
-// The weights stream through a ring of stages in shared memory, 16 rows x 2 KB
-// each; 16 warps split a stage's k and add their parts through shared memory
-// at a tile's end.  The ring runs across tiles, and from the first product
-// into the second before the grid barrier between them.  One warp fills it.
-// Rows that are multiples of 128 bytes come as two tensor copies a stage (8
-// rows x 16 pieces of 128 bytes, swizzled so that ldmatrix meets no bank
-// conflict); others of whole 16-byte vectors as 16 bulk copies of 2 KB, rows
+// The weights stream through a ring of stages in shared memory, 16 rows x 1 or
+// 2 KB each.  Four teams of 4 warps take the tiles in turn; a team splits a
+// stage's k and adds its parts through shared memory at a tile's end, while the
+// others multiply (one team of 16 lost a quarter of its time there).  The
+// ring runs across tiles, and from the first product into the second before
+// the grid barrier between them.  One warp fills it.  Rows that are multiples
+// of 128 bytes come as two tensor copies a stage (8 rows x 8 pieces of 128
+// bytes, swizzled so that ldmatrix meets no bank conflict; 90 KB in flight on
+// each SM are needed for HBM's rate, so stages are small); others of whole
+// 16-byte vectors as 16 bulk copies of 2 KB, rows
 // 2064 bytes apart, which the copy engine takes at 70 - 85 ns each, below the
 // rate of HBM; the rest by plain loads of four warps.  Lanes that copied their
 // own fragments (cp.async) spent 110 instructions on each KB: 3.2 TB/s.
@@ -47,16 +50,15 @@ namespace cg = cooperative_groups;
 constexpr int kConsumers = 16;       // warps that multiply
 constexpr int kMaxWarps = kConsumers + 4;
 enum Copy { kPlain, kBulk, kTensor };  // how rows come: by element, in 16-byte vectors, in 128-byte pieces
+__host__ __device__ constexpr int most_bytes(int copy) { return copy == kTensor ? 1024 : 2048; }  // of a row in one stage
+__host__ __device__ constexpr int stage_bytes(int copy) { return copy == kTensor ? 16 * 1024 : 16 * (2048 + 16); }
 __host__ __device__ constexpr int warps_of(int copy) { return kConsumers + (copy == kPlain ? 4 : 1); }
 constexpr int kMaxSlots = 2048;      // (token, chosen expert) pairs of one launch
 constexpr int kMaxTokens = 256;
 constexpr int kMaxExperts = 1024;
 constexpr int kGroup = 8;            // tokens of one router product
-constexpr int kRowBytes = 2048;      // of a row in one stage
-constexpr int kRowPitch = kRowBytes + 16;
-constexpr int kStageBytes = 33 * 1024;  // 16 rows of either pitch, a multiple of the swizzle's 1024
-static_assert(16 * kRowPitch <= kStageBytes, "");
-constexpr int kMaxStages = 6;
+constexpr int kTeam = 4;             // multiplying warps that take a tile together
+constexpr int kMaxStages = 12;
 
 struct LayerArgs {
   ExpertArgs e;
@@ -64,8 +66,10 @@ struct LayerArgs {
   int ip;           // i rounded up to 8: the pitch of b's rows
   int unit;         // tokens of an expert that a CTA takes at a time
   int stages;
+  int row_bytes[2];    // of a row in one stage of each product: even parts of the row
   int xpitch, bpitch;  // bytes of a token's row of x / of b's parts in shared memory
-  int op_bytes;     // shared memory for either
+  int op_bytes;     // shared memory for either, and for an expert's scales behind it
+  int scale_at;     // where those start; -1: they stay in global memory
   float* logits;    // [tokens, experts]
   float* b;         // [slots, ip]
   float* o;         // [slots, h]
@@ -134,7 +138,7 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, int byt
                "r"(bar)
                : "memory");
 }
-// 8 rows x 16 pieces of 128 bytes, piece by piece, 128-byte swizzle.
+// 8 rows of a box of pieces of 128 bytes, piece by piece, 128-byte swizzle.
 __device__ __forceinline__ void tensor_copy(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int piece) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
@@ -384,10 +388,11 @@ struct Layer {
   static constexpr int kWarps = warps_of(COPY), kThreads = kWarps * 32;
   static constexpr bool kScaled = sizeof(W) == 1;
   static constexpr bool kHalf = std::is_same_v<M, __half>;
-  static constexpr int kRowK = kRowBytes / (int)sizeof(W);    // k of a stage
+  static constexpr int kStageBytes = stage_bytes(COPY);
+  static constexpr int kRowPitch = most_bytes(COPY) + 16;     // (not kTensor)
   static constexpr int kStepK = kScaled ? 128 : 32;           // k of a warp's step: one scale, or two MMAs
   static constexpr int kStepBytes = kStepK * (int)sizeof(W);
-  static constexpr int kRed = kConsumers * NT * 128;          // floats of a tile's parts
+  static constexpr int kRed = kTeam * NT * 128;               // floats of a tile's parts
 
   // What brings a row whose largest value is at `most` into float16's range,
   // 2^-x, or (sign 1) what takes it back.
@@ -402,8 +407,8 @@ struct Layer {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2;
     unsigned char* op = dyn;                                        // x, then b, of the unit's tokens
-    float* red = reinterpret_cast<float*>(dyn + a.op_bytes);        // two buffers of parts
-    unsigned char* ring = dyn + a.op_bytes + 2 * kRed * 4;
+    float* red = reinterpret_cast<float*>(dyn + a.op_bytes);        // two buffers of parts a team
+    unsigned char* ring = dyn + a.op_bytes + 2 * kConsumers / kTeam * kRed * 4;
     ring += (1024 - (smem_u32(ring) & 1023)) & 1023;
     const uint32_t full = smem_u32(bars), empty = full + 8 * kMaxStages;
     __shared__ float back[NT * 8];  // what takes a token's results back from float16's range
@@ -448,14 +453,26 @@ struct Layer {
         __syncwarp();
       }
     } else {
+      const int team = warp / kTeam, part = warp % kTeam;
       int stage = 0, parity = 0;
       uint32_t phase = 0;
+      // Over another team's stages.  Every team gives every stage back, so that
+      // none is ever a whole round of the ring from another and a barrier's
+      // parity stays unambiguous.
+      auto pass = [&](int k, int row_bytes) {
+        for (int b = 0; b < k * (int)sizeof(W); b += row_bytes) {
+          mbar_wait(full + 8 * stage, phase, gave_up, a.flag);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty + 8 * stage);
+          if (++stage == a.stages) stage = 0, phase ^= 1;
+        }
+      };
       auto park = [&](float (*acc)[4]) {  // this warp's part of the tile, for the warps that finish it
-        float* at = red + parity * kRed;
+        float* at = red + (team * 2 + parity) * kRed;
 #pragma unroll
         for (int j = 0; j < NT; j++)
-          *reinterpret_cast<float4*>(at + ((warp * NT + j) * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
-        consumers_sync();  // one a tile: two buffers alternate
+          *reinterpret_cast<float4*>(at + ((part * NT + j) * 32 + lane) * 4) = make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+        asm volatile("bar.sync %0, %1;" ::"r"(2 + team), "n"(kTeam * 32) : "memory");  // one a tile: two buffers alternate
         parity ^= 1;
         return (const float*)at;
       };
@@ -466,21 +483,25 @@ struct Layer {
         const int u = task / tiles0, i0 = (task - u * tiles0) * 8;
         const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(a.unit, L.first[e + 1] - n0);
         if (u != unit) {
-          if (unit < 0 || a.tokens > 1) stage_x(a, L, n0, n, op, back);
+          if (unit < 0 || a.tokens > 1 || kScaled) stage_x(a, L, e, n0, n, op, back);
           unit = u;
+        }
+        if ((task - first0) % (kConsumers / kTeam) != team) {
+          pass(a.h, a.row_bytes[0]);
+          continue;
         }
         float acc[NT][4] = {};
         const int row_a = min(i0 + g, a.i - 1);
         multiply<0>(a, acc, e, row_a, a.i + row_a, n, op, ring, full, empty, stage, phase, gave_up);
         const float* parts = park(acc);
         // accumulator (row g: gate; row g + 8: up; columns 2 q, 2 q + 1) of column tile j; which warps finish goes round
-        for (int o = ((warp + kConsumers - (task * 2 * NT) % kConsumers) % kConsumers) * 32 + lane; o < NT * 64; o += kConsumers * 32) {
+        for (int o = ((part + (task / kTeam & 1) * 2) % kTeam) * 32 + lane; o < NT * 64; o += kTeam * 32) {
           const int j = o >> 6, ln = o >> 1 & 31, half = o & 1;
           const int col = j * 8 + (ln & 3) * 2 + half, row = i0 + (ln >> 2);
           if (col >= n || row >= a.i) continue;
           float ga = 0.f, up = 0.f;
 #pragma unroll
-          for (int w = 0; w < kConsumers; w++) {
+          for (int w = 0; w < kTeam; w++) {
             const float* p = parts + ((w * NT + j) * 32 + ln) * 4 + half;
             ga += p[0], up += p[2];
           }
@@ -499,22 +520,25 @@ struct Layer {
         const int u = task / tiles1, tile = task - u * tiles1, r0 = tile * 16;
         const int e = L.unit_expert[u], n0 = L.unit_first[u], n = min(a.unit, L.first[e + 1] - n0);
         if (u != unit) {
-          stage_b(a, L, n0, n, op, back);
+          stage_b(a, L, e, n0, n, op, back);
           unit = u;
+        }
+        if ((task - first1) % (kConsumers / kTeam) != team) {
+          pass(a.i, a.row_bytes[1]);
+          continue;
         }
         float acc[NT][4] = {};
         multiply<1>(a, acc, e, min(r0 + g, a.h - 1), min(r0 + g + 8, a.h - 1), n, op, ring, full, empty, stage, phase, gave_up);
         const float* parts = park(acc);
-        // a warp finishes accumulator `turn` of every lane
-        const int turn = (warp + kConsumers - (task & 3) * 4) % kConsumers;
-        if (turn >= 4) continue;
+        // warp `part` finishes accumulator `part` of every lane
+        static_assert(kTeam == 4, "");
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-          const int col = j * 8 + (lane & 3) * 2 + (turn & 1), row = r0 + (lane >> 2) + (turn & 2) * 4;
+          const int col = j * 8 + (lane & 3) * 2 + (part & 1), row = r0 + (lane >> 2) + (part & 2) * 4;
           if (col >= n || row >= a.h) continue;
           float s = 0.f;
 #pragma unroll
-          for (int w = 0; w < kConsumers; w++) s += parts[((w * NT + j) * 32 + lane) * 4 + turn];
+          for (int w = 0; w < kTeam; w++) s += parts[((w * NT + j) * 32 + lane) * 4 + part];
           const int slot = L.slots[n0 + col];
           a.o[(int64_t)slot * a.h + row] = kHalf ? s * back[col] : s;
         }
@@ -524,13 +548,27 @@ struct Layer {
     // (A counter a tile, whose last part sums it, saves this barrier; its
     // fence in every tile cost four times as much.)
     grid.sync();
-    const int64_t all = (int64_t)a.tokens * a.h;
-    for (int64_t c = blockIdx.x * (int64_t)kThreads + threadIdx.x; c < all; c += (int64_t)gridDim.x * kThreads) {
-      const int t = (int)(c / a.h), row = (int)(c - (int64_t)t * a.h);
-      float s = 0.f;
-#pragma unroll 8
-      for (int r = 0; r < a.top; r++) s += __ldcg(a.e.weights + t * a.top + r) * __ldcg(a.o + ((int64_t)t * a.top + r) * a.h + row);
-      ((X*)a.e.y)[(int64_t)t * a.e.ldy + row] = from_f32<X>(s);
+    const bool four = a.h % 4 == 0 && a.e.ldy % 4 == 0 && (uintptr_t)a.e.y % (4 * sizeof(X)) == 0;
+    const int step = four ? 4 : 1, columns = a.h / step;
+    for (int c = blockIdx.x * kThreads + threadIdx.x; c < a.tokens * columns; c += gridDim.x * kThreads) {
+      const int t = c / columns, row = (c - t * columns) * step;
+      float s[4] = {};
+#pragma unroll 4
+      for (int r = 0; r < a.top; r++) {
+        const float w = __ldcg(a.e.weights + t * a.top + r);
+        const float* o = a.o + ((int64_t)t * a.top + r) * a.h + row;
+        if (four) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(o));
+          s[0] = fmaf(w, v.x, s[0]), s[1] = fmaf(w, v.y, s[1]), s[2] = fmaf(w, v.z, s[2]), s[3] = fmaf(w, v.w, s[3]);
+        } else {
+          s[0] = fmaf(w, __ldcg(o), s[0]);
+        }
+      }
+      X* y = (X*)a.e.y + (int64_t)t * a.e.ldy + row;
+      if (four)
+        *reinterpret_cast<uint2*>(y) = make_uint2(pack2<X>(s[0], s[1]), pack2<X>(s[2], s[3]));
+      else
+        *y = from_f32<X>(s[0]);
     }
   }
 
@@ -542,8 +580,8 @@ struct Layer {
   __device__ static __forceinline__ void all_consumers_sync(const LayerArgs& a, volatile int* gave_up) {
     consumers_sync();
     if (threadIdx.x == 0) {
-      __threadfence();
-      atomicAdd(a.arrived, 1u);
+      // (release and acquire at the GPU's scope: the CTA's barriers carry the other warps' writes)
+      asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(a.arrived) : "memory");
       const long long t0 = clock64();
       unsigned n;
       do {
@@ -554,7 +592,6 @@ struct Layer {
           break;
         }
       } while (n < gridDim.x);
-      __threadfence();
     }
     consumers_sync();
   }
@@ -576,25 +613,26 @@ struct Layer {
     for (int task = first; task < end; task++) {
       const int u = task / tiles, tile = task - u * tiles;
       const int64_t expert = L.unit_expert[u];
-      for (int k0 = 0; k0 < k; k0 += kRowK) {
+      const int row_bytes = a.row_bytes[PRODUCT], row_k = row_bytes / (int)sizeof(W);
+      for (int k0 = 0; k0 < k; k0 += row_k) {
         mbar_wait(empty + 8 * stage, phase ^ 1, gave_up, a.flag);
         __syncwarp();
         unsigned char* dst = ring + stage * kStageBytes;
         if constexpr (COPY == kTensor) {
           if (lane == 0) {
             const int bar = full + 8 * stage, piece = k0 * (int)sizeof(W) / 128;
-            mbar_expect_tx(bar, 16 * kRowBytes);  // whole boxes: what is outside the tensor comes as zeros
+            mbar_expect_tx(bar, 16 * row_bytes);  // whole boxes: what is outside the tensor comes as zeros
             tensor_copy(smem_u32(dst), map, bar, (int)(expert * rows) + (PRODUCT == 0 ? tile * 8 : tile * 16), piece);
-            tensor_copy(smem_u32(dst) + 8 * kRowBytes, map, bar, (int)(expert * rows) + (PRODUCT == 0 ? a.i + tile * 8 : tile * 16 + 8), piece);
+            tensor_copy(smem_u32(dst) + 8 * 1024, map, bar, (int)(expert * rows) + (PRODUCT == 0 ? a.i + tile * 8 : tile * 16 + 8), piece);
           }
           __syncwarp();
         } else if constexpr (COPY == kBulk) {
-          const int bytes = min(kRowBytes, (k - k0) * (int)sizeof(W));
+          const int bytes = min(row_bytes, (k - k0) * (int)sizeof(W));
           if (lane == 0) mbar_expect_tx(full + 8 * stage, 16 * bytes);
           __syncwarp();
           if (lane < 16) bulk_copy(smem_u32(dst + lane * kRowPitch), w + (expert * rows + row_of(tile, lane)) * k + k0, bytes, full + 8 * stage);
         } else {
-          const int m = min(kRowK, k - k0);
+          const int m = min(row_k, k - k0);
           for (int r = copier; r < 16; r += kWarps - kConsumers) {
             const W* src = w + (expert * rows + row_of(tile, r)) * k + k0;
             for (int c = lane * 16 / (int)sizeof(W); c < m; c += 512 / (int)sizeof(W))
@@ -608,12 +646,23 @@ struct Layer {
     }
   }
 
+  // The scales of one expert's [rows, k] weights behind the tokens, where they
+  // fit: a tile's would wait for L2 in every stage.
+  __device__ static __forceinline__ void stage_scales(const LayerArgs& a, const float* scales, int expert, int rows, int k,
+                                                      unsigned char* op) {
+    if (!kScaled || a.scale_at < 0) return;
+    const int n = (rows + 127) / 128 * ((k + 127) / 128);
+    float* to = reinterpret_cast<float*>(op + a.scale_at);
+    for (int c = threadIdx.x; c < n; c += kConsumers * 32) to[c] = __ldg(scales + (int64_t)expert * n + c);
+  }
+
   // The unit's tokens of x as rows of `op`, zeros up to a multiple of 128.  8-bit
   // weights are exact in float16 (one instruction for two), so x goes there too.
-  __device__ static __forceinline__ void stage_x(const LayerArgs& a, const Lists& L, int n0, int n, unsigned char* op, float* back) {
+  __device__ static __forceinline__ void stage_x(const LayerArgs& a, const Lists& L, int expert, int n0, int n, unsigned char* op, float* back) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     consumers_sync();
     if (kScaled && threadIdx.x < n) back[threadIdx.x] = power(a.xmax + L.slots[n0 + threadIdx.x] / a.top, 1);
+    stage_scales(a, a.e.in_scales, expert, 2 * a.i, a.h, op);
     const int padded = (a.h + 127) / 128 * 128;
     for (int c = warp * 32 + lane; c < n * (padded / 8); c += kConsumers * 32) {
       const int t = c / (padded / 8), k = (c - t * (padded / 8)) * 8;
@@ -633,10 +682,11 @@ struct Layer {
     consumers_sync();
   }
   // The unit's rows of b as high parts, then low parts.
-  __device__ static __forceinline__ void stage_b(const LayerArgs& a, const Lists& L, int n0, int n, unsigned char* op, float* back) {
+  __device__ static __forceinline__ void stage_b(const LayerArgs& a, const Lists& L, int expert, int n0, int n, unsigned char* op, float* back) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     consumers_sync();
     if (kHalf && threadIdx.x < n) back[threadIdx.x] = power(a.bmax + L.slots[n0 + threadIdx.x], 1);
+    stage_scales(a, a.e.out_scales, expert, a.h, a.i, op);
     const int padded = (a.i + 127) / 128 * 128;
     for (int c = warp * 32 + lane; c < n * (padded / 4); c += kConsumers * 32) {
       const int t = c / (padded / 4), k = (c - t * (padded / 4)) * 4;
@@ -667,18 +717,19 @@ struct Layer {
                                                   const unsigned char* op, const unsigned char* ring, uint32_t full,
                                                   uint32_t empty, int& stage, uint32_t& phase, volatile int* gave_up) {
     constexpr int kParts = PRODUCT == 0 ? 1 : 2;  // b comes in two parts
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int part = (threadIdx.x >> 5) % kTeam, lane = threadIdx.x & 31;
     const int g = lane >> 2, q = lane & 3;
     const int k = PRODUCT == 0 ? a.h : a.i;
     const int pitch = PRODUCT == 0 ? a.xpitch : a.bpitch;
     const float *sa = nullptr, *sb = nullptr;
     if (kScaled) {
       const int64_t kb = (k + 127) / 128, rb = ((PRODUCT == 0 ? 2 * a.i : a.h) + 127) / 128;
-      const float* s = (PRODUCT == 0 ? a.e.in_scales : a.e.out_scales) + expert * rb * kb;
+      const float* s = a.scale_at < 0 ? (PRODUCT == 0 ? a.e.in_scales : a.e.out_scales) + expert * rb * kb
+                                      : reinterpret_cast<const float*>(op + a.scale_at);
       sa = s + (row_a >> 7) * kb, sb = s + (row_b >> 7) * kb;
     }
     // the lane's row of the weights' 8 x 16 byte pieces: rows 0 - 7, 8 - 15, the same of the next 16 bytes
-    const uint32_t wrow = smem_u32(ring) + (COPY == kTensor ? (lane >> 3 & 1) * 8 * kRowBytes + (lane & 7) * 128
+    const uint32_t wrow = smem_u32(ring) + (COPY == kTensor ? (lane >> 3 & 1) * 8 * 1024 + (lane & 7) * 128
                                                             : (lane & 15) * kRowPitch + (lane >> 4) * 16);
     auto piece = [&](int byte) {  // of the stage's row, a multiple of 32
       return COPY == kTensor ? (byte >> 7) * 1024 + ((((byte >> 4 & 7) + (lane >> 4)) ^ (lane & 7)) << 4) : byte;
@@ -686,19 +737,17 @@ struct Layer {
     // 16-bit weights: the lane's token and piece of k of the tokens' four 8 x 16 byte pieces
     const uint32_t ops = smem_u32(op);
     float odd[NT][4] = {};  // every second MMA's sums: a chain of dependent ones is half as long
-    for (int k0 = 0; k0 < k; k0 += kRowK) {
+    const int row_bytes = a.row_bytes[PRODUCT], row_k = row_bytes / (int)sizeof(W);
+    int turn = part;  // the team's warps take the tile's steps in turn: this stage's first of this warp
+    for (int k0 = 0; k0 < k; k0 += row_k) {
       // bytes of a row in this stage, whole 16-byte pieces (zeros past the row's end)
-      const int bytes = min(kRowBytes, ((k - k0) * (int)sizeof(W) + 15) / 16 * 16);
-      float fa = 0.f, fb = 0.f;  // a warp has one block of 128 of a stage
-      static_assert(!kScaled || kRowBytes / kStepBytes == kConsumers, "");
-      if (kScaled && warp * 128 < bytes) fa = __ldg(sa + k0 / 128 + warp), fb = __ldg(sb + k0 / 128 + warp);
+      const int bytes = min(row_bytes, ((k - k0) * (int)sizeof(W) + 15) / 16 * 16);
       mbar_wait(full + 8 * stage, phase, gave_up, a.flag);
       __syncwarp();
       const uint32_t at = wrow + stage * kStageBytes;
+      int byte = turn * kStepBytes;  // of the stage's row
 #pragma unroll 2
-      for (int st = 0; st < kRowBytes / kStepBytes / kConsumers; st++) {
-        const int byte = (st * kConsumers + warp) * kStepBytes;  // of the stage's row
-        if (byte >= bytes) break;
+      for (; byte < bytes; byte += kTeam * kStepBytes) {
         const int kk = k0 + byte / (int)sizeof(W);
         if constexpr (!kScaled) {
           uint32_t w[8];
@@ -719,6 +768,7 @@ struct Layer {
             }
           }
         } else {
+          const float fa = sa[kk >> 7], fb = sb[kk >> 7];
           float sum[NT][2][4] = {};
           uint32_t w[4][4];  // 32 bytes of k each: two pieces of 16
 #pragma unroll
@@ -751,6 +801,7 @@ struct Layer {
           }
         }
       }
+      turn = (byte - row_bytes) / kStepBytes;
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + 8 * stage);
       if (++stage == a.stages) stage = 0, phase ^= 1;
@@ -779,27 +830,37 @@ constexpr int red_bytes(int nt) { return 2 * kConsumers * nt * 128 * 4; }
 int room(int nt) { return (int)ctx().smem_optin - (int)sizeof(Lists) - kMaxExperts * 4 - 2048 - red_bytes(nt); }
 
 // Rows of `bytes` as [piece of 128 bytes][row][byte].
-CUtensorMap weight_map(const void* w, int64_t rows, int64_t bytes) {
+CUtensorMap weight_map(const void* w, int64_t rows, int64_t bytes, int stage_row) {
   const cuuint64_t dims[3] = {128, (cuuint64_t)rows, (cuuint64_t)(bytes / 128)}, strides[2] = {(cuuint64_t)bytes, 128};
-  const cuuint32_t box[3] = {128, 8, kRowBytes / 128};
+  const cuuint32_t box[3] = {128, 8, (cuuint32_t)stage_row / 128};
   return byte_map(w, 3, dims, strides, box);
 }
 
 template <typename W, typename X, typename M, int COPY, int NT>
 void launch(LayerArgs& a, int64_t row, cudaStream_t s) {
   auto kern = layer_kernel<W, X, M, COPY, NT>;
-  // as many tokens as fit beside three stages (at least one, beside two), and stages for the rest
-  const int space = room(NT);
-  if (row > space - 2 * kStageBytes) throw Error(ErrKind::InvalidArgument, "h or i is too large for a token's row to fit shared memory");
-  a.unit = (int)std::max<int64_t>(1, std::min<int64_t>({NT * 8, a.tokens, (space - 3 * kStageBytes) / row}));
+  // as many tokens as fit beside kKeep of stages (at least one, beside two stages), and stages for the rest
+  const int space = room(NT), kStageBytes = stage_bytes(COPY), kKeep = 100 * 1024;
+  if (row > space - 8192 - 2 * kStageBytes) throw Error(ErrKind::InvalidArgument, "h or i is too large for a token's row to fit shared memory");
+  a.unit = (int)std::max<int64_t>(1, std::min<int64_t>({NT * 8, a.tokens, (space - kKeep - (sizeof(W) == 1 ? 8192 : 0)) / row}));
   a.op_bytes = (int)(a.unit * row);
+  for (int p = 0; p < 2; p++) {
+    const int64_t bytes = (int64_t)(p == 0 ? a.h : a.i) * sizeof(W), n = (bytes + most_bytes(COPY) - 1) / most_bytes(COPY);
+    a.row_bytes[p] = (int)((bytes + n * 128 - 1) / (n * 128) * 128);
+  }
+  a.scale_at = -1;
+  if (sizeof(W) == 1) {
+    const int64_t hb = (a.h + 127) / 128, ib = (a.i + 127) / 128, jb = (2 * (int64_t)a.i + 127) / 128;
+    const int64_t bytes = std::max(hb * jb, hb * ib) * 4;
+    if (bytes <= 8192) a.scale_at = a.op_bytes, a.op_bytes += (int)((bytes + 15) / 16 * 16);
+  }
   a.stages = std::min(kMaxStages, (space - a.op_bytes) / kStageBytes);
   const size_t smem = (size_t)a.op_bytes + red_bytes(NT) + 1024 + (size_t)a.stages * kStageBytes;
   ensure_dynamic_smem((const void*)kern, smem);
   Maps maps{};
   if (COPY == kTensor) {
-    maps.m[0] = weight_map(a.e.w_in, 2 * a.e.experts * a.e.i, a.e.h * sizeof(W));
-    maps.m[1] = weight_map(a.e.w_out, a.e.experts * a.e.h, a.e.i * sizeof(W));
+    maps.m[0] = weight_map(a.e.w_in, 2 * a.e.experts * a.e.i, a.e.h * sizeof(W), a.row_bytes[0]);
+    maps.m[1] = weight_map(a.e.w_out, a.e.experts * a.e.h, a.e.i * sizeof(W), a.row_bytes[1]);
   }
   void* args[] = {&a, &maps};
   NDT_CUDA(cudaLaunchCooperativeKernel((const void*)kern, dim3((unsigned)ctx().sm_count), dim3(warps_of(COPY) * 32), args, smem, s));
@@ -842,7 +903,7 @@ void expert_layer(const ExpertArgs& e, cudaStream_t s) {
     const int64_t row = std::max((int64_t)a.xpitch, 2 * (int64_t)a.bpitch);
     // An expert's second unit of tokens reads its weights again (from L2): more
     // columns where an expert gets more than 6 tokens on average and 16 fit.
-    const bool many = a.tokens * e.top > 6 * e.experts && a.tokens > 8 && 16 * row <= room(2) - 3 * kStageBytes;
+    const bool many = a.tokens * e.top > 6 * e.experts && a.tokens > 8 && 16 * row <= room(2) - 108 * 1024;
     auto go = [&](auto w, auto x, auto m) {
       using W = decltype(w);
       using X = decltype(x);
