@@ -22,8 +22,9 @@ namespace ndt {
 namespace {
 
 constexpr int kSortThreads = 1024;
-constexpr int kPerThread = 4;                      // ids a thread takes in turn
-constexpr int kList = kSortThreads * kPerThread + kSortThreads;  // compacted ids of a range
+constexpr int kPlacers = 512;                      // threads that place ids while the others write zeros
+constexpr int kPerThread = 8;                      // ids a placer takes in turn
+constexpr int kList = kPlacers * kPerThread + kPlacers;  // compacted ids of a range
 constexpr int kEntries = 32;                       // sorted entries a tile
 constexpr int kSumThreads = 256;
 
@@ -74,33 +75,31 @@ __global__ void __launch_bounds__(256) lookup_kernel(const T* __restrict__ table
 }
 
 // ------------------------------------------------------------------ sort
-__device__ __forceinline__ int block_exclusive_scan(int v, int* warp_sums, int* total) {
+// Exclusive sum over the first N threads of the CTA, which all call it; the
+// total too.
+template <int N>
+__device__ __forceinline__ void group_sync() {
+  asm volatile("bar.sync %0, %1;" ::"n"(N == kSortThreads ? 0 : 1), "n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ int exclusive_scan(int v, int* warp_sums, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(~0u, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) warp_sums[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    int s = warp_sums[lane], t = s;
+  auto inclusive = [&](int x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(~0u, t, o);
-      if (lane >= o) t += y;
+      const int y = __shfl_up_sync(~0u, x, o);
+      if (lane >= o) x += y;
     }
-    warp_sums[lane] = t - s;
-    if (lane == 31) *total = t;
-  }
-  __syncthreads();
-  const int r = warp_sums[warp] + x - v;
-  const int tot = *total;
-  __syncthreads();
-  v = r;
-  *total = tot;
-  return v;
+    return x;
+  };
+  const int x = inclusive(v);
+  if (lane == 31) warp_sums[warp] = x;
+  group_sync<N>();
+  const int sums = inclusive(lane < N / 32 ? warp_sums[lane] : 0);
+  total = __shfl_sync(~0u, sums, 31);
+  const int before = __shfl_sync(~0u, sums, (warp + 31) & 31);
+  group_sync<N>();
+  return (warp ? before : 0) + x - v;
 }
 
 struct SortArgs {
@@ -120,56 +119,66 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortArgs a) {
   int* list_key = sm + a.range;     // [kList]
   int* list_pos = list_key + kList;
   __shared__ int warp_sums[32];
-  __shared__ int total, list_n;
-  __shared__ int below_s;
+  __shared__ int list_n, below_s;
+  __shared__ unsigned present[1024];  // a bit a row of the range: it has an id
   pdl_release();
   pdl_wait();
   const uint64_t v0 = blockIdx.x * (uint64_t)a.range, v1 = min((uint64_t)a.v, v0 + a.range);
   const int rows = (int)(v1 - v0);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < a.range; i += kSortThreads) start[i] = 0;
   if (threadIdx.x == 0) below_s = 0, list_n = 0;
   __syncthreads();
   int below = 0;
-  for (int64_t i = threadIdx.x; i < a.n; i += kSortThreads) {
-    const uint64_t r = row_at<IDS64>(a.ids, i, a.first);
-    if (r < v0) below++;
-    if (r >= v0 && r < v1) atomicAdd(&start[r - v0], 1);
+  for (int64_t i0 = threadIdx.x; i0 < a.n; i0 += kSortThreads * 8) {
+    uint64_t r[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) r[j] = i0 + j * kSortThreads < a.n ? row_at<IDS64>(a.ids, i0 + j * kSortThreads, a.first) : ~0ull;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      if (r[j] < v0) below++;
+      if (r[j] >= v0 && r[j] < v1) atomicAdd(&start[r[j] - v0], 1);
+    }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) below += __shfl_xor_sync(~0u, below, o);
-  if ((threadIdx.x & 31) == 0 && below) atomicAdd(&below_s, below);
+  if (lane == 0 && below) atomicAdd(&below_s, below);
   __syncthreads();
-  // the zeros of rows without an id
-  if (a.out) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // counts -> first places
+  const int base0 = below_s;
+  int base = base0;
+  for (int i0 = 0; i0 < a.range; i0 += kSortThreads) {
+    const int i = i0 + threadIdx.x;
+    const int c = i < a.range ? start[i] : 0;
+    const unsigned on = __ballot_sync(~0u, c > 0);
+    if (lane == 0) present[i >> 5] = on;
+    int total;
+    const int before = exclusive_scan<kSortThreads>(c, warp_sums, total);
+    if (i < a.range) start[i] = base + before;
+    base += total;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && v1 == (uint64_t)a.v) *a.count = base;
+  const bool none = base == base0;  // no id in this range
+  if (threadIdx.x >= kPlacers || none) {
+    // the zeros of rows without an id
+    if (!a.out) return;
+    const int first = none ? 0 : kPlacers / 32, step = kSortThreads / 32 - first;
     const bool vec = a.d_bytes % 16 == 0 && a.ld_bytes % 16 == 0 && (uintptr_t)a.out % 16 == 0;
-    for (int r = warp; r < rows; r += kSortThreads / 32) {
-      if (start[r]) continue;
+    for (int r = warp - first; r < rows; r += step) {
+      if (present[r >> 5] >> (r & 31) & 1) continue;
       unsigned char* p = (unsigned char*)a.out + (v0 + r) * a.ld_bytes;
       if (vec)
         for (int64_t c = lane * 16; c < a.d_bytes; c += 512) *reinterpret_cast<uint4*>(p + c) = make_uint4(0, 0, 0, 0);
       else
         for (int64_t c = lane * 2; c < a.d_bytes; c += 64) *reinterpret_cast<uint16_t*>(p + c) = 0;
     }
+    return;
   }
-  __syncthreads();
-  // counts -> first places
-  int base = below_s;
-  for (int64_t i0 = 0; i0 < a.range; i0 += kSortThreads) {
-    const int64_t i = i0 + threadIdx.x;
-    const int c = i < a.range ? start[i] : 0;
-    const int before = block_exclusive_scan(c, warp_sums, &total);
-    if (i < a.range) start[i] = base + before;
-    base += total;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0 && v1 == (uint64_t)a.v) *a.count = base;
-  if (base == below_s) return;  // no id in this range
   // ids of the range, compacted in order of position, then placed
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto place = [&](int upto) {  // whole list: batches of one entry a thread
-    for (int b = 0; b < upto; b += kSortThreads) {
-      const int m = min(kSortThreads, upto - b);
+  auto place = [&](int upto) {  // the whole list: batches of one entry a thread
+    for (int b = 0; b < upto; b += kPlacers) {
+      const int m = min(kPlacers, upto - b);
       const bool on = (int)threadIdx.x < m;
       const int key = on ? list_key[b + threadIdx.x] : -1;
       const unsigned same = __match_any_sync(~0u, key);
@@ -187,53 +196,39 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortArgs a) {
             a.rows[at] = (int)(v0 + key);
           }
         }
-        __syncthreads();
+        group_sync<kPlacers>();
       }
     }
   };
-  for (int64_t i0 = 0; i0 < a.n; i0 += kSortThreads * kPerThread) {
-    int key[kPerThread], mine = 0;
+  for (int64_t i0 = 0; i0 < a.n; i0 += kPlacers * kPerThread) {
+    uint64_t r[kPerThread];
+    int mine = 0;
+    const int64_t at0 = i0 + threadIdx.x * kPerThread;
 #pragma unroll
-    for (int j = 0; j < kPerThread; j++) {
-      const int64_t i = i0 + threadIdx.x * kPerThread + j;
-      const uint64_t r = i < a.n ? row_at<IDS64>(a.ids, i, a.first) : ~0ull;
-      key[j] = r >= v0 && r < v1 ? (int)(r - v0) : -1;
-      mine += key[j] >= 0;
-    }
-    int at = list_n + block_exclusive_scan(mine, warp_sums, &total);
+    for (int j = 0; j < kPerThread; j++) r[j] = at0 + j < a.n ? row_at<IDS64>(a.ids, at0 + j, a.first) : ~0ull;
+#pragma unroll
+    for (int j = 0; j < kPerThread; j++) mine += r[j] >= v0 && r[j] < v1;
+    int total;
+    int at = list_n + exclusive_scan<kPlacers>(mine, warp_sums, total);
 #pragma unroll
     for (int j = 0; j < kPerThread; j++)
-      if (key[j] >= 0) {
-        list_key[at] = key[j];
-        list_pos[at++] = (int)(i0 + threadIdx.x * kPerThread + j);
+      if (r[j] >= v0 && r[j] < v1) {
+        list_key[at] = (int)(r[j] - v0);
+        list_pos[at++] = (int)(at0 + j);
       }
     const int have = list_n + total;
-    __syncthreads();
-    if (have > kSortThreads || i0 + kSortThreads * kPerThread >= a.n) {
+    group_sync<kPlacers>();
+    if (have > kPlacers || i0 + kPlacers * kPerThread >= a.n) {
       place(have);
       if (threadIdx.x == 0) list_n = 0;
     } else if (threadIdx.x == 0) {
       list_n = have;
     }
-    __syncthreads();
+    group_sync<kPlacers>();
   }
 }
 
 // ------------------------------------------------------------------- sum
-template <typename T>
-__device__ __forceinline__ void add_vec(const T* p, float* acc, int n, bool vec) {
-  constexpr int kN = 16 / sizeof(T);
-  if (vec) {
-    const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
-    const T* e = reinterpret_cast<const T*>(&x);
-#pragma unroll
-    for (int q = 0; q < kN; q++) acc[q] += to_f32<T>(e[q]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < kN; q++)
-      if (q < n) acc[q] += to_f32<T>(p[q]);
-  }
-}
 __device__ __forceinline__ void put(void* out, int64_t i, MType t, float v, bool add) {
   if (t == MType::F32) {
     float* p = (float*)out + i;
@@ -257,7 +252,7 @@ struct SumArgs {
   void* out;
   int64_t ldo;
   MType ot;
-  bool accumulate, vec;
+  bool accumulate, vec, out_vec;  // out_vec: out has grad's type and 16-byte rows
   float* head;  // [tiles, d] a tile's part of the row it shares with the tile before
   float* tail;  // [tiles, d] ... of the row it shares with the tile after (and not before)
 };
@@ -283,69 +278,95 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(const SumArgs a) {
   const int nc = (int)min((int64_t)kN, a.d - c);
   float acc[kN] = {};
   bool started_before = rows[0] == rows[1];
-  for (int e = 0; e < m; e++) {
-    add_vec<T>((const T*)a.grad + (int64_t)order[e] * a.ldg + c, acc, nc, a.vec);
-    const int row = rows[e + 1];
-    if (rows[e + 2] == row && e + 1 < m) continue;
-    const bool goes_on = rows[e + 2] == row;  // into the next tile
-    if (started_before || goes_on) {
-      float* p = (started_before ? a.head : a.tail) + blockIdx.x * a.d + c;
+  constexpr int kFly = 8;  // rows of grad in flight a thread
+  for (int e0 = 0; e0 < m; e0 += kFly) {
+    uint4 x[kFly];
 #pragma unroll
-      for (int q = 0; q < kN; q++)
-        if (q < nc) p[q] = acc[q];
-    } else {
+    for (int j = 0; j < kFly; j++) {
+      x[j] = make_uint4(0, 0, 0, 0);
+      if (e0 + j >= m) continue;
+      const T* p = (const T*)a.grad + (int64_t)order[e0 + j] * a.ldg + c;
+      if (a.vec) {
+        x[j] = __ldg(reinterpret_cast<const uint4*>(p));
+      } else {
+        T* v = reinterpret_cast<T*>(&x[j]);
 #pragma unroll
-      for (int q = 0; q < kN; q++)
-        if (q < nc) put(a.out, row * a.ldo + c + q, a.ot, acc[q] * a.scale, a.accumulate);
+        for (int q = 0; q < kN; q++)
+          if (q < nc) v[q] = p[q];
+      }
     }
 #pragma unroll
-    for (int q = 0; q < kN; q++) acc[q] = 0.f;
-    started_before = false;
+    for (int j = 0; j < kFly; j++) {
+      const int e = e0 + j;
+      if (e >= m) break;
+      const T* v = reinterpret_cast<const T*>(&x[j]);
+#pragma unroll
+      for (int q = 0; q < kN; q++) acc[q] += to_f32<T>(v[q]);
+      const int row = rows[e + 1];
+      if (rows[e + 2] == row && e + 1 < m) continue;
+      const bool goes_on = rows[e + 2] == row;  // into the next tile
+      if (started_before || goes_on) {
+        float* p = (started_before ? a.head : a.tail) + blockIdx.x * a.d + c;
+#pragma unroll
+        for (int q = 0; q < kN; q++)
+          if (q < nc) p[q] = acc[q];
+      } else if (nc == kN && a.out_vec && !a.accumulate) {
+        if constexpr (sizeof(T) == 4) {  // (out has grad's type here)
+          *reinterpret_cast<float4*>((float*)a.out + row * a.ldo + c) = make_float4(acc[0] * a.scale, acc[1] * a.scale, acc[2] * a.scale, acc[3] * a.scale);
+        } else {
+          alignas(16) T w[kN];
+#pragma unroll
+          for (int q = 0; q < kN; q++) w[q] = from_f32<T>(acc[q] * a.scale);
+          *reinterpret_cast<uint4*>((T*)a.out + row * a.ldo + c) = *reinterpret_cast<const uint4*>(w);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kN; q++)
+          if (q < nc) put(a.out, row * a.ldo + c + q, a.ot, acc[q] * a.scale, a.accumulate);
+      }
+#pragma unroll
+      for (int q = 0; q < kN; q++) acc[q] = 0.f;
+      started_before = false;
+    }
   }
 }
 
-// Rows that cross tiles: the CTA of the tile where the row starts adds its
-// tail and the heads of the tiles after it, in order.  Eight warps take
-// neighbouring stretches of the tiles and are added in warp order.
-__global__ void __launch_bounds__(256) join_kernel(const SumArgs a) {
-  __shared__ float part[8][32];
-  __shared__ int last_s;
+// Rows that cross tiles: the CTAs of the tile where the row starts add its
+// tail and the heads of the tiles after it, in order.  Eight groups of 128
+// threads take neighbouring stretches of the tiles and are added in their
+// order; a CTA has 128 columns (a few ids make up much of a batch, so one
+// row's chain can be most of the work).
+constexpr int kJoinColumns = 128, kStretches = 8;
+__global__ void __launch_bounds__(kJoinColumns* kStretches) join_kernel(const SumArgs a) {
+  __shared__ float part[kStretches][kJoinColumns];
   pdl_release();
   pdl_wait();
   const int n = *a.count;
   const int64_t t = blockIdx.x, e0 = t * kEntries, e1 = e0 + kEntries;
   if (e1 >= n) return;
-  const int row = a.rows[e1 - 1];
-  if (a.rows[e1] != row) return;
-  if (a.rows[e0] == row && e0 > 0 && a.rows[e0 - 1] == row) return;  // starts earlier
-  if (threadIdx.x == 0) {
-    int64_t lo = e1, hi = n;  // first entry of another row
-    while (lo < hi) {
-      const int64_t mid = (lo + hi) / 2;
-      if (a.rows[mid] == row)
-        lo = mid + 1;
-      else
-        hi = mid;
-    }
-    last_s = (int)((lo - 1) / kEntries);
+  const int row = a.rows[e1 - 1], next = a.rows[e1], first = a.rows[e0], before = e0 > 0 ? a.rows[e0 - 1] : -1;
+  if (next != row || (first == row && before == row)) return;  // does not cross, or starts earlier
+  // the tiles after t that begin with the row
+  int64_t heads = 0;
+  for (int more = blockDim.x; more == (int)blockDim.x; heads += more) {
+    const int64_t e = e1 + (heads + threadIdx.x) * kEntries;
+    more = __syncthreads_count(e < n && a.rows[e] == row);
   }
-  __syncthreads();
-  const int64_t heads = last_s - t;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t per = (heads + 7) / 8, h0 = t + 1 + warp * per, h1 = min(t + 1 + heads, h0 + per);
-  for (int64_t c0 = 0; c0 < a.d; c0 += 32) {
+  const int group = threadIdx.x / kJoinColumns, lane = threadIdx.x % kJoinColumns;
+  const int64_t per = (heads + kStretches - 1) / kStretches, h0 = t + 1 + group * per, h1 = min(t + 1 + heads, h0 + per);
+  for (int64_t c0 = blockIdx.y * (int64_t)kJoinColumns; c0 < a.d; c0 += gridDim.y * (int64_t)kJoinColumns) {
     const int64_t c = c0 + lane;
     float v = 0.f;
     if (c < a.d) {
 #pragma unroll 8
       for (int64_t h = h0; h < h1; h++) v += a.head[h * a.d + c];
     }
-    part[warp][lane] = v;
+    part[group][lane] = v;
     __syncthreads();
-    if (warp == 0 && c < a.d) {
+    if (group == 0 && c < a.d) {
       float s = a.tail[t * a.d + c];
 #pragma unroll
-      for (int w = 0; w < 8; w++) s += part[w][lane];
+      for (int w = 0; w < kStretches; w++) s += part[w][lane];
       put(a.out, row * a.ldo + c, a.ot, s * a.scale, a.accumulate);
     }
     __syncthreads();
@@ -414,6 +435,7 @@ void embedding_grad(MType gt, const void* grad, int64_t ldg, const void* ids, bo
   b.head = parts, b.tail = parts + tiles * d;
   const int kn = 16 / msize(gt);
   b.vec = d % kn == 0 && ldg % kn == 0 && (uintptr_t)grad % 16 == 0;
+  b.out_vec = ot == gt && ldo % kn == 0 && (uintptr_t)out % 16 == 0;
   const dim3 grid((unsigned)tiles, (unsigned)((d + kSumThreads * kn - 1) / (kSumThreads * kn)));
   if (gt == MType::F32)
     launch_pdl(sum_kernel<float>, grid, dim3(kSumThreads), 0, s, b);
@@ -423,7 +445,8 @@ void embedding_grad(MType gt, const void* grad, int64_t ldg, const void* ids, bo
     launch_pdl(sum_kernel<__half>, grid, dim3(kSumThreads), 0, s, b);
   count_launch();
   if (tiles > 1) {
-    launch_pdl(join_kernel, dim3((unsigned)(tiles - 1)), dim3(256), 0, s, b);
+    const unsigned chunks = (unsigned)std::min<int64_t>(8, (d + kJoinColumns - 1) / kJoinColumns);
+    launch_pdl(join_kernel, dim3((unsigned)(tiles - 1), chunks), dim3(kJoinColumns * kStretches), 0, s, b);
     count_launch();
   }
 }

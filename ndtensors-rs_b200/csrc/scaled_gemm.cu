@@ -62,7 +62,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 }
 __device__ __forceinline__ uint32_t mapa(uint32_t addr, uint32_t rank) {
   uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
   return r;
 }
 template <int CTAS>
@@ -163,7 +163,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 }
 __device__ __forceinline__ float ld_cluster(uint32_t addr) {
   float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr));
   return v;
 }
 // One 4-byte element into shared memory; zero where !valid.
@@ -479,16 +479,34 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
     const int rows = min(128, g.m - tm * 128), cols = min(BN, g.n - tn * BN);
     const bool by_row = g.crs == 1;
     const int fast = by_row ? rows : cols, total = rows * cols;
-    for (int e = total * split / g.ksplit + threadIdx.x; e < total * (split + 1) / g.ksplit; e += kThreads) {
-      const int lo = e % fast, hi = e / fast;
-      const int r = by_row ? lo : hi, j = by_row ? hi : lo;
-      const uint32_t at = stage0 + (uint32_t)(j * 129 + r) * 4;
-      float v = 0.f;
-      for (int p = 0; p < g.ksplit; p++) v += ld_cluster(mapa(at, p));
+    const int end = total * (split + 1) / g.ksplit;
+    constexpr int kFly = 8;  // elements a thread fetches at a time: a peer's memory is far
+    for (int e0 = total * split / g.ksplit + threadIdx.x; e0 < end; e0 += kThreads * kFly) {
+      float v[kFly] = {};
+      uint32_t at[kFly];
+      int64_t to[kFly];
+#pragma unroll
+      for (int i = 0; i < kFly; i++) {
+        const int e = min(e0 + i * kThreads, end - 1);
+        const int lo = e % fast, hi = e / fast;
+        const int r = by_row ? lo : hi, j = by_row ? hi : lo;
+        at[i] = stage0 + (uint32_t)(j * 129 + r) * 4;
+        to[i] = (tm * 128 + r) * g.crs + (tn * BN + j) * g.ccs;
+      }
+      for (int p = 0; p < g.ksplit; p++) {
+        float w[kFly];
+#pragma unroll
+        for (int i = 0; i < kFly; i++) w[i] = ld_cluster(mapa(at[i], p));
+#pragma unroll
+        for (int i = 0; i < kFly; i++) v[i] += w[i];
+      }
       if (*gave_up) continue;
-      const int64_t i = (tm * 128 + r) * g.crs + (tn * BN + j) * g.ccs;
-      if (g.accumulate) v += load_c(g.c, i, g.ctype);
-      store_c(g.c, i, g.ctype, v);
+#pragma unroll
+      for (int i = 0; i < kFly; i++) {
+        if (e0 + i * kThreads >= end) break;
+        if (g.accumulate) v[i] += load_c(g.c, to[i], g.ctype);
+        store_c(g.c, to[i], g.ctype, v[i]);
+      }
     }
     cluster_sync();
   } else if (CTAS == 2) {
