@@ -222,7 +222,7 @@ int ndt_b200_scaled_linear_dev(int x_type, const void* x, long tokens, long k, l
     Workspace ws(qx.bytes(), s);
     qx.place(ws.p);
     quantize(xt, qx.x, 1, MType::E4M3, qx.out(), QuantOut{}, s);
-    scaled_gemm(qx.operand(), lw.o, k, yt, y, ldy, false, s);
+    scaled_gemm(qx.operand(), lw.o, k, yt, y, ldy, false, s, !lw.copy.p);
   });
 }
 

@@ -52,8 +52,11 @@ struct ScaledOperand {
   int64_t srs, scs;
   bool per_row;  // a scale for each row; else for each 128 rows
 };
+// b_early: b was complete before the kernel that the stream ran last began (a
+// quantize(), which waits for what is ahead of it before it lets the next
+// kernel start), so its loads need not wait for that kernel.
 void scaled_gemm(const ScaledOperand& a, const ScaledOperand& b, int64_t k, MType ct, void* c, int64_t ldc,
-                 bool accumulate, cudaStream_t s);
+                 bool accumulate, cudaStream_t s, bool b_early = false);
 
 // Embedding (embedding.cu).
 void embedding(MType t, const void* table, int64_t v, int64_t d, int64_t ldt, const void* ids, bool ids64, int64_t n,

@@ -124,8 +124,8 @@ __device__ __forceinline__ void store8(const QArgs& a, int64_t r, int64_t c, con
 constexpr int kRows = 4;
 template <typename T, typename Q, bool VEC>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QArgs a) {
-  pdl_release();
   pdl_wait();
+  pdl_release();  // (in this order: the next kernel may read what was ready before this one)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t r0 = ((int64_t)blockIdx.y * (kThreads / 32) + warp) * kRows, c = blockIdx.x * 256ll + lane * 8;
   if (r0 >= a.rows) return;

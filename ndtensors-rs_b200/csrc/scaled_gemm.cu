@@ -9,7 +9,7 @@
 // accumulators in registers, in 32 bits.  Two TMEM buffers let the tensor
 // core work on block kb + 1 meanwhile.
 //
-// Roles (12 warps): 0 loads the operand tiles by TMA into a ring of 128-byte
+// Roles: warp 0 loads the operand tiles by TMA into a ring of 128-byte
 // swizzled stages, 1 issues the MMAs, 2 loads the scales into a ring of its
 // own (cp.async), 4 - 11 scale and sum (a thread holds one row and half the
 // tile's columns).
@@ -31,9 +31,7 @@ namespace ndt {
 namespace {
 
 constexpr int kBK = 128;     // one scale block, one swizzled row
-constexpr int kThreads = 384;
-constexpr int kEpiWarp0 = 4;  // the epilogue is two whole warpgroups (setmaxnreg)
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarp0 = 4;  // the epilogue is whole warpgroups (setmaxnreg)
 constexpr int kSlots = 8;    // scale ring
 
 struct GemmArgs {
@@ -50,6 +48,7 @@ struct GemmArgs {
   int ctype;       // MType of C
   int accumulate;
   int vec;         // rows of C are contiguous and their 16-byte stores aligned
+  int early_a;     // A was there before the kernel ahead in the stream: its first tiles need not wait for it
   int* flag;       // set when a bounded wait ran out
 };
 
@@ -207,6 +206,9 @@ struct Shape {
   static constexpr int kStages = (kResident == 2 ? 100 : 192) * 1024 / kStage;
   static constexpr int kScaleFloats = kBM + (BN + 31) / 32 * 32;  // a slot of the scale ring
   static constexpr int kTmemCols = 2 * BN;
+  static constexpr int kEpiWarps = 8;  // (16, with half the registers each, wait in each other's way: 86 -> 107 us for 4096^3)
+  static constexpr int kCols = BN / (kEpiWarps / 4);  // columns of one epilogue thread
+  static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
   static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + (size_t)kSlots * kScaleFloats * 4;
   static_assert(kTmemCols >= 32 && kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns");
   static_assert((size_t)BN * 129 * 4 <= (size_t)kStages * kStage || CTAS == 2, "the split's buffer reuses the stages");
@@ -214,11 +216,11 @@ struct Shape {
 };
 
 template <int CTAS, int BN, bool BROW>
-__global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
+__global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, Shape<CTAS, BN>::kResident)
     scaled_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                        const GemmArgs g) {
   using S = Shape<CTAS, BN>;
-  constexpr int kHalf = BN / 2;  // columns of one epilogue thread
+  constexpr int kCols = S::kCols, kThreads = S::kThreads, kEpiWarps = S::kEpiWarps;
   extern __shared__ unsigned char raw[];
   __shared__ __align__(8) uint64_t bars[2 * S::kStages + 2 * kSlots + 4];
   __shared__ uint32_t tmem_base_s;
@@ -255,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
   fence_after();
   const uint32_t tmem = tmem_base_s;
   pdl_release();
-  pdl_wait();
+  if (CTAS == 2 || !g.early_a || warp != 0) pdl_wait();
 
   const int split = CTAS == 1 && g.ksplit > 1 ? (int)cluster_rank() : 0;
   const int unit = CTAS == 1 ? blockIdx.x / g.ksplit : blockIdx.x / 2;
@@ -274,11 +276,27 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
+      int ahead = 0;  // stages whose A is on its way already
+      if (CTAS == 1 && g.early_a) {
+        int tm, tn;
+        tile_at(unit, g.tiles_m, g.tiles_n, tm, tn);
+        for (; ahead < S::kStages && kb0 + ahead < kb1; ahead++) {
+          mbar_expect_tx(full + 8 * ahead, S::kStage);
+          tma_load<CTAS>(stage0 + ahead * S::kStage, &map_a, full + 8 * ahead, (kb0 + ahead) * kBK, tm * 128);
+        }
+        pdl_wait();
+      }
       for (int t = unit; t < ntiles && ok; t += units) {
         int tm, tn;
         tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
         const int row_a = tm * 128 * CTAS + rank * 128, row_b = tn * BN + rank * S::kBRows;
         for (int kb = kb0; kb < kb1; kb++) {
+          if (ahead > 0) {
+            ahead--;
+            tma_load<CTAS>(stage0 + stage * S::kStage + S::kABytes, &map_b, full + 8 * stage, kb * kBK, row_b);
+            if (++stage == S::kStages) stage = 0, phase ^= 1;
+            continue;
+          }
           if (!(ok = mbar_wait(empty + 8 * stage, phase ^ 1, gave_up, g.flag))) break;
           const uint32_t dst = stage0 + stage * S::kStage;
           uint32_t bar = full + 8 * stage;
@@ -326,33 +344,22 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
       int tm, tn;
       tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
       const int row_a = tm * 128 * CTAS + rank * 128, row_b = tn * BN;
-      // this lane's rows: their addresses at k block 0
-      const float* pa[4];
-      bool va[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int r = row_a + lane + 32 * j;
-        va[j] = r < g.m;
-        pa[j] = g.sa + (va[j] ? (int64_t)(g.a_row ? r : r >> 7) * g.sa_rs : 0);
-      }
+      // this lane's rows; those past the matrix read its last and are stored as zeros
+      auto scale_a = [&](int j) { return min(row_a + lane + 32 * j, g.m - 1) >> (g.a_row ? 0 : 7); };
       constexpr int kNB = BROW ? (BN + 31) / 32 : 1;
-      const float* pb[kNB];
-      bool vb[kNB];
-#pragma unroll
-      for (int j = 0; j < kNB; j++) {
-        const int r = BROW ? row_b + lane + 32 * j : row_b + lane * 128;
-        vb[j] = r < g.n && (BROW ? lane + 32 * j < BN : lane < (BN + 127) / 128);
-        pb[j] = g.sb + (vb[j] ? (int64_t)(BROW && g.b_row ? r : r >> 7) * g.sb_rs : 0);
-      }
+      auto row_of_b = [&](int j) { return BROW ? row_b + lane + 32 * j : row_b + lane * 128; };
+      auto scale_b = [&](int j) { return min(row_of_b(j), g.n - 1) >> (BROW && g.b_row ? 0 : 7); };
       for (int kb = kb0; kb < kb1; kb++, it++) {
         const uint32_t slot = it % kSlots, ph = (it / kSlots) & 1;
         if (!(ok = warp_wait(sempty + 8 * slot, ph ^ 1, gave_up, g.flag))) break;
         const uint32_t dst = smem_u32(scale_ring + slot * S::kScaleFloats) + 4 * lane;
 #pragma unroll
-        for (int j = 0; j < 4; j++) cp4(dst + 128 * j, pa[j] + (int64_t)kb * g.sa_cs, va[j]);
+        for (int j = 0; j < 4; j++)
+          cp4(dst + 128 * j, g.sa + scale_a(j) * g.sa_rs + kb * g.sa_cs, row_a + lane + 32 * j < g.m);
 #pragma unroll
         for (int j = 0; j < kNB; j++)
-          if (BROW || lane < (BN + 127) / 128) cp4(dst + 512 + 128 * j, pb[j] + (int64_t)kb * g.sb_cs, vb[j]);
+          if (BROW ? lane + 32 * j < BN : lane < (BN + 127) / 128)
+            cp4(dst + 512 + 128 * j, g.sb + scale_b(j) * g.sb_rs + kb * g.sb_cs, row_of_b(j) < g.n);
         asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sfull + 8 * slot) : "memory");
       }
     }
@@ -362,25 +369,25 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
     fewer();
   } else {
     more();
-    const int quad = warp & 3, half = (warp - kEpiWarp0) >> 2;
+    const int quad = warp & 3, band = (warp - kEpiWarp0) >> 2;
     const int row = quad * 32 + lane;
-    const uint32_t tmem_row = tmem + ((uint32_t)(quad * 32) << 16) + half * kHalf;
+    const uint32_t tmem_row = tmem + ((uint32_t)(quad * 32) << 16) + band * kCols;
     const uint32_t tempty_leader = CTAS == 2 ? mapa(tempty, 0) : tempty;
-    constexpr int kLd = kHalf < 16 ? kHalf : 16, kLoads = kHalf / kLd, kFly = kLoads < 4 ? kLoads : 4;
+    constexpr int kLd = kCols < 16 ? kCols : 16, kLoads = kCols / kLd, kFly = kLoads < 4 ? kLoads : 4;
     uint32_t it = 0;
     bool ok = true;
     for (int t = unit; t < ntiles && ok; t += units) {
       int tm, tn;
       tile_at(t, g.tiles_m, g.tiles_n, tm, tn);
-      uint64_t acc[kHalf / 2];
+      uint64_t acc[kCols / 2];
 #pragma unroll
-      for (int j = 0; j < kHalf / 2; j++) acc[j] = 0;
+      for (int j = 0; j < kCols / 2; j++) acc[j] = 0;
       for (int kb = kb0; kb < kb1; kb++, it++) {
         const uint32_t slot = it % kSlots, sph = (it / kSlots) & 1, buf = it & 1, ph = (it >> 1) & 1;
         if (!(ok = warp_wait(sfull + 8 * slot, sph, gave_up, g.flag))) break;
         const float* sc = scale_ring + slot * S::kScaleFloats;
         const float sa = sc[row];
-        const float sab = BROW ? sa : sa * sc[128 + (BN == 256 ? half : 0)];
+        const float sab = BROW ? sa : sa * sc[128 + (BN == 256 ? band : 0)];
         const uint64_t s2 = pair(sab, sab);
         if (!(ok = warp_wait(tfull + 8 * buf, ph, gave_up, g.flag))) break;
         fence_after();
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
           for (int j = 0; j < kLd; j += 4) {
             uint64_t f0 = s2, f1 = s2;
             if (BROW) {
-              const float4 b = *reinterpret_cast<const float4*>(sc + 128 + half * kHalf + q * kLd + j);
+              const float4 b = *reinterpret_cast<const float4*>(sc + 128 + band * kCols + q * kLd + j);
               f0 = mul2(s2, pair(b.x, b.y)), f1 = mul2(s2, pair(b.z, b.w));
             }
             uint64_t& a0 = acc[(q * kLd + j) / 2];
@@ -423,24 +430,24 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
       }
       if (!ok) break;
       auto at = [&](int j) { return __uint_as_float((uint32_t)(acc[j / 2] >> (j & 1) * 32)); };
-      const int row_c = tm * 128 * CTAS + rank * 128 + row, col_c = tn * BN + half * kHalf;
+      const int row_c = tm * 128 * CTAS + rank * 128 + row, col_c = tn * BN + band * kCols;
       if (CTAS == 1 && g.ksplit > 1) {
         // this CTA's part, column-major with an odd pitch, over the stages (all consumed)
         float* part = reinterpret_cast<float*>(raw + (stage0 - smem_u32(raw)));
 #pragma unroll
-        for (int j = 0; j < kHalf; j++) part[(half * kHalf + j) * 129 + row] = at(j);
+        for (int j = 0; j < kCols; j++) part[(band * kCols + j) * 129 + row] = at(j);
       } else if (row_c < g.m) {
         const int64_t base = row_c * g.crs + col_c * g.ccs;
-        const int cols = min(kHalf, g.n - col_c);
-        if (g.vec && cols == kHalf && !g.accumulate) {
+        const int cols = min(kCols, g.n - col_c);
+        if (g.vec && cols == kCols && !g.accumulate) {
           if (g.ctype == (int)MType::F32) {
             float4* p = reinterpret_cast<float4*>((float*)g.c + base);
 #pragma unroll
-            for (int j = 0; j < kHalf / 4; j++) p[j] = make_float4(at(4 * j), at(4 * j + 1), at(4 * j + 2), at(4 * j + 3));
+            for (int j = 0; j < kCols / 4; j++) p[j] = make_float4(at(4 * j), at(4 * j + 1), at(4 * j + 2), at(4 * j + 3));
           } else {
             uint4* p = reinterpret_cast<uint4*>((uint16_t*)g.c + base);
 #pragma unroll
-            for (int j = 0; j < kHalf / 8; j++) {
+            for (int j = 0; j < kCols / 8; j++) {
               uint32_t w[4];
 #pragma unroll
               for (int i = 0; i < 4; i++) {
@@ -457,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, Shape<CTAS, BN>::kResident)
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < kHalf; j++)
+          for (int j = 0; j < kCols; j++)
             if (j < cols) {
               float v = at(j);
               if (g.accumulate) v += load_c(g.c, base + j * g.ccs, g.ctype);
@@ -537,7 +544,7 @@ void launch(const ScaledOperand& a, const ScaledOperand& b, int64_t k, GemmArgs 
   ensure_dynamic_smem((const void*)kern, S::kSmem);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kSmem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];
@@ -555,7 +562,7 @@ void launch(const ScaledOperand& a, const ScaledOperand& b, int64_t k, GemmArgs 
 }  // namespace
 
 void scaled_gemm(const ScaledOperand& a_, const ScaledOperand& b_, int64_t k, MType ct, void* c, int64_t ldc,
-                 bool accumulate, cudaStream_t s) {
+                 bool accumulate, cudaStream_t s, bool b_early) {
   // Up to 64 rows of A: B's rows on the 128 lanes, A's as 16 to 64 columns.
   const bool swap = a_.rows <= 64;
   const ScaledOperand &a = swap ? b_ : a_, &b = swap ? a_ : b_;
@@ -569,6 +576,7 @@ void scaled_gemm(const ScaledOperand& a_, const ScaledOperand& b_, int64_t k, MT
   g.vec = !swap && (uintptr_t)c % 16 == 0 && ldc * msize(ct) % 16 == 0;
   g.flag = wait_flag_device();
   g.ksplit = 1;
+  g.early_a = swap && b_early;
   const int sms = ctx().sm_count;
   auto cdiv = [](int64_t x, int64_t y) { return (int)((x + y - 1) / y); };
   // bits of the instruction descriptor: 32-bit accumulators, the operands'
@@ -591,9 +599,11 @@ void scaled_gemm(const ScaledOperand& a_, const ScaledOperand& b_, int64_t k, MT
   const int bn = !swap ? 128 : g.n <= 16 ? 16 : g.n <= 32 ? 32 : 64;
   g.tiles_m = cdiv(g.m, 128), g.tiles_n = cdiv(g.n, bn);
   g.idesc = idesc(128, bn);
-  // k is split while the CTAs fit the GPU at once and keep at least 4 blocks each
+  // k is split while the CTAs fit the GPU at once and keep enough blocks each:
+  // adding the parts of a 128 x 128 tile costs what 16 blocks do (train step of
+  // 1000 tokens: 29 us for 7 blocks a CTA, 16 us unsplit with 9), of few columns less
   const int room = sms * (swap ? 2 : 1), tiles = g.tiles_m * g.tiles_n;
-  g.ksplit = std::max(1, std::min({8, room / tiles, g.kblocks / 4}));
+  g.ksplit = std::max(1, std::min({8, room / tiles, g.kblocks / (swap ? 4 : 16)}));
   const int grid = tiles * g.ksplit;
   if (!swap)
     b.per_row ? launch<1, 128, true>(a, b, k, g, grid, g.ksplit, s) : launch<1, 128, false>(a, b, k, g, grid, g.ksplit, s);
