@@ -28,7 +28,7 @@ def expert_layer(x, router, w_in, w_out, top: int, in_scales=None, out_scales=No
 
     Returns ``(y, ids, weights)``: x's shape and type, and int32 / float32
     [..., top].  Made for at most about a hundred tokens (a decoding batch);
-    more are right, but each 8 to 32 tokens of an expert read its weights anew.
+    more are right, but each 8 or 16 tokens of an expert read its weights anew.
     """
     device = device_of("expert_layer", x, router, w_in, w_out, in_scales, out_scales)
     xt = code_of("expert_layer", "x", x.dtype, _HALF)
