@@ -26,7 +26,7 @@ constexpr int kPlacers = 512;                      // threads that place ids whi
 constexpr int kPerThread = 8;                      // ids a placer takes in turn
 constexpr int kList = kPlacers * kPerThread + kPlacers;  // compacted ids of a range
 constexpr int kEntries = 32;                       // sorted entries a tile
-constexpr int kSumThreads = 256;
+constexpr int kSumThreads = 128;                   // (256 leave a last wave of half the SMs)
 
 // The table's row of id i; at least 2^63 for an id below the table's first.
 template <bool IDS64>
@@ -119,7 +119,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortArgs a) {
   int* list_key = sm + a.range;     // [kList]
   int* list_pos = list_key + kList;
   __shared__ int warp_sums[32];
-  __shared__ int list_n, below_s;
+  __shared__ int list_n, below_s, next_row;
   __shared__ unsigned present[1024];  // a bit a row of the range: it has an id
   pdl_release();
   pdl_wait();
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortArgs a) {
   const int rows = (int)(v1 - v0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < a.range; i += kSortThreads) start[i] = 0;
-  if (threadIdx.x == 0) below_s = 0, list_n = 0;
+  if (threadIdx.x == 0) below_s = 0, list_n = 0, next_row = 0;
   __syncthreads();
   int below = 0;
   for (int64_t i0 = threadIdx.x; i0 < a.n; i0 += kSortThreads * 8) {
@@ -160,19 +160,27 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortArgs a) {
   __syncthreads();
   if (threadIdx.x == 0 && v1 == (uint64_t)a.v) *a.count = base;
   const bool none = base == base0;  // no id in this range
-  if (threadIdx.x >= kPlacers || none) {
-    // the zeros of rows without an id
+  // the zeros of rows without an id: a warp takes the next four rows
+  auto zeros = [&] {
     if (!a.out) return;
-    const int first = none ? 0 : kPlacers / 32, step = kSortThreads / 32 - first;
     const bool vec = a.d_bytes % 16 == 0 && a.ld_bytes % 16 == 0 && (uintptr_t)a.out % 16 == 0;
-    for (int r = warp - first; r < rows; r += step) {
-      if (present[r >> 5] >> (r & 31) & 1) continue;
-      unsigned char* p = (unsigned char*)a.out + (v0 + r) * a.ld_bytes;
-      if (vec)
-        for (int64_t c = lane * 16; c < a.d_bytes; c += 512) *reinterpret_cast<uint4*>(p + c) = make_uint4(0, 0, 0, 0);
-      else
-        for (int64_t c = lane * 2; c < a.d_bytes; c += 64) *reinterpret_cast<uint16_t*>(p + c) = 0;
+    while (true) {
+      int r0 = 0;
+      if (lane == 0) r0 = atomicAdd(&next_row, 4);
+      r0 = __shfl_sync(~0u, r0, 0);
+      if (r0 >= rows) return;
+      for (int r = r0; r < min(r0 + 4, rows); r++) {
+        if (present[r >> 5] >> (r & 31) & 1) continue;
+        unsigned char* p = (unsigned char*)a.out + (v0 + r) * a.ld_bytes;
+        if (vec)
+          for (int64_t c = lane * 16; c < a.d_bytes; c += 512) *reinterpret_cast<uint4*>(p + c) = make_uint4(0, 0, 0, 0);
+        else
+          for (int64_t c = lane * 2; c < a.d_bytes; c += 64) *reinterpret_cast<uint16_t*>(p + c) = 0;
+      }
     }
+  };
+  if (threadIdx.x >= kPlacers || none) {
+    zeros();
     return;
   }
   // ids of the range, compacted in order of position, then placed
@@ -226,6 +234,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const SortArgs a) {
     }
     group_sync<kPlacers>();
   }
+  zeros();
 }
 
 // ------------------------------------------------------------------- sum
@@ -332,13 +341,14 @@ __global__ void __launch_bounds__(kSumThreads) sum_kernel(const SumArgs a) {
 }
 
 // Rows that cross tiles: the CTAs of the tile where the row starts add its
-// tail and the heads of the tiles after it, in order.  Eight groups of 128
+// tail and the heads of the tiles after it, in order.  Four groups of 64
 // threads take neighbouring stretches of the tiles and are added in their
-// order; a CTA has 128 columns (a few ids make up much of a batch, so one
-// row's chain can be most of the work).
-constexpr int kJoinColumns = 128, kStretches = 8;
-__global__ void __launch_bounds__(kJoinColumns* kStretches) join_kernel(const SumArgs a) {
-  __shared__ float part[kStretches][kJoinColumns];
+// order; a CTA has 256 columns (a few ids make up much of a batch, so one
+// row's chain can be most of the work).  Most CTAs find nothing to join:
+// they are small, so that the GPU is through with them at once.
+constexpr int kJoinThreads = 64, kJoinColumns = 4 * kJoinThreads, kStretches = 4;
+__global__ void __launch_bounds__(kJoinThreads* kStretches) join_kernel(const SumArgs a) {
+  __shared__ float4 part[kStretches][kJoinThreads];
   pdl_release();
   pdl_wait();
   const int n = *a.count;
@@ -352,22 +362,36 @@ __global__ void __launch_bounds__(kJoinColumns* kStretches) join_kernel(const Su
     const int64_t e = e1 + (heads + threadIdx.x) * kEntries;
     more = __syncthreads_count(e < n && a.rows[e] == row);
   }
-  const int group = threadIdx.x / kJoinColumns, lane = threadIdx.x % kJoinColumns;
+  const int group = threadIdx.x / kJoinThreads, lane = threadIdx.x % kJoinThreads;
   const int64_t per = (heads + kStretches - 1) / kStretches, h0 = t + 1 + group * per, h1 = min(t + 1 + heads, h0 + per);
+  const bool vec = a.d % 4 == 0;  // (head and tail start on 16 bytes)
+  auto load = [&](const float* p, int64_t left) {
+    if (vec) return *reinterpret_cast<const float4*>(p);
+    return make_float4(p[0], left > 1 ? p[1] : 0.f, left > 2 ? p[2] : 0.f, left > 3 ? p[3] : 0.f);
+  };
   for (int64_t c0 = blockIdx.y * (int64_t)kJoinColumns; c0 < a.d; c0 += gridDim.y * (int64_t)kJoinColumns) {
-    const int64_t c = c0 + lane;
-    float v = 0.f;
+    const int64_t c = c0 + lane * 4;
+    float4 v = make_float4(0, 0, 0, 0);
     if (c < a.d) {
 #pragma unroll 8
-      for (int64_t h = h0; h < h1; h++) v += a.head[h * a.d + c];
+      for (int64_t h = h0; h < h1; h++) {
+        const float4 x = load(a.head + h * a.d + c, a.d - c);
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
     }
     part[group][lane] = v;
     __syncthreads();
     if (group == 0 && c < a.d) {
-      float s = a.tail[t * a.d + c];
+      float4 s = load(a.tail + t * a.d + c, a.d - c);
 #pragma unroll
-      for (int w = 0; w < kStretches; w++) s += part[w][lane];
-      put(a.out, row * a.ldo + c, a.ot, s * a.scale, a.accumulate);
+      for (int w = 0; w < kStretches; w++) {
+        const float4 x = part[w][lane];
+        s.x += x.x, s.y += x.y, s.z += x.z, s.w += x.w;
+      }
+      const float e[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+      for (int q = 0; q < 4; q++)
+        if (c + q < a.d) put(a.out, row * a.ldo + c + q, a.ot, e[q] * a.scale, a.accumulate);
     }
     __syncthreads();
   }
@@ -446,7 +470,7 @@ void embedding_grad(MType gt, const void* grad, int64_t ldg, const void* ids, bo
   count_launch();
   if (tiles > 1) {
     const unsigned chunks = (unsigned)std::min<int64_t>(8, (d + kJoinColumns - 1) / kJoinColumns);
-    launch_pdl(join_kernel, dim3((unsigned)(tiles - 1), chunks), dim3(kJoinColumns * kStretches), 0, s, b);
+    launch_pdl(join_kernel, dim3((unsigned)(tiles - 1), chunks), dim3(kJoinThreads * kStretches), 0, s, b);
     count_launch();
   }
 }
