@@ -19,6 +19,8 @@
 //                    table, grouped contraction, sharding, ABI exports
 //   blocksparse_kernels.cu  block-sparse <-> dense maps, diagonal placement
 //                    and scaling
+//   model_ops.h      language-model operators on device memory: quantize.cu,
+//                    scaled_gemm.cu, embedding.cu, experts.cu, model_ops.cpp
 //   fp64_peak.cu     FP64 tensor peak microbenchmark (its own library, for
 //                    the bench's roofline)
 #pragma once
