@@ -80,6 +80,7 @@ struct QArgs {
   const void* x;
   int64_t rows, cols, rs, cs;
   QuantOut q, t;
+  uint32_t across;  // CTAs along a row; the grid is one line of them, row after row
 };
 
 // Eight elements of a row from column c (zeros outside the matrix).
@@ -127,7 +128,8 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QArgs a) 
   pdl_wait();
   pdl_release();  // (in this order: the next kernel may read what was ready before this one)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t r0 = ((int64_t)blockIdx.y * (kThreads / 32) + warp) * kRows, c = blockIdx.x * 256ll + lane * 8;
+  const uint32_t by = blockIdx.x / a.across, bx = blockIdx.x - by * a.across;
+  const int64_t r0 = ((int64_t)by * (kThreads / 32) + warp) * kRows, c = bx * 256ll + lane * 8;
   if (r0 >= a.rows) return;
   float v[kRows][8], m[kRows];
 #pragma unroll
@@ -158,7 +160,8 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const QArgs a) 
   __shared__ float quarter[4][kTile];
   pdl_release();
   pdl_wait();
-  const int64_t r0 = (int64_t)blockIdx.y * kTile, c0 = (int64_t)blockIdx.x * kTile;
+  const uint32_t by = blockIdx.x / a.across, bx = blockIdx.x - by * a.across;
+  const int64_t r0 = (int64_t)by * kTile, c0 = (int64_t)bx * kTile;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int sub = lane >> 4, col8 = (lane & 15) * 8;
   float v[8][8], m[8];
@@ -195,8 +198,8 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const QArgs a) 
     for (int i = 0; i < kThreads / 32; i++) most = fmaxf(most, red[i]);
     block = divisor<Q>(most);
     if (threadIdx.x == 0) {
-      if (a.q.q) a.q.s[blockIdx.y * a.q.srs + blockIdx.x * a.q.scs] = block.s;
-      if (a.t.q) a.t.s[blockIdx.x * a.t.srs + blockIdx.y * a.t.scs] = block.s;
+      if (a.q.q) a.q.s[by * a.q.srs + bx * a.q.scs] = block.s;
+      if (a.t.q) a.t.s[bx * a.t.srs + by * a.t.scs] = block.s;
     }
   }
   if (a.q.q) {
@@ -210,7 +213,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const QArgs a) 
       const int64_t r = r0 + warp * 16 + i * 2 + sub;
       const Divisor d = BLOCK ? block : divisor<Q>(m[i]);
       store8<Q>(a, r, c0 + col8, v[i], d);
-      if (!BLOCK && (lane & 15) == 0 && r < a.rows) a.q.s[r * a.q.srs + blockIdx.x * a.q.scs] = d.s;
+      if (!BLOCK && (lane & 15) == 0 && r < a.rows) a.q.s[r * a.q.srs + bx * a.q.scs] = d.s;
     }
   }
   if (!a.t.q) return;
@@ -241,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const QArgs a) 
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       d[k] = divisor<Q>(fmaxf(fmaxf(quarter[0][col + k], quarter[1][col + k]), fmaxf(quarter[2][col + k], quarter[3][col + k])));
-      if (part == 0 && c0 + col + k < a.cols) a.t.s[(c0 + col + k) * a.t.srs + blockIdx.y * a.t.scs] = d[k].s;
+      if (part == 0 && c0 + col + k < a.cols) a.t.s[(c0 + col + k) * a.t.srs + by * a.t.scs] = d[k].s;
     }
   }
   const int nr = (int)min((int64_t)kTile, a.rows - r0);
@@ -266,17 +269,22 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const QArgs a) 
 }
 
 template <typename T, typename Q>
-void launch(const QArgs& a, bool block, cudaStream_t s) {
+void launch(QArgs a, bool block, cudaStream_t s) {
   const bool vec = a.cs == 1 && a.cols % 8 == 0 && a.rs % (16 / sizeof(T)) == 0 && (uintptr_t)a.x % 16 == 0;
-  auto blocks = [](int64_t n, int64_t of) { return (unsigned)((n + of - 1) / of); };
+  auto grid_of = [&](int64_t rows, int64_t cols) {
+    const int64_t across = (a.cols + cols - 1) / cols, all = across * ((a.rows + rows - 1) / rows);
+    if (all > INT32_MAX) throw Error(ErrKind::InvalidArgument, "the matrix has too many blocks for one launch");
+    a.across = (uint32_t)across;
+    return dim3((unsigned)all);
+  };
   if (!block && !a.t.q) {
-    const dim3 grid(blocks(a.cols, 256), blocks(a.rows, kThreads / 32 * kRows));
+    const dim3 grid = grid_of(kThreads / 32 * kRows, 256);
     if (vec)
       launch_pdl(quantize_rows_kernel<T, Q, true>, grid, dim3(kThreads), 0, s, a);
     else
       launch_pdl(quantize_rows_kernel<T, Q, false>, grid, dim3(kThreads), 0, s, a);
   } else {
-    const dim3 grid(blocks(a.cols, kTile), blocks(a.rows, kTile));
+    const dim3 grid = grid_of(kTile, kTile);
     const size_t smem = a.t.q ? (size_t)kTile * (kTile + 16 / sizeof(T)) * sizeof(T) : 0;
     auto go = [&](auto kern) {
       if (smem > 48 * 1024) ensure_dynamic_smem((const void*)kern, smem);
@@ -327,8 +335,7 @@ __global__ void __launch_bounds__(kThreads) pack8_kernel(const uint8_t* __restri
 void quantize(MType xt, const MatView& x, int block_rows, MType q8, const QuantOut& q, const QuantOut& t,
               cudaStream_t s) {
   if (x.rows == 0 || x.cols == 0 || (!q.q && !t.q)) return;
-  if (x.rows > 65535ll * (kThreads / 32 * kRows)) throw Error(ErrKind::InvalidArgument, "more than 65535 * 32 rows");
-  QArgs a{x.p, x.rows, x.cols, x.rs, x.cs, q, t};
+  QArgs a{x.p, x.rows, x.cols, x.rs, x.cs, q, t, 0};
   const bool block = block_rows != 1;
   auto pick = [&](auto qv) {
     using Q = decltype(qv);

@@ -397,6 +397,10 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, Shape<CTAS, BN>::kR
         for (int q = 0; q < kFly; q++) tmem_ld<kLd>(tmem_row + buf * BN + q * kLd, d[q]);
 #pragma unroll
         for (int q = 0; q < kLoads; q++) {
+          float4 b[kLd / 4];  // the columns' scales, on their way before the wait
+          if (BROW)
+#pragma unroll
+            for (int j = 0; j < kLd / 4; j++) b[j] = *reinterpret_cast<const float4*>(sc + 128 + band * kCols + q * kLd + 4 * j);
           if (q % kFly == 0) {
             tmem_ld_wait();
             if (q + kFly >= kLoads) {  // the last column is in registers: the tensor core may have the buffer
@@ -415,8 +419,7 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, Shape<CTAS, BN>::kR
           for (int j = 0; j < kLd; j += 4) {
             uint64_t f0 = s2, f1 = s2;
             if (BROW) {
-              const float4 b = *reinterpret_cast<const float4*>(sc + 128 + band * kCols + q * kLd + j);
-              f0 = mul2(s2, pair(b.x, b.y)), f1 = mul2(s2, pair(b.z, b.w));
+              f0 = mul2(s2, pair(b[j / 4].x, b[j / 4].y)), f1 = mul2(s2, pair(b[j / 4].z, b[j / 4].w));
             }
             uint64_t& a0 = acc[(q * kLd + j) / 2];
             uint64_t& a1 = acc[(q * kLd + j) / 2 + 1];

@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from ._model import REAL, code_of, device_of, launch, unit_rows
 
@@ -70,9 +71,17 @@ class _Embedding(Function):
 
     @staticmethod
     def backward(ctx, grad):
+        # (once_differentiable costs as much as the call; only a graph of the gradient needs it)
+        return _once(ctx, grad) if torch.is_grad_enabled() else _Embedding.grads(ctx, grad)
+
+    @staticmethod
+    def grads(ctx, grad):
         (ids,) = ctx.saved_tensors
         rows, scale, first, dtype = ctx.args
         return embedding_grad(grad, ids, rows, scale, first, out_dtype=dtype), None, None, None
+
+
+_once = once_differentiable(_Embedding.grads)
 
 
 def torch_embedding(table, ids, scale: float = 1.0, first: int = 0):

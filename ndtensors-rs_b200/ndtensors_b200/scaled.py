@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
 from ._model import FLOAT8, REAL, code_of, device_of, launch, rows_of
 
@@ -158,6 +159,11 @@ class _ScaledLinear(Function):
 
     @staticmethod
     def backward(ctx, dy):
+        # (once_differentiable costs as much as the call; only a graph of the gradient needs it)
+        return _once(ctx, dy) if torch.is_grad_enabled() else _ScaledLinear.grads(ctx, dy)
+
+    @staticmethod
+    def grads(ctx, dy):
         x2, kept = ctx.saved_tensors
         device, xt, g8, x_shape, (n, k), w_dtype, x_dtype = ctx.args
         need_x, need_w, _ = ctx.needs_input_grad
@@ -171,6 +177,9 @@ class _ScaledLinear(Function):
                kept.data_ptr() if need_x else None, ld, kept.data_ptr() + k * ld if need_x else None, g8,
                dx.data_ptr() if need_x else None, max(1, k), REAL[w_dtype], dw.data_ptr() if need_w else None, max(1, k))
         return dx if dx is None or len(x_shape) == 2 else dx.view(x_shape), dw, None
+
+
+_once = once_differentiable(_ScaledLinear.grads)
 
 
 def torch_scaled_linear(x, weight, grad_dtype=E4M3):

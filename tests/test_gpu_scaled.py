@@ -94,6 +94,18 @@ def test_quantize_empty(gpu, shape):
     assert q.shape == shape and qt.shape == shape[::-1] and s.shape == (shape[0], -(-shape[1] // 128))
 
 
+def test_quantize_many_rows(gpu):
+    """More rows than a grid's second axis counts, and 64-bit offsets."""
+    rows, cols = 2300000, 1000
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    x[-1] = torch.arange(cols, device="cuda")
+    x[rows // 2, 5] = -3.0
+    q, s = gpu.quantize_blocks(x)
+    rq, rs = quantize(x[-1:], 1, E4)
+    assert same(q[-1:], rq) and torch.equal(s[-1:].double(), rs)
+    assert float(q[rows // 2, 5].float()) == -448 and float(q[: rows // 2].view(torch.uint8).max()) == 0
+
+
 # ---------------------------------------------------------------- products
 
 
@@ -282,6 +294,13 @@ def test_gradients_against_differences(gpu):
         y_err = 2.0 ** -23 * 160 * (x.abs() @ w.abs().T).double() * dy.abs().double()
         far = 2.2 * float((y_err[i] if t == 0 else y_err[:, i]).sum()) / abs(step)
         assert abs(got - want) <= bound + far, (t, i, j, got, want)
+
+
+def test_second_derivatives_are_refused(gpu):
+    x, w = normal(gen(21), 16, 128).requires_grad_(), normal(gen(22), 16, 128).requires_grad_()
+    (dx,) = torch.autograd.grad(gpu.torch_scaled_linear(x, w).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.sum().backward()
 
 
 # --------------------------------------------------------------- refusals
