@@ -1,15 +1,37 @@
 """What the language-model operators share: element types, streams, checks.
 
-A call for a few tokens costs the host more than the GPU, so the wrappers read
-each attribute of a tensor once and leave the messages to the failing path.
+A call for a few tokens costs the host more than the GPU, so the plain cases
+go through ``calls``, a small C++ module (``csrc/torch_calls.cpp``) that
+returns None for any other; the wrappers then check, lay out or refuse.
 """
 
 from __future__ import annotations
+
+import ctypes
+import importlib.machinery
+import importlib.util
+from pathlib import Path
 
 import torch
 
 from ._lib import get_lib, last_error
 from .tensor import NDTensorsError, StatusCode
+
+
+def _load_calls():
+    path = Path(__file__).resolve().parent.parent / "lib" / "ndt_torch_calls.so"
+    if not path.exists():
+        raise FileNotFoundError(f"{path} not found: build it with `make -C ndtensors-rs_b200`")
+    loader = importlib.machinery.ExtensionFileLoader("ndt_torch_calls", str(path))
+    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("ndt_torch_calls", loader))
+    loader.exec_module(module)
+    lib = get_lib()
+    names = ("scaled_linear_dev", "scaled_linear_fwd_dev", "scaled_linear_vjp_dev", "embedding_dev", "embedding_grad_dev", "last_error")
+    module.bind([ctypes.cast(getattr(lib, f"ndt_b200_{n}"), ctypes.c_void_p).value for n in names])
+    return module
+
+
+calls = _load_calls()
 
 #: element type codes of the C ABI
 REAL = {torch.float32: 2, torch.bfloat16: 3, torch.float16: 4}
@@ -73,4 +95,4 @@ def unit_rows(x):
     return x if cs == 1 and rs >= x.shape[1] else x.contiguous()
 
 
-__all__ = ["REAL", "FLOAT8", "launch", "device_of", "code_of", "rows_of", "unit_rows"]
+__all__ = ["calls", "REAL", "FLOAT8", "launch", "device_of", "code_of", "rows_of", "unit_rows"]

@@ -7,7 +7,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._model import REAL, code_of, device_of, launch, unit_rows
+from ._model import REAL, calls, code_of, device_of, launch, unit_rows
 
 _IDS = {torch.int32: 0, torch.int64: 1}
 
@@ -19,6 +19,9 @@ def embedding(table, ids, scale: float = 1.0, first: int = 0):
     slices of a vocabulary (``first``: the slice's first id) add up to the
     whole lookup.
     """
+    out = calls.embedding(table, ids, scale, first)
+    if out is not None:
+        return out
     device = device_of("embedding", table, ids)
     tt, it = code_of("embedding", "table", table.dtype, REAL), code_of("embedding", "ids", ids.dtype, _IDS)
     if table.dim() != 2:
@@ -86,7 +89,8 @@ _once = once_differentiable(_Embedding.grads)
 
 def torch_embedding(table, ids, scale: float = 1.0, first: int = 0):
     """``embedding`` with autograd (a dense gradient of the table's type)."""
-    return _Embedding.apply(table, ids, scale, first)
+    out = calls.torch_embedding(table, ids, scale, first)
+    return _Embedding.apply(table, ids, scale, first) if out is None else out
 
 
 __all__ = ["embedding", "embedding_grad", "torch_embedding"]

@@ -16,7 +16,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._model import FLOAT8, REAL, code_of, device_of, launch, rows_of
+from ._model import FLOAT8, REAL, calls, code_of, device_of, launch, rows_of
 
 E4M3 = torch.float8_e4m3fn
 
@@ -118,6 +118,9 @@ def scaled_linear(x, weight, weight_scales, out_dtype=None):
     in the call (e4m3, a scale for each row and 128 columns).  ``out_dtype``
     defaults to x's type.
     """
+    y = calls.scaled_linear(x, weight, weight_scales, out_dtype)
+    if y is not None:
+        return y
     device = device_of("scaled_linear", x, weight, weight_scales)
     xt = code_of("scaled_linear", "x", x.dtype, REAL)
     wt = code_of("scaled_linear", "weight", weight.dtype, FLOAT8)
@@ -191,6 +194,9 @@ def torch_scaled_linear(x, weight, grad_dtype=E4M3):
     ``grad_dtype`` is the 8-bit type of the output's gradient (e4m3 or e5m2).
     The result has x's type, the gradients their tensors' types.
     """
+    y = calls.torch_scaled_linear(x, weight, grad_dtype)
+    if y is not None:
+        return y
     device_of("torch_scaled_linear", x, weight)
     code_of("torch_scaled_linear", "x", x.dtype, REAL)
     code_of("torch_scaled_linear", "weight", weight.dtype, REAL)

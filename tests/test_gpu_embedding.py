@@ -189,6 +189,24 @@ def test_autograd_against_differences(gpu):
     assert abs(float((g.double() * step.double()).sum()) - want) <= 2.0 ** -21 * size
 
 
+def test_autograd_of_views_and_of_sums(gpu):
+    """A table with gaps (its own path on the host), ids with gaps, and a gradient that is one number broadcast."""
+    base = normal(gen(22), 30, 40)
+    ids = torch.randint(0, 30, (6, 10), generator=gen(23), device="cuda")
+    grads = []
+    for table, at in ((base[:, ::2].contiguous(), ids.T.contiguous()), (base[:, ::2], ids.T)):
+        table = table.detach().requires_grad_()
+        out = gpu.torch_embedding(table, at, scale=2.0)
+        grads.append(torch.autograd.grad(out.sum(), table)[0])
+    assert torch.equal(*grads)
+    count = torch.bincount(ids.reshape(-1), minlength=30).float()
+    assert torch.equal(grads[0], 2 * count[:, None].expand(30, 20))
+    table = base.clone().requires_grad_()
+    (g,) = torch.autograd.grad(gpu.torch_embedding(table, ids).square().sum(), table, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_refusals(gpu):
     table, ids = normal(gen(21), 10, 8), torch.zeros(4, dtype=torch.int64, device="cuda")
     with pytest.raises(TypeError):

@@ -296,6 +296,38 @@ def test_gradients_against_differences(gpu):
         assert abs(got - want) <= bound + far, (t, i, j, got, want)
 
 
+def test_gradients_of_views_and_of_sums(gpu):
+    """Three axes, x with gaps (its own path on the host), and a gradient that is one number broadcast."""
+    base = normal(gen(23), 4, 9, 280)
+    w = normal(gen(24), 72, 140)
+    grads = []
+    for x in (base[..., ::2].contiguous(), base[..., ::2]):
+        x, v = x.detach().requires_grad_(), w.clone().requires_grad_()
+        y = gpu.torch_scaled_linear(x, v)
+        assert y.shape == (4, 9, 72)
+        grads.append((y.detach(),) + torch.autograd.grad(y.sum(), (x, v)))
+    for a, b in zip(*grads):
+        assert torch.equal(a, b)
+    x8, ones = base[..., ::2].reshape(36, 140), torch.ones(36, 72, device="cuda")
+    vx = lambda m, rows: stands_for(*quantize(m, rows, E4), rows)  # noqa: E731
+    check(grads[0][1].view(36, 140), vx(ones, 1), vx(w, 128).T)
+    check(grads[0][2], vx(ones.T, 1), vx(x8.T, 1))
+    with torch.no_grad():
+        assert not gpu.torch_scaled_linear(x, v).requires_grad
+
+
+def test_gradients_on_another_stream(gpu):
+    x, w, dy = normal(gen(25), 64, 256), normal(gen(26), 96, 256), normal(gen(27), 64, 96)
+    pairs = []
+    for stream in (torch.cuda.current_stream(), torch.cuda.Stream()):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            both = [t.clone().requires_grad_() for t in (x, w)]
+            pairs.append(torch.autograd.grad(gpu.torch_scaled_linear(*both), both, dy))
+        torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(*pairs))
+
+
 def test_second_derivatives_are_refused(gpu):
     x, w = normal(gen(21), 16, 128).requires_grad_(), normal(gen(22), 16, 128).requires_grad_()
     (dx,) = torch.autograd.grad(gpu.torch_scaled_linear(x, w).square().sum(), x, create_graph=True)
