@@ -28,8 +28,9 @@
 // each SM are needed for HBM's rate, so stages are small); others of whole
 // 16-byte vectors as 16 bulk copies of 2 KB, rows
 // 2064 bytes apart, which the copy engine takes at 70 - 85 ns each, below the
-// rate of HBM; the rest by plain loads of four warps.  Lanes that copied their
-// own fragments (cp.async) spent 110 instructions on each KB: 3.2 TB/s.
+// rate of HBM.  Rows of any other length come by bulk copies of the 16-byte
+// granules that they touch, and four warps shift them into place.  Lanes that
+// copied their own fragments (cp.async) spent 110 instructions on each KB: 3.2 TB/s.
 //
 // All sums are in 32 bits.  The activations b enter the second product as the
 // sum of two 16-bit numbers (16 or 22 bits of mantissa), so it loses nothing
@@ -49,16 +50,17 @@ namespace cg = cooperative_groups;
 
 constexpr int kConsumers = 16;       // warps that multiply
 constexpr int kMaxWarps = kConsumers + 4;
-enum Copy { kPlain, kBulk, kTensor };  // how rows come: by element, in 16-byte vectors, in 128-byte pieces
+enum Copy { kShift, kBulk, kTensor };  // how rows come: at any byte, in 16-byte vectors, in 128-byte pieces
 __host__ __device__ constexpr int most_bytes(int copy) { return copy == kTensor ? 1024 : 2048; }  // of a row in one stage
 __host__ __device__ constexpr int stage_bytes(int copy) { return copy == kTensor ? 16 * 1024 : 16 * (2048 + 16); }
-__host__ __device__ constexpr int warps_of(int copy) { return kConsumers + (copy == kPlain ? 4 : 1); }
+__host__ __device__ constexpr int warps_of(int copy) { return kConsumers + (copy == kShift ? 4 : 1); }
 constexpr int kMaxSlots = 2048;      // (token, chosen expert) pairs of one launch
 constexpr int kMaxTokens = 256;
 constexpr int kMaxExperts = 1024;
 constexpr int kGroup = 8;            // tokens of one router product
 constexpr int kTeam = 4;             // multiplying warps that take a tile together
 constexpr int kMaxStages = 12;
+constexpr int kRawPitch = 2048 + 32, kRawBytes = 16 * kRawPitch, kMaxRaw = 4;  // (kShift)
 
 struct LayerArgs {
   ExpertArgs e;
@@ -66,6 +68,7 @@ struct LayerArgs {
   int ip;           // i rounded up to 8: the pitch of b's rows
   int unit;         // tokens of an expert that a CTA takes at a time
   int stages;
+  int raw;             // slots for rows at any byte (kShift)
   int row_bytes[2];    // of a row in one stage of each product: even parts of the row
   int xpitch, bpitch;  // bytes of a token's row of x / of b's parts in shared memory
   int op_bytes;     // shared memory for either, and for an expert's scales behind it
@@ -325,7 +328,7 @@ template <typename X, int COPY, bool MAX, int RE>
 __device__ __forceinline__ void router(const LayerArgs& a, float* red) {
   static_assert(RE * kGroup <= 32, "");
   constexpr int kWarps = warps_of(COPY), kThreads = kWarps * 32;
-  constexpr bool VEC = COPY != kPlain;
+  constexpr bool VEC = COPY != kShift;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int groups = (a.tokens + kGroup - 1) / kGroup, es = (a.experts + RE - 1) / RE;
   for (int u = blockIdx.x; u < es * groups; u += gridDim.x) {
@@ -384,7 +387,7 @@ __device__ __forceinline__ void router(const LayerArgs& a, float* red) {
 // NT: column tiles of 8 tokens that a product takes at a time.
 template <typename W, typename X, typename M, int COPY, int NT>
 struct Layer {
-  static constexpr bool VEC = COPY != kPlain;
+  static constexpr bool VEC = COPY != kShift;
   static constexpr int kWarps = warps_of(COPY), kThreads = kWarps * 32;
   static constexpr bool kScaled = sizeof(W) == 1;
   static constexpr bool kHalf = std::is_same_v<M, __half>;
@@ -420,6 +423,7 @@ struct Layer {
         mbar_init(full + 8 * st, VEC ? 1 : kWarps - kConsumers);
         mbar_init(empty + 8 * st, kConsumers);
       }
+      for (int st = 0; st < kMaxRaw; st++) mbar_init(empty + 8 * kMaxStages + 8 * st, 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (a.tokens <= 8)
@@ -442,7 +446,9 @@ struct Layer {
     const int first1 = share(L.units * tiles1, blockIdx.x), end1 = share(L.units * tiles1, blockIdx.x + 1);
 
     if (warp >= kConsumers) {
-      if (!VEC || warp == kConsumers) {
+      if (COPY == kShift) {
+        shift_tiles(a, L, first0, end0, tiles0, first1, end1, tiles1, ring, full, empty, gave_up);
+      } else {
         int stage = 0;
         uint32_t phase = 0;
         copy_tiles<0>(a, maps, L, first0, end0, tiles0, ring, full, empty, stage, phase, gave_up);
@@ -603,7 +609,7 @@ struct Layer {
   __device__ static __forceinline__ void copy_tiles(const LayerArgs& a, const CUtensorMap* map, const Lists& L, int first, int end, int tiles,
                                                     unsigned char* ring, uint32_t full, uint32_t empty, int& stage,
                                                     uint32_t& phase, volatile int* gave_up) {
-    const int lane = threadIdx.x & 31, copier = (threadIdx.x >> 5) - kConsumers;
+    const int lane = threadIdx.x & 31;
     const int k = PRODUCT == 0 ? a.h : a.i;
     const int64_t rows = PRODUCT == 0 ? 2 * (int64_t)a.i : a.h;
     const W* w = (const W*)(PRODUCT == 0 ? a.e.w_in : a.e.w_out);
@@ -626,23 +632,121 @@ struct Layer {
             tensor_copy(smem_u32(dst) + 8 * 1024, map, bar, (int)(expert * rows) + (PRODUCT == 0 ? a.i + tile * 8 : tile * 16 + 8), piece);
           }
           __syncwarp();
-        } else if constexpr (COPY == kBulk) {
+        } else {
           const int bytes = min(row_bytes, (k - k0) * (int)sizeof(W));
           if (lane == 0) mbar_expect_tx(full + 8 * stage, 16 * bytes);
           __syncwarp();
           if (lane < 16) bulk_copy(smem_u32(dst + lane * kRowPitch), w + (expert * rows + row_of(tile, lane)) * k + k0, bytes, full + 8 * stage);
-        } else {
-          const int m = min(row_k, k - k0);
-          for (int r = copier; r < 16; r += kWarps - kConsumers) {
-            const W* src = w + (expert * rows + row_of(tile, r)) * k + k0;
-            for (int c = lane * 16 / (int)sizeof(W); c < m; c += 512 / (int)sizeof(W))
-              *reinterpret_cast<uint4*>(dst + r * kRowPitch + c * sizeof(W)) = row16<W, false>(src, c, m, true);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full + 8 * stage);
         }
         if (++stage == a.stages) stage = 0, phase ^= 1;
       }
+    }
+  }
+
+  // The same for rows that start at any byte: the 16-byte granules that a row
+  // touches come by a bulk copy into a slot, and the copying warps shift the
+  // bytes into a stage.  (Granules that reach past the weights' first or last
+  // byte are not copied; what they hold of a row is read byte by byte.)
+  __device__ static __forceinline__ void shift_tiles(const LayerArgs& a, const Lists& L, int first0, int end0, int tiles0, int first1,
+                                                     int end1, int tiles1, unsigned char* ring, uint32_t full, uint32_t empty,
+                                                     volatile int* gave_up) {
+    const int lane = threadIdx.x & 31, copier = (threadIdx.x >> 5) - kConsumers;
+    constexpr int kCopiers = kWarps - kConsumers;
+    unsigned char* raw = ring + a.stages * kStageBytes;
+    const uint32_t arrived = empty + 8 * kMaxStages;  // a slot's copies
+    struct At {
+      int product, task, byte;
+    };
+    auto settle = [&](At& p) {
+      if (p.product == 0 && p.task >= end0) p.product = 1, p.task = first1;
+      if (p.product == 1 && p.task >= end1) p.product = 2;
+    };
+    auto next = [&](At& p) {
+      p.byte += a.row_bytes[p.product];
+      if (p.byte < (p.product == 0 ? a.h : a.i) * (int)sizeof(W)) return;
+      p.byte = 0, p.task++;
+      settle(p);
+    };
+    struct Row {
+      uintptr_t at, lo, hi;  // the row's first byte; the granules that are copied
+      int bytes;
+    };
+    auto row_of = [&](const At& p, int r) {
+      const bool p0 = p.product == 0;
+      const int tiles = p0 ? tiles0 : tiles1, u = p.task / tiles, tile = p.task - u * tiles;
+      const int row = p0 ? min(tile * 8 + (r & 7), a.i - 1) + (r >= 8 ? a.i : 0) : min(tile * 16 + r, a.h - 1);
+      const int64_t rows = p0 ? 2 * (int64_t)a.i : a.h, length = (int64_t)(p0 ? a.h : a.i) * sizeof(W);
+      const uintptr_t w = (uintptr_t)(p0 ? a.e.w_in : a.e.w_out), end = w + a.experts * rows * length;
+      Row x;
+      x.at = w + (L.unit_expert[u] * rows + row) * length + p.byte;
+      x.bytes = (int)min((int64_t)a.row_bytes[p.product], length - p.byte);
+      x.lo = max(x.at & ~(uintptr_t)15, (w + 15) & ~(uintptr_t)15);
+      x.hi = max(x.lo, min((x.at + x.bytes + 15) & ~(uintptr_t)15, end & ~(uintptr_t)15));
+      return x;
+    };
+    auto issue = [&](const At& p, int slot) {  // one warp
+      const Row x = row_of(p, lane & 15);
+      const int bytes = lane < 16 ? (int)(x.hi - x.lo) : 0;
+      const int all = __reduce_add_sync(~0u, bytes);
+      if (lane == 0) mbar_expect_tx(arrived + 8 * slot, all);
+      __syncwarp();
+      if (bytes)
+        bulk_copy(smem_u32(raw + slot * kRawBytes + lane * kRawPitch) + (uint32_t)(x.lo - (x.at & ~(uintptr_t)15)), (const void*)x.lo, bytes,
+                  arrived + 8 * slot);
+    };
+    At p{0, first0, 0};
+    settle(p);
+    At ahead = p;
+    if (copier == 0)
+      for (int i = 0; i < a.raw && ahead.product < 2; i++) {
+        issue(ahead, i);
+        next(ahead);
+      }
+    int stage = 0, slot = 0;
+    uint32_t phase = 0, turn = 0;
+    for (; p.product < 2; next(p)) {
+      mbar_wait(arrived + 8 * slot, turn, gave_up, a.flag);
+      mbar_wait(empty + 8 * stage, phase ^ 1, gave_up, a.flag);
+      __syncwarp();
+      for (int r = copier; r < 16; r += kCopiers) {
+        const Row x = row_of(p, r);
+        const unsigned char* from = raw + slot * kRawBytes + r * kRawPitch;
+        const uintptr_t base = x.at & ~(uintptr_t)15;
+        const int skew = (int)(x.at - base), lo = (int)(x.lo - base), hi = (int)(x.hi - base);
+        for (int c = lane * 16; c < x.bytes; c += 512) {
+          const int n = min(16, x.bytes - c), at = skew + c;
+          uint32_t v[4];
+          if (at >= lo && at + n <= hi) {  // five words of the slot hold the 16 bytes
+            const uint32_t* q = reinterpret_cast<const uint32_t*>(from) + (at >> 2);
+            const uint32_t shift = (at & 3) * 8;
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __funnelshift_r(q[j], q[j + 1], shift);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const int keep = n - 4 * j;  // zeros past the row's end
+              v[j] = keep >= 4 ? v[j] : keep <= 0 ? 0 : v[j] & ((1u << 8 * keep) - 1);
+            }
+          } else {
+            const unsigned char* g = reinterpret_cast<const unsigned char*>(x.at) + c;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              v[j] = 0;
+              for (int b = 0; b < 4; b++)
+                if (4 * j + b < n) v[j] |= (uint32_t)g[4 * j + b] << 8 * b;
+            }
+          }
+          *reinterpret_cast<uint4*>(ring + stage * kStageBytes + r * kRowPitch + c) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full + 8 * stage);
+      if (++stage == a.stages) stage = 0, phase ^= 1;
+      asm volatile("bar.sync 15, %0;" ::"n"(kCopiers * 32) : "memory");  // the slot has been read
+      if (copier == 0 && ahead.product < 2) {
+        issue(ahead, slot);
+        next(ahead);
+      }
+      if (++slot == a.raw) slot = 0, turn ^= 1;
     }
   }
 
@@ -819,7 +923,7 @@ __global__ void __launch_bounds__(warps_of(COPY) * 32, 1)
     layer_kernel(const __grid_constant__ LayerArgs a, const __grid_constant__ Maps maps) {
   __shared__ Lists lists;
   __shared__ int scratch[kMaxExperts];
-  __shared__ __align__(8) uint64_t bars[2 * kMaxStages];
+  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + kMaxRaw];
   __shared__ int gave_up;
   extern __shared__ __align__(16) unsigned char dyn[];
   Layer<W, X, M, COPY, NT>::run(a, maps.m, lists, scratch, bars, &gave_up, dyn);
@@ -840,8 +944,8 @@ template <typename W, typename X, typename M, int COPY, int NT>
 void launch(LayerArgs& a, int64_t row, cudaStream_t s) {
   auto kern = layer_kernel<W, X, M, COPY, NT>;
   // as many tokens as fit beside kKeep of stages (at least one, beside two stages), and stages for the rest
-  const int space = room(NT), kStageBytes = stage_bytes(COPY), kKeep = 100 * 1024;
-  if (row > space - 8192 - 2 * kStageBytes) throw Error(ErrKind::InvalidArgument, "h or i is too large for a token's row to fit shared memory");
+  const int space = room(NT), kStageBytes = stage_bytes(COPY), kKeep = (COPY == kShift ? 132 : 100) * 1024;
+  if (row > space - 8192 - 2 * kStageBytes - (COPY == kShift ? kRawBytes : 0)) throw Error(ErrKind::InvalidArgument, "h or i is too large for a token's row to fit shared memory");
   a.unit = (int)std::max<int64_t>(1, std::min<int64_t>({NT * 8, a.tokens, (space - kKeep - (sizeof(W) == 1 ? 8192 : 0)) / row}));
   a.op_bytes = (int)(a.unit * row);
   for (int p = 0; p < 2; p++) {
@@ -854,8 +958,9 @@ void launch(LayerArgs& a, int64_t row, cudaStream_t s) {
     const int64_t bytes = std::max(hb * jb, hb * ib) * 4;
     if (bytes <= 8192) a.scale_at = a.op_bytes, a.op_bytes += (int)((bytes + 15) / 16 * 16);
   }
-  a.stages = std::min(kMaxStages, (space - a.op_bytes) / kStageBytes);
-  const size_t smem = (size_t)a.op_bytes + red_bytes(NT) + 1024 + (size_t)a.stages * kStageBytes;
+  a.stages = COPY == kShift ? 2 : std::min(kMaxStages, (space - a.op_bytes) / kStageBytes);
+  a.raw = COPY == kShift ? std::min(kMaxRaw, (space - a.op_bytes - 2 * kStageBytes) / kRawBytes) : 0;
+  const size_t smem = (size_t)a.op_bytes + red_bytes(NT) + 1024 + (size_t)a.stages * kStageBytes + (size_t)a.raw * kRawBytes;
   ensure_dynamic_smem((const void*)kern, smem);
   Maps maps{};
   if (COPY == kTensor) {
@@ -903,13 +1008,13 @@ void expert_layer(const ExpertArgs& e, cudaStream_t s) {
     const int64_t row = std::max((int64_t)a.xpitch, 2 * (int64_t)a.bpitch);
     // An expert's second unit of tokens reads its weights again (from L2): more
     // columns where an expert gets more than 6 tokens on average and 16 fit.
-    const bool many = a.tokens * e.top > 6 * e.experts && a.tokens > 8 && 16 * row <= room(2) - 108 * 1024;
+    const bool many = a.tokens * e.top > 6 * e.experts && a.tokens > 8 && 16 * row <= room(2) - 140 * 1024;
     auto go = [&](auto w, auto x, auto m) {
       using W = decltype(w);
       using X = decltype(x);
       using M = decltype(m);
       if (!vec)
-        many ? launch<W, X, M, kPlain, 2>(a, row, s) : launch<W, X, M, kPlain, 1>(a, row, s);
+        many ? launch<W, X, M, kShift, 2>(a, row, s) : launch<W, X, M, kShift, 1>(a, row, s);
       else if (!pieces)
         many ? launch<W, X, M, kBulk, 2>(a, row, s) : launch<W, X, M, kBulk, 1>(a, row, s);
       else
