@@ -713,18 +713,31 @@ struct Layer {
         const unsigned char* from = raw + slot * kRawBytes + r * kRawPitch;
         const uintptr_t base = x.at & ~(uintptr_t)15;
         const int skew = (int)(x.at - base), lo = (int)(x.lo - base), hi = (int)(x.hi - base);
-        for (int c = lane * 16; c < x.bytes; c += 512) {
-          const int n = min(16, x.bytes - c), at = skew + c;
+        unsigned char* to = ring + stage * kStageBytes + r * kRowPitch;
+        constexpr int kFly = most_bytes(COPY) / 512;  // a lane's 16-byte pieces of the row: all at once
+        uint32_t q[kFly][5];
+        const uint32_t shift = (skew & 3) * 8;
+#pragma unroll
+        for (int f = 0; f < kFly; f++) {  // five words of the slot hold 16 bytes (the slot has room behind the row)
+          const uint32_t* words = reinterpret_cast<const uint32_t*>(from) + (skew >> 2) + lane * 4 + f * 128;
+          if (lane * 16 + f * 512 < x.bytes)
+#pragma unroll
+            for (int j = 0; j < 5; j++) q[f][j] = words[j];
+        }
+#pragma unroll
+        for (int f = 0; f < kFly; f++) {
+          const int c = lane * 16 + f * 512, n = min(16, x.bytes - c), at = skew + c;
+          if (n <= 0) break;
           uint32_t v[4];
-          if (at >= lo && at + n <= hi) {  // five words of the slot hold the 16 bytes
-            const uint32_t* q = reinterpret_cast<const uint32_t*>(from) + (at >> 2);
-            const uint32_t shift = (at & 3) * 8;
+          if (at >= lo && at + n <= hi) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = __funnelshift_r(q[j], q[j + 1], shift);
+            for (int j = 0; j < 4; j++) v[j] = __funnelshift_r(q[f][j], q[f][j + 1], shift);
+            if (n < 16) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const int keep = n - 4 * j;  // zeros past the row's end
-              v[j] = keep >= 4 ? v[j] : keep <= 0 ? 0 : v[j] & ((1u << 8 * keep) - 1);
+              for (int j = 0; j < 4; j++) {
+                const int keep = n - 4 * j;  // zeros past the row's end
+                v[j] = keep >= 4 ? v[j] : keep <= 0 ? 0 : v[j] & ((1u << 8 * keep) - 1);
+              }
             }
           } else {
             const unsigned char* g = reinterpret_cast<const unsigned char*>(x.at) + c;
@@ -735,7 +748,7 @@ struct Layer {
                 if (4 * j + b < n) v[j] |= (uint32_t)g[4 * j + b] << 8 * b;
             }
           }
-          *reinterpret_cast<uint4*>(ring + stage * kStageBytes + r * kRowPitch + c) = make_uint4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<uint4*>(to + c) = make_uint4(v[0], v[1], v[2], v[3]);
         }
       }
       __syncwarp();
