@@ -21,6 +21,7 @@
 //                    and scaling
 //   model_ops.h      language-model operators on device memory: quantize.cu,
 //                    scaled_gemm.cu, embedding.cu, experts.cu, model_ops.cpp
+//   torch_calls.cpp  their plain calls from torch (its own library)
 //   fp64_peak.cu     FP64 tensor peak microbenchmark (its own library, for
 //                    the bench's roofline)
 #pragma once
