@@ -21,6 +21,13 @@
 // lanes and A's few the columns.  CTAS = 2: a CTA pair computes 256 x 256 with
 // cta_group::2 MMAs, each CTA staging its half of both operands; persistent.
 //
+// Measured on one B200 (1 x 128 by 128 x 128 scales, bf16 result): 4096^3 86 us
+// = 1600 TFLOP/s, 8192^3 537 us = 2050; with a scale for each row of both
+// 4096^3 125 us.  The tensor pipe is busy 45 % of the time.  With a quarter of
+// the MMAs 8192^3 still takes 463 us, with half the TMEM reads too 434: the
+// bound is the operand tiles' way from L2 to the SMs, 32 KB for each SM and
+// block of k (9.8 TB/s).  One row against 10240 x 8192 weights: 19 us, 4.5 TB/s.
+//
 // sa * sb is formed in 32 bits: it stays finite while the product of two
 // blocks' largest values is below 2^127.
 #include <algorithm>
@@ -566,7 +573,9 @@ void launch(const ScaledOperand& a, const ScaledOperand& b, int64_t k, GemmArgs 
 
 void scaled_gemm(const ScaledOperand& a_, const ScaledOperand& b_, int64_t k, MType ct, void* c, int64_t ldc,
                  bool accumulate, cudaStream_t s, bool b_early) {
-  // Up to 64 rows of A: B's rows on the 128 lanes, A's as 16 to 64 columns.
+  // Up to 64 rows of A: B's rows on the 128 lanes, A's as 16 to 64 columns
+  // (8192 x 8192 weights, 17 / 33 / 64 rows: 19.1 / 23.9 / 25.5 us, against
+  // 24.9 / 26.3 / 30.1 as they are).
   const bool swap = a_.rows <= 64;
   const ScaledOperand &a = swap ? b_ : a_, &b = swap ? a_ : b_;
   GemmArgs g{};
@@ -588,11 +597,15 @@ void scaled_gemm(const ScaledOperand& a_, const ScaledOperand& b_, int64_t k, MT
     return 1u << 4 | (a.type == MType::E5M2 ? 1u : 0u) << 7 | (b.type == MType::E5M2 ? 1u : 0u) << 10 |
            (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
   };
-  const int pair_tiles = cdiv(g.m, 256) * cdiv(g.n, 256);
-  if (!swap && pair_tiles * 2 >= sms / 2) {
+  // Waves of 128 x 128 tiles against waves of 256 x 256 pairs, which take 5 / 4
+  // of the time (k 2048: 1024 x 2048 15.2 us in one wave of tiles, 16.9 of
+  // pairs; 1024 x 2560 25.1 in two of tiles, 17.7 in one of pairs).
+  const int64_t pair_tiles = (int64_t)cdiv(g.m, 256) * cdiv(g.n, 256);
+  const int64_t waves = ((int64_t)cdiv(g.m, 128) * cdiv(g.n, 128) + sms - 1) / sms, pair_waves = (pair_tiles + sms / 2 - 1) / (sms / 2);
+  if (!swap && 5 * pair_waves < 4 * waves) {
     g.tiles_m = cdiv(g.m, 256), g.tiles_n = cdiv(g.n, 256);
     g.idesc = idesc(256, 256);
-    const int grid = 2 * std::min(pair_tiles, sms / 2);
+    const int grid = 2 * (int)std::min<int64_t>(pair_tiles, sms / 2);
     if (b.per_row)
       launch<2, 256, true>(a, b, k, g, grid, 2, s);
     else
