@@ -84,28 +84,47 @@ struct QArgs {
   uint32_t across;  // CTAs along a row; the grid is one line of them, row after row
 };
 
+// How x lies: columns apart; columns together, rows starting anywhere (read in
+// aligned words); whole aligned vectors of 8 columns.
+enum Lie { kApart, kTogether, kVectors };
+
 // Eight elements of a row from column c (zeros outside the matrix).
-template <typename T, bool VEC>
+template <typename T, int LIE>
 __device__ __forceinline__ void load8(const QArgs& a, int64_t r, int64_t c, float* v) {
   const T* p = (const T*)a.x + r * a.rs;
-  if (VEC) {  // cols is a multiple of 8 here
-    if (r < a.rows && c < a.cols) {
-      if constexpr (sizeof(T) == 4) {
-        const float4 w0 = *reinterpret_cast<const float4*>(p + c), w1 = *reinterpret_cast<const float4*>(p + c + 4);
+  if (LIE != kApart && r < a.rows && c + 8 <= a.cols) {
+    p += c;
+    if constexpr (sizeof(T) == 4) {
+      if (LIE == kVectors || ((uintptr_t)p & 15) == 0) {
+        const float4 w0 = *reinterpret_cast<const float4*>(p), w1 = *reinterpret_cast<const float4*>(p + 4);
         v[0] = w0.x, v[1] = w0.y, v[2] = w0.z, v[3] = w0.w, v[4] = w1.x, v[5] = w1.y, v[6] = w1.z, v[7] = w1.w;
       } else {
-        const uint4 w = *reinterpret_cast<const uint4*>(p + c);
-        const T* e = reinterpret_cast<const T*>(&w);
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = to_f32<T>(e[j]);
+        for (int j = 0; j < 8; j++) v[j] = p[j];
       }
     } else {
+      uint32_t w[4];
+      if (LIE == kVectors) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+      } else {  // four aligned words hold the elements, or five where the row starts in the middle of one
+        const uint32_t* q = reinterpret_cast<const uint32_t*>((uintptr_t)p & ~(uintptr_t)3);
+        const bool odd = (uintptr_t)p & 2;
+        uint32_t x[5];
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = 0.f;
+        for (int j = 0; j < 4; j++) x[j] = q[j];
+        x[4] = odd ? q[4] : 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = odd ? __funnelshift_r(x[j], x[j + 1], 16) : x[j];
+      }
+      const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = to_f32<T>(e[j]);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = r < a.rows && c + j < a.cols ? to_f32<T>(p[(c + j) * a.cs]) : 0.f;
+    for (int j = 0; j < 8; j++)
+      v[j] = LIE != kVectors && r < a.rows && c + j < a.cols ? to_f32<T>(p[(c + j) * (LIE == kApart ? a.cs : 1)]) : 0.f;
   }
 }
 __device__ __forceinline__ float max8(const float* v) {
@@ -124,7 +143,7 @@ __device__ __forceinline__ void store8(const QArgs& a, int64_t r, int64_t c, con
 // Blocks of 1 x 128, x as it lies: half a warp takes a block, a thread 8
 // columns of kRows rows.  Bound by HBM: 16-bit in, 8-bit out.
 constexpr int kRows = 4;
-template <typename T, typename Q, bool VEC>
+template <typename T, typename Q, int LIE>
 __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QArgs a) {
   pdl_wait();
   pdl_release();  // (in this order: the next kernel may read what was ready before this one)
@@ -134,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QArgs a) 
   if (r0 >= a.rows) return;
   float v[kRows][8], m[kRows];
 #pragma unroll
-  for (int i = 0; i < kRows; i++) load8<T, VEC>(a, r0 + i, c, v[i]);
+  for (int i = 0; i < kRows; i++) load8<T, LIE>(a, r0 + i, c, v[i]);
 #pragma unroll
   for (int i = 0; i < kRows; i++) m[i] = max8(v[i]);
 #pragma unroll
@@ -152,7 +171,7 @@ __global__ void __launch_bounds__(kThreads) quantize_rows_kernel(const QArgs a) 
 // One 128 x 128 tile a CTA: blocks of 128 x 128, or the transpose too.  The
 // tile lies in shared memory, so x is read once for both outputs; there a
 // thread takes two columns of a quarter of the rows.
-template <typename T, typename Q, bool BLOCK, bool VEC>
+template <typename T, typename Q, bool BLOCK, int LIE>
 __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const QArgs a) {
   extern __shared__ __align__(16) unsigned char dyn[];
   constexpr int kPitch = kTile + 16 / (int)sizeof(T);
@@ -167,7 +186,7 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const QArgs a) 
   const int sub = lane >> 4, col8 = (lane & 15) * 8;
   float v[8][8], m[8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) load8<T, VEC>(a, r0 + warp * 16 + i * 2 + sub, c0 + col8, v[i]);
+  for (int i = 0; i < 8; i++) load8<T, LIE>(a, r0 + warp * 16 + i * 2 + sub, c0 + col8, v[i]);
 #pragma unroll
   for (int i = 0; i < 8; i++) m[i] = max8(v[i]);
   if (a.t.q) {
@@ -271,7 +290,8 @@ __global__ void __launch_bounds__(kThreads) quantize_tile_kernel(const QArgs a) 
 
 template <typename T, typename Q>
 void launch(QArgs a, bool block, cudaStream_t s) {
-  const bool vec = a.cs == 1 && a.cols % 8 == 0 && a.rs % (16 / sizeof(T)) == 0 && (uintptr_t)a.x % 16 == 0;
+  const Lie lie = a.cs != 1 ? kApart
+                  : a.cols % 8 == 0 && a.rs % (16 / sizeof(T)) == 0 && (uintptr_t)a.x % 16 == 0 ? kVectors : kTogether;
   auto grid_of = [&](int64_t rows, int64_t cols) {
     const int64_t across = (a.cols + cols - 1) / cols, all = across * ((a.rows + rows - 1) / rows);
     if (all > INT32_MAX) throw Error(ErrKind::InvalidArgument, "the matrix has too many blocks for one launch");
@@ -280,10 +300,9 @@ void launch(QArgs a, bool block, cudaStream_t s) {
   };
   if (!block && !a.t.q) {
     const dim3 grid = grid_of(kThreads / 32 * kRows, 256);
-    if (vec)
-      launch_pdl(quantize_rows_kernel<T, Q, true>, grid, dim3(kThreads), 0, s, a);
-    else
-      launch_pdl(quantize_rows_kernel<T, Q, false>, grid, dim3(kThreads), 0, s, a);
+    auto go = [&](auto kern) { launch_pdl(kern, grid, dim3(kThreads), 0, s, a); };
+    lie == kVectors ? go(quantize_rows_kernel<T, Q, kVectors>)
+    : lie == kTogether ? go(quantize_rows_kernel<T, Q, kTogether>) : go(quantize_rows_kernel<T, Q, kApart>);
   } else {
     const dim3 grid = grid_of(kTile, kTile);
     const size_t smem = a.t.q ? (size_t)kTile * (kTile + 16 / sizeof(T)) * sizeof(T) : 0;
@@ -292,9 +311,11 @@ void launch(QArgs a, bool block, cudaStream_t s) {
       launch_pdl(kern, grid, dim3(kThreads), smem, s, a);
     };
     if (block)
-      vec ? go(quantize_tile_kernel<T, Q, true, true>) : go(quantize_tile_kernel<T, Q, true, false>);
+      lie == kVectors ? go(quantize_tile_kernel<T, Q, true, kVectors>)
+      : lie == kTogether ? go(quantize_tile_kernel<T, Q, true, kTogether>) : go(quantize_tile_kernel<T, Q, true, kApart>);
     else
-      vec ? go(quantize_tile_kernel<T, Q, false, true>) : go(quantize_tile_kernel<T, Q, false, false>);
+      lie == kVectors ? go(quantize_tile_kernel<T, Q, false, kVectors>)
+      : lie == kTogether ? go(quantize_tile_kernel<T, Q, false, kTogether>) : go(quantize_tile_kernel<T, Q, false, kApart>);
   }
   count_launch();
 }

@@ -204,6 +204,7 @@ __device__ __forceinline__ void tile_at(int t, int tiles_m, int tiles_n, int& tm
 
 template <int CTAS, int BN>
 struct Shape {
+  static constexpr int kEpiWarps = 8;  // (16, with half the registers each, wait in each other's way: 86 -> 107 us for 4096^3)
   static constexpr int kBM = 128;                    // rows of one CTA
   static constexpr int kBRows = BN / CTAS;           // rows of B that one CTA stages
   static constexpr int kABytes = kBM * kBK, kBBytes = kBRows * kBK;
@@ -213,10 +214,13 @@ struct Shape {
   static constexpr int kStages = (kResident == 2 ? 100 : 192) * 1024 / kStage;
   static constexpr int kScaleFloats = kBM + (BN + 31) / 32 * 32;  // a slot of the scale ring
   static constexpr int kTmemCols = 2 * BN;
-  static constexpr int kEpiWarps = 8;  // (16, with half the registers each, wait in each other's way: 86 -> 107 us for 4096^3)
   static constexpr int kCols = BN / (kEpiWarps / 4);  // columns of one epilogue thread
   static constexpr int kThreads = 32 * (kEpiWarp0 + kEpiWarps);
-  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + (size_t)kSlots * kScaleFloats * 4;
+  // rows of C that vectors do not fit go through 32 x 16 values a warp, so that
+  // its stores are runs of a row (wide tiles; narrow ones lie along C's columns).
+  // 7080 x 2703 x 512, bf16 result, x quantised in the call: 211 -> 60 us.
+  static constexpr int kTurn = BN >= 128 ? 32 * 17 : 0;
+  static constexpr size_t kSmem = 1024 + (size_t)kStages * kStage + ((size_t)kSlots * kScaleFloats + kEpiWarps * kTurn) * 4;
   static_assert(kTmemCols >= 32 && kTmemCols <= 512 && (kTmemCols & (kTmemCols - 1)) == 0, "TMEM columns");
   static_assert((size_t)BN * 129 * 4 <= (size_t)kStages * kStage || CTAS == 2, "the split's buffer reuses the stages");
   static_assert(kStage % 1024 == 0, "swizzled tiles start on 1024 bytes");
@@ -446,6 +450,25 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, Shape<CTAS, BN>::kR
         float* part = reinterpret_cast<float*>(raw + (stage0 - smem_u32(raw)));
 #pragma unroll
         for (int j = 0; j < kCols; j++) part[(band * kCols + j) * 129 + row] = at(j);
+      } else if (S::kTurn && (!g.vec || g.accumulate || col_c + kCols > g.n) && g.ccs == 1) {
+        float* turn = scale_ring + kSlots * S::kScaleFloats + (warp - kEpiWarp0) * S::kTurn;
+        const int first = tm * 128 * CTAS + rank * 128 + quad * 32;
+#pragma unroll
+        for (int q = 0; q < kCols / 16; q++) {
+#pragma unroll
+          for (int j = 0; j < 16; j++) turn[lane * 17 + j] = at(q * 16 + j);
+          __syncwarp();
+          const int col = col_c + q * 16 + (lane & 15);
+#pragma unroll 4
+          for (int r = lane >> 4; r < 32; r += 2) {
+            if (first + r >= g.m || col >= g.n) continue;
+            const int64_t i = (int64_t)(first + r) * g.crs + col;
+            float v = turn[r * 17 + (lane & 15)];
+            if (g.accumulate) v += load_c(g.c, i, g.ctype);
+            store_c(g.c, i, g.ctype, v);
+          }
+          __syncwarp();
+        }
       } else if (row_c < g.m) {
         const int64_t base = row_c * g.crs + col_c * g.ccs;
         const int cols = min(kCols, g.n - col_c);
