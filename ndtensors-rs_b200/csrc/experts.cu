@@ -27,9 +27,9 @@
 // bytes, swizzled so that ldmatrix meets no bank conflict; 90 KB in flight on
 // each SM are needed for HBM's rate, so stages are small); others of whole
 // 16-byte vectors as 16 bulk copies of 2 KB, rows 2064 bytes apart, which the
-// copy engine takes at 70 - 85 ns each, below the rate of HBM.  Rows of any other length come by bulk copies of the 16-byte
-// granules that they touch, and four warps shift them into place.  Lanes that
-// copied their own fragments (cp.async) spent 110 instructions on each KB: 3.2 TB/s.
+// copy engine takes at 70 - 85 ns each, below the rate of HBM.  Rows of any
+// other length come by bulk copies of the 16-byte granules that they touch, and
+// seven warps shift them into place: 1.1 - 1.5 TB/s.  Lanes that copied their own fragments (cp.async) spent 110 instructions on each KB: 3.2 TB/s.
 //
 // Measured on one B200: 1 token, 8 of 64 experts, h 2048, i 1024, bf16 39 us
 // (router 1.4, choice 5, products 10 and 6, barriers 6, the rest the launch); 8
@@ -54,11 +54,15 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kConsumers = 16;       // warps that multiply
-constexpr int kMaxWarps = kConsumers + 4;
+// (kShift) Warps that shift rows into place; one more issues their copies.  The
+// shifts bound such layers: 64 tokens, 4 of 64, h 2049, i 641, bf16 takes 405 us
+// with 7 and 496 with 4, which leave no more registers to a thread (80).
+constexpr int kShifters = 7;
+constexpr int kMaxWarps = kConsumers + kShifters + 1;
 enum Copy { kShift, kBulk, kTensor };  // how rows come: at any byte, in 16-byte vectors, in 128-byte pieces
 __host__ __device__ constexpr int most_bytes(int copy) { return copy == kTensor ? 1024 : 2048; }  // of a row in one stage
 __host__ __device__ constexpr int stage_bytes(int copy) { return copy == kTensor ? 16 * 1024 : 16 * (2048 + 16); }
-__host__ __device__ constexpr int warps_of(int copy) { return kConsumers + (copy == kShift ? 4 : 1); }
+__host__ __device__ constexpr int warps_of(int copy) { return kConsumers + (copy == kShift ? kShifters + 1 : 1); }
 constexpr int kMaxSlots = 2048;      // (token, chosen expert) pairs of one launch
 constexpr int kMaxTokens = 256;
 constexpr int kMaxExperts = 1024;
@@ -425,10 +429,13 @@ struct Layer {
     if (threadIdx.x == 0) {
       *gave_up = 0;
       for (int st = 0; st < a.stages; st++) {
-        mbar_init(full + 8 * st, VEC ? 1 : kWarps - kConsumers);
+        mbar_init(full + 8 * st, VEC ? 1 : kShifters);
         mbar_init(empty + 8 * st, kConsumers);
       }
-      for (int st = 0; st < kMaxRaw; st++) mbar_init(empty + 8 * kMaxStages + 8 * st, 1);
+      for (int st = 0; st < kMaxRaw; st++) {
+        mbar_init(empty + 8 * (kMaxStages + st), 1);
+        mbar_init(empty + 8 * (kMaxStages + kMaxRaw + st), kShifters);
+      }
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (a.tokens <= 8)
@@ -458,11 +465,11 @@ struct Layer {
         uint32_t phase = 0;
         copy_tiles<0>(a, maps, L, first0, end0, tiles0, ring, full, empty, stage, phase, gave_up);
         copy_tiles<1>(a, maps + 1, L, first1, end1, tiles1, ring, full, empty, stage, phase, gave_up);
-        // after a wait that gave up: let the copies in flight land before the CTA's memory goes
-        if (*gave_up)
-          for (int n = 0; n < 1000; n++) __nanosleep(1000);
-        __syncwarp();
       }
+      // after a wait that gave up: let the copies in flight land before the CTA's memory goes
+      if (*gave_up)
+        for (int n = 0; n < 1000; n++) __nanosleep(1000);
+      __syncwarp();
     } else {
       const int team = warp / kTeam, part = warp % kTeam;
       int stage = 0, parity = 0;
@@ -651,14 +658,16 @@ struct Layer {
   // The same for rows that start at any byte: the 16-byte granules that a row
   // touches come by a bulk copy into a slot, and the copying warps shift the
   // bytes into a stage.  (Granules that reach past the weights' first or last
-  // byte are not copied; what they hold of a row is read byte by byte.)
+  // byte are not copied; what they hold of a row is read byte by byte.)  Rows
+  // that one stage holds whole lie one behind the other: one copy brings a tile's
+  // 16 of w_out, two its 8 and 8 of w_in (a copy costs 70 - 85 ns of its SM at
+  // any size; h 4096, i 181 400 -> 390 us when it came).
   __device__ static __forceinline__ void shift_tiles(const LayerArgs& a, const Lists& L, int first0, int end0, int tiles0, int first1,
                                                      int end1, int tiles1, unsigned char* ring, uint32_t full, uint32_t empty,
                                                      volatile int* gave_up) {
     const int lane = threadIdx.x & 31, copier = (threadIdx.x >> 5) - kConsumers;
-    constexpr int kCopiers = kWarps - kConsumers;
     unsigned char* raw = ring + a.stages * kStageBytes;
-    const uint32_t arrived = empty + 8 * kMaxStages;  // a slot's copies
+    const uint32_t arrived = empty + 8 * kMaxStages, read = arrived + 8 * kMaxRaw;  // a slot's copies; its rows' shifts
     struct At {
       int product, task, byte;
     };
@@ -673,9 +682,10 @@ struct Layer {
       settle(p);
     };
     struct Row {
-      uintptr_t at, lo, hi;  // the row's first byte; the granules that are copied
-      int bytes;
+      uintptr_t at, base, lo, hi;  // the row's first byte; its copy's first granule; the granules that are copied
+      int bytes, from;             // where the copy's first granule goes in the slot
     };
+    auto whole = [&](int product) { return a.row_bytes[product] >= (product == 0 ? a.h : a.i) * (int)sizeof(W); };
     auto row_of = [&](const At& p, int r) {
       const bool p0 = p.product == 0;
       const int tiles = p0 ? tiles0 : tiles1, u = p.task / tiles, tile = p.task - u * tiles;
@@ -685,39 +695,50 @@ struct Layer {
       Row x;
       x.at = w + (L.unit_expert[u] * rows + row) * length + p.byte;
       x.bytes = (int)min((int64_t)a.row_bytes[p.product], length - p.byte);
-      x.lo = max(x.at & ~(uintptr_t)15, (w + 15) & ~(uintptr_t)15);
-      x.hi = max(x.lo, min((x.at + x.bytes + 15) & ~(uintptr_t)15, end & ~(uintptr_t)15));
+      uintptr_t first = x.at, last = x.at + x.bytes;  // what the row's copy brings
+      x.from = r * kRawPitch;
+      if (whole(p.product)) {
+        const int run = p0 ? 8 : 16, first_row = tile * run, last_row = min(first_row + run, p0 ? a.i : a.h);
+        const uintptr_t block = w + (L.unit_expert[u] * rows + (p0 && r >= 8 ? a.i : 0)) * length;
+        first = block + first_row * length, last = block + last_row * length;
+        x.from = (p0 ? r & 8 : 0) * kRawPitch;
+      }
+      x.base = first & ~(uintptr_t)15;
+      x.lo = max(x.base, (w + 15) & ~(uintptr_t)15);
+      x.hi = max(x.lo, min((last + 15) & ~(uintptr_t)15, end & ~(uintptr_t)15));
       return x;
     };
     auto issue = [&](const At& p, int slot) {  // one warp
       const Row x = row_of(p, lane & 15);
-      const int bytes = lane < 16 ? (int)(x.hi - x.lo) : 0;
+      const bool copies = lane < 16 && (!whole(p.product) || lane == 0 || (lane == 8 && p.product == 0));
+      const int bytes = copies ? (int)(x.hi - x.lo) : 0;
       const int all = __reduce_add_sync(~0u, bytes);
       if (lane == 0) mbar_expect_tx(arrived + 8 * slot, all);
       __syncwarp();
       if (bytes)
-        bulk_copy(smem_u32(raw + slot * kRawBytes + lane * kRawPitch) + (uint32_t)(x.lo - (x.at & ~(uintptr_t)15)), (const void*)x.lo, bytes,
-                  arrived + 8 * slot);
+        bulk_copy(smem_u32(raw + slot * kRawBytes + x.from) + (uint32_t)(x.lo - x.base), (const void*)x.lo, bytes, arrived + 8 * slot);
     };
     At p{0, first0, 0};
     settle(p);
-    At ahead = p;
-    if (copier == 0)
-      for (int i = 0; i < a.raw && ahead.product < 2; i++) {
-        issue(ahead, i);
-        next(ahead);
-      }
     int stage = 0, slot = 0;
     uint32_t phase = 0, turn = 0;
+    // (16 copies take a warp as long as its share of the shifts: a warp of their own)
+    if (copier == kShifters) {
+      for (; p.product < 2; next(p)) {
+        if (!warp_wait(read + 8 * slot, turn ^ 1, gave_up, a.flag)) break;
+        issue(p, slot);
+        if (++slot == a.raw) slot = 0, turn ^= 1;
+      }
+      return;
+    }
     for (; p.product < 2; next(p)) {
       mbar_wait(arrived + 8 * slot, turn, gave_up, a.flag);
       mbar_wait(empty + 8 * stage, phase ^ 1, gave_up, a.flag);
       __syncwarp();
-      for (int r = copier; r < 16; r += kCopiers) {
+      for (int r = copier; r < 16; r += kShifters) {
         const Row x = row_of(p, r);
-        const unsigned char* from = raw + slot * kRawBytes + r * kRawPitch;
-        const uintptr_t base = x.at & ~(uintptr_t)15;
-        const int skew = (int)(x.at - base), lo = (int)(x.lo - base), hi = (int)(x.hi - base);
+        const unsigned char* from = raw + slot * kRawBytes + x.from;
+        const int skew = (int)(x.at - x.base), lo = (int)(x.lo - x.base), hi = (int)(x.hi - x.base);
         unsigned char* to = ring + stage * kStageBytes + r * kRowPitch;
         constexpr int kFly = most_bytes(COPY) / 512;  // a lane's 16-byte pieces of the row: all at once
         uint32_t q[kFly][5];
@@ -757,13 +778,11 @@ struct Layer {
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(full + 8 * stage);
-      if (++stage == a.stages) stage = 0, phase ^= 1;
-      asm volatile("bar.sync 15, %0;" ::"n"(kCopiers * 32) : "memory");  // the slot has been read
-      if (copier == 0 && ahead.product < 2) {
-        issue(ahead, slot);
-        next(ahead);
+      if (lane == 0) {
+        mbar_arrive(full + 8 * stage);
+        mbar_arrive(read + 8 * slot);
       }
+      if (++stage == a.stages) stage = 0, phase ^= 1;
       if (++slot == a.raw) slot = 0, turn ^= 1;
     }
   }
@@ -941,7 +960,7 @@ __global__ void __launch_bounds__(warps_of(COPY) * 32, 1)
     layer_kernel(const __grid_constant__ LayerArgs a, const __grid_constant__ Maps maps) {
   __shared__ Lists lists;
   __shared__ int scratch[kMaxExperts];
-  __shared__ __align__(8) uint64_t bars[2 * kMaxStages + kMaxRaw];
+  __shared__ __align__(8) uint64_t bars[2 * (kMaxStages + kMaxRaw)];
   __shared__ int gave_up;
   extern __shared__ __align__(16) unsigned char dyn[];
   Layer<W, X, M, COPY, NT>::run(a, maps.m, lists, scratch, bars, &gave_up, dyn);
