@@ -29,7 +29,8 @@
 // 16-byte vectors as 16 bulk copies of 2 KB, rows 2064 bytes apart, which the
 // copy engine takes at 70 - 85 ns each, below the rate of HBM.  Rows of any
 // other length come by bulk copies of the 16-byte granules that they touch, and
-// seven warps shift them into place: 1.1 - 1.5 TB/s.  Lanes that copied their own fragments (cp.async) spent 110 instructions on each KB: 3.2 TB/s.
+// seven warps shift them into place: 0.5 - 1.5 TB/s.  Lanes that copied their
+// own fragments (cp.async) spent 110 instructions on each KB: 3.2 TB/s.
 //
 // Measured on one B200: 1 token, 8 of 64 experts, h 2048, i 1024, bf16 39 us
 // (router 1.4, choice 5, products 10 and 6, barriers 6, the rest the launch); 8
