@@ -39,10 +39,12 @@
 // barriers.
 //
 // All sums are in 32 bits.  The activations b enter the second product as the
-// sum of two 16-bit numbers (16 or 22 bits of mantissa), so it loses nothing
-// against a 32-bit b; for float16 each row of b is scaled by a power of two
-// first, since b may be out of that type's range.  8-bit weights multiply in
-// float16, x scaled likewise.
+// sum of two 16-bit numbers, which keeps 16 bits of mantissa in bfloat16 (2^-17
+// of each b at most) and 22 in float16 (2^-23, and 2^-39 of the row's largest),
+// where a 32-bit b has 24: below the rounding of y, 2^-9 and 2^-12, by as much.
+// For float16 each row of b is scaled by a power of two first, since b may be
+// out of that type's range.  8-bit weights multiply in float16, x scaled
+// likewise: exact down to 2^-28 of the token's largest, 2^-40 of it at most below.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -86,8 +88,8 @@ struct LayerArgs {
   float* logits;    // [tokens, experts]
   float* b;         // [slots, ip]
   float* o;         // [slots, h]
-  unsigned* bmax;   // [slots] bits of max |b|
-  unsigned* xmax;   // [tokens] bits of max |x| (8-bit layers)
+  unsigned* bmax;   // [slots] magnitude of the largest b
+  unsigned* xmax;   // [tokens] ... of the largest x (8-bit layers)
   unsigned* arrived;  // CTAs whose part of b is written
   int* flag;        // set when a bounded wait ran out
 };
@@ -128,6 +130,12 @@ __device__ __forceinline__ float2 unpack2(uint32_t w) {
 __device__ __forceinline__ uint32_t widen(uint32_t w) {
   const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)w, __NV_E4M3);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The bits of |x|, which order as it does; infinities and NaN do not count.
+__device__ __forceinline__ unsigned magnitude(float x) {
+  const unsigned u = __float_as_uint(x) & 0x7fffffffu;
+  return u < 0x7f800000u ? u : 0;
 }
 
 // 16 bytes of a row of n elements from element k; zeros outside it.
@@ -359,7 +367,7 @@ __device__ __forceinline__ void router(const LayerArgs& a, float* red) {
         const X* xe = reinterpret_cast<const X*>(&xv[t]);
         if (MAX)
 #pragma unroll
-          for (int c = 0; c < 8; c++) top[t] = max(top[t], __float_as_uint(fabsf(to_f32<X>(xe[c]))));
+          for (int c = 0; c < 8; c++) top[t] = max(top[t], magnitude(to_f32<X>(xe[c])));
 #pragma unroll
         for (int j = 0; j < RE; j++) {
           const X* re = reinterpret_cast<const X*>(&rv[j]);
@@ -407,11 +415,15 @@ struct Layer {
   static constexpr int kStepBytes = kStepK * (int)sizeof(W);
   static constexpr int kRed = kTeam * NT * 128;               // floats of a tile's parts
 
-  // What brings a row whose largest value is at `most` into float16's range,
-  // 2^-x, or (sign 1) what takes it back.
-  __device__ static __forceinline__ float power(const unsigned* most, int sign) {
+  // The power of two that brings a row whose largest finite value is at `most`
+  // to float16's upper end, from 2^top up (sign 1), or what takes it back.  There
+  // the row has its type's bits down to 2^-28 of the largest: a channel that
+  // dominates it, and may meet zero weights, costs the others none.  (The sums
+  // are in 32 bits; float16 is 2^16 at most.)
+  static constexpr int kTopX = 15, kTopB = 14;  // x has no more bits than float16; b may round up
+  __device__ static __forceinline__ float power(const unsigned* most, int top, int sign) {
     const int ex = (int)(__ldcg(most) >> 23) - 127;
-    const int c = ex < -100 || ex > 127 ? 0 : min(ex, 126);  // tiny, infinite or NaN: as it is
+    const int c = min(top - ex, 126);  // (a smaller row than 2^-111: as far as 32 bits go)
     return __uint_as_float((uint32_t)(127 + sign * c) << 23);
   }
 
@@ -528,7 +540,7 @@ struct Layer {
           if (kScaled) ga *= back[col], up *= back[col];
           const float v = ga / (1.f + expf(-ga)) * up;
           a.b[slot * a.ip + row] = v;
-          if (kHalf) atomicMax(a.bmax + slot, __float_as_uint(fabsf(v)));
+          if (kHalf) atomicMax(a.bmax + slot, magnitude(v));
         }
       }
       all_consumers_sync(a, gave_up);
@@ -803,7 +815,7 @@ struct Layer {
   __device__ static __forceinline__ void stage_x(const LayerArgs& a, const Lists& L, int expert, int n0, int n, unsigned char* op, float* back) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     consumers_sync();
-    if (kScaled && threadIdx.x < n) back[threadIdx.x] = power(a.xmax + L.slots[n0 + threadIdx.x] / a.top, 1);
+    if (kScaled && threadIdx.x < n) back[threadIdx.x] = power(a.xmax + L.slots[n0 + threadIdx.x] / a.top, kTopX, -1);
     stage_scales(a, a.e.in_scales, expert, 2 * a.i, a.h, op);
     const int padded = (a.h + 127) / 128 * 128;
     for (int c = warp * 32 + lane; c < n * (padded / 8); c += kConsumers * 32) {
@@ -811,7 +823,7 @@ struct Layer {
       const int token = L.slots[n0 + t] / a.top;
       uint4 v = row16<X, VEC>((const X*)a.e.x + (int64_t)token * a.e.ldx, k, a.h, true);
       if (kScaled) {
-        const float f = power(a.xmax + token, -1);
+        const float f = power(a.xmax + token, kTopX, 1);
         uint32_t* w = reinterpret_cast<uint32_t*>(&v);
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -827,13 +839,13 @@ struct Layer {
   __device__ static __forceinline__ void stage_b(const LayerArgs& a, const Lists& L, int expert, int n0, int n, unsigned char* op, float* back) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     consumers_sync();
-    if (kHalf && threadIdx.x < n) back[threadIdx.x] = power(a.bmax + L.slots[n0 + threadIdx.x], 1);
+    if (kHalf && threadIdx.x < n) back[threadIdx.x] = power(a.bmax + L.slots[n0 + threadIdx.x], kTopB, -1);
     stage_scales(a, a.e.out_scales, expert, a.h, a.i, op);
     const int padded = (a.i + 127) / 128 * 128;
     for (int c = warp * 32 + lane; c < n * (padded / 4); c += kConsumers * 32) {
       const int t = c / (padded / 4), k = (c - t * (padded / 4)) * 4;
       const int slot = L.slots[n0 + t];
-      const float scale = kHalf ? power(a.bmax + slot, -1) : 1.f;
+      const float scale = kHalf ? power(a.bmax + slot, kTopB, 1) : 1.f;
       float4 f = make_float4(0, 0, 0, 0);
       if (k < a.i) f = __ldcg(reinterpret_cast<const float4*>(a.b + (int64_t)slot * a.ip + k));
       float v[4] = {f.x, f.y, f.z, f.w};
