@@ -63,7 +63,9 @@ int real_code(const Tensor& t) {
   }
 }
 int code8(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? NDT_E4M3 : t == at::kFloat8_e5m2 ? NDT_E5M2 : 0; }
-bool here(const Tensor& t) { return t.is_cuda() && t.get_device() == c10::cuda::current_device(); }
+// (with the negative bit memory holds the opposite of the tensor's numbers)
+bool here(const Tensor& t) { return t.is_cuda() && !t.is_neg() && t.get_device() == c10::cuda::current_device(); }
+bool beside(const Tensor& t, const Tensor& x) { return t.is_cuda() && !t.is_neg() && t.get_device() == x.get_device(); }
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 void* data(const Tensor& t) { return t.data_ptr(); }
 long at_least(int64_t a, int64_t b) { return (long)std::max(a, b); }
@@ -99,7 +101,7 @@ variable_list once(variable_list grads) {
 
 // ---------------------------------------------------------------- embedding
 bool plain_embedding(const Tensor& table, const Tensor& ids) {
-  return here(table) && ids.is_cuda() && ids.get_device() == table.get_device() && table.dim() == 2 && real_code(table) &&
+  return here(table) && beside(ids, table) && table.dim() == 2 && real_code(table) &&
          unit_rows(table) && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.is_contiguous();
 }
 Maybe embedding(const Tensor& table, const Tensor& ids, double scale, int64_t first) {
@@ -131,6 +133,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     const Tensor ids = ctx->get_saved_variables()[0];
     const int64_t rows = ctx->saved_data["rows"].toInt(), d = grad.size(-1), n = ids.numel();
     at::AutoDispatchBelowADInplaceOrView below;
+    grad = grad.resolve_neg();
     if (grad.dim() != 2) grad = grad.reshape({n, d});
     if (!unit_rows(grad)) grad = grad.contiguous();
     const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
@@ -148,8 +151,7 @@ Maybe torch_embedding(const Tensor& table, const Tensor& ids, double scale, int6
 
 // ------------------------------------------------------------ scaled linear
 Maybe scaled_linear(const Tensor& x, const Tensor& w, const Tensor& scales, std::optional<at::ScalarType> out_type) {
-  if (!here(x) || !w.is_cuda() || !scales.is_cuda() || w.get_device() != x.get_device() || scales.get_device() != x.get_device() ||
-      !real_code(x) || !code8(w.scalar_type()) || w.dim() != 2 || scales.dim() != 2 || scales.scalar_type() != at::kFloat)
+  if (!here(x) || !beside(w, x) || !beside(scales, x) || !real_code(x) || !code8(w.scalar_type()) || w.dim() != 2 || scales.dim() != 2 || scales.scalar_type() != at::kFloat)
     return std::nullopt;
   const int64_t n = w.size(0), k = w.size(1);
   if (x.dim() < 1 || x.size(-1) != k || scales.size(0) != (n + 127) / 128 || scales.size(1) != (k + 127) / 128) return std::nullopt;
@@ -194,6 +196,7 @@ struct ScaledLinearFunction : torch::autograd::Function<ScaledLinearFunction> {
     const int64_t n = ctx->saved_data["n"].toInt(), k = x_sizes.back(), ld = (n + 15) / 16 * 16;
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     at::AutoDispatchBelowADInplaceOrView below;
+    dy = dy.resolve_neg();
     if (dy.dim() != 2) dy = dy.reshape({dy.numel() / std::max<int64_t>(n, 1), n});
     const int64_t t = dy.size(0);
     Tensor dx = need_x ? at::empty({t, k}, dy.options()) : Tensor();
@@ -208,7 +211,7 @@ struct ScaledLinearFunction : torch::autograd::Function<ScaledLinearFunction> {
   }
 };
 Maybe torch_scaled_linear(const Tensor& x, const Tensor& w, at::ScalarType grad_type) {
-  if (!here(x) || !w.is_cuda() || w.get_device() != x.get_device() || !real_code(x) || !real_code(w) || !code8(grad_type) ||
+  if (!here(x) || !beside(w, x) || !real_code(x) || !real_code(w) || !code8(grad_type) ||
       w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(1) || w.size(0) == 0 || !rows_of(x))
     return std::nullopt;
   const bool graph = at::GradMode::is_enabled();

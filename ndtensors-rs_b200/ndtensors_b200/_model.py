@@ -71,6 +71,17 @@ def device_of(what: str, first, *others) -> int:
     return device
 
 
+def plain(*tensors):
+    """The tensors with the numbers that they stand for in memory (torch may hold a tensor as its opposite)."""
+    return [t if t is None or not t.is_neg() else t.resolve_neg() for t in tensors]
+
+
+def out_of(what: str, out) -> None:
+    """A result can be written to ``out`` as it lies."""
+    if out is not None and out.is_neg():
+        raise ValueError(f"{what}: out must not have torch's negative bit")
+
+
 def code_of(what: str, name: str, dtype, allowed) -> int:
     """The C ABI's code of an element type, one of those allowed."""
     code = allowed.get(dtype)
@@ -95,4 +106,4 @@ def unit_rows(x):
     return x if cs == 1 and rs >= x.shape[1] else x.contiguous()
 
 
-__all__ = ["calls", "REAL", "FLOAT8", "launch", "device_of", "code_of", "rows_of", "unit_rows"]
+__all__ = ["calls", "REAL", "FLOAT8", "launch", "device_of", "plain", "out_of", "code_of", "rows_of", "unit_rows"]

@@ -7,7 +7,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._model import REAL, calls, code_of, device_of, launch, unit_rows
+from ._model import REAL, calls, code_of, device_of, launch, out_of, plain, unit_rows
 
 _IDS = {torch.int32: 0, torch.int64: 1}
 
@@ -26,6 +26,7 @@ def embedding(table, ids, scale: float = 1.0, first: int = 0):
     tt, it = code_of("embedding", "table", table.dtype, REAL), code_of("embedding", "ids", ids.dtype, _IDS)
     if table.dim() != 2:
         raise ValueError("embedding: table must be a matrix")
+    table, ids = plain(table, ids)
     table, ids = unit_rows(table), ids.contiguous()
     v, d = table.shape
     out = table.new_empty(ids.shape + (d,))
@@ -48,6 +49,8 @@ def embedding_grad(grad, ids, rows: int, scale: float = 1.0, first: int = 0, out
         raise ValueError("embedding_grad: grad must have the shape of ids and one axis more")
     if rows < 0:
         raise ValueError("embedding_grad: rows must not be negative")
+    out_of("embedding_grad", out)
+    grad, ids = plain(grad, ids)
     d, n = grad.shape[-1], ids.numel()
     g = unit_rows(grad if grad.dim() == 2 else grad.reshape(n, d))
     ids = ids.contiguous()
@@ -90,7 +93,7 @@ _once = once_differentiable(_Embedding.grads)
 def torch_embedding(table, ids, scale: float = 1.0, first: int = 0):
     """``embedding`` with autograd (a dense gradient of the table's type)."""
     out = calls.torch_embedding(table, ids, scale, first)
-    return _Embedding.apply(table, ids, scale, first) if out is None else out
+    return _Embedding.apply(*plain(table, ids), scale, first) if out is None else out
 
 
 __all__ = ["embedding", "embedding_grad", "torch_embedding"]

@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import torch
 
-from ._model import code_of, device_of, launch, rows_of, unit_rows
+from ._model import code_of, device_of, launch, plain, rows_of, unit_rows
 
 E4M3 = torch.float8_e4m3fn
 _HALF = {torch.bfloat16: 3, torch.float16: 4}
@@ -43,6 +43,7 @@ def expert_layer(x, router, w_in, w_out, top: int, in_scales=None, out_scales=No
         raise ValueError("expert_layer: the sizes of x, router, w_in and w_out do not fit")
     if not 1 <= top <= e:
         raise ValueError("expert_layer: top must be from 1 to the number of experts")
+    x, router, w_in, w_out, in_scales, out_scales = plain(x, router, w_in, w_out, in_scales, out_scales)
     if w_in.dtype == E4M3:
         if in_scales is None or out_scales is None:
             raise ValueError("expert_layer: float8 weights need in_scales and out_scales")

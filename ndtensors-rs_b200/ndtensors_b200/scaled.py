@@ -16,7 +16,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._model import FLOAT8, REAL, calls, code_of, device_of, launch, rows_of
+from ._model import FLOAT8, REAL, calls, code_of, device_of, launch, out_of, plain, rows_of
 
 E4M3 = torch.float8_e4m3fn
 
@@ -55,6 +55,7 @@ def quantize_blocks(x, block_rows: int = 1, dtype=E4M3, transposed: bool = False
     if not (values or transposed):
         raise ValueError("quantize_blocks: nothing to compute")
     r, c = x.shape
+    (x,) = plain(x)
     q = s = t = u = None
     qa = ta = (None, 0, None, 0, 0)
     if values:
@@ -96,6 +97,8 @@ def scaled_gemm(a, a_scales, b, b_scales, out_dtype=torch.bfloat16, out=None, ac
     n = b.shape[0]
     if b.shape[1] != k:
         raise ValueError("scaled_gemm: the contracted sizes of a and b differ")
+    out_of("scaled_gemm", out)
+    a, a_scales, b, b_scales = plain(a, a_scales, b, b_scales)
     if out is None:
         if accumulate:
             raise ValueError("scaled_gemm: accumulate needs out")
@@ -130,6 +133,7 @@ def scaled_linear(x, weight, weight_scales, out_dtype=None):
     if x.dim() < 1 or x.shape[-1] != k:
         raise ValueError("scaled_linear: the last axis of x does not fit the weights")
     yt = xt if out_dtype is None else code_of("scaled_linear", "out_dtype", out_dtype, REAL)
+    x, weight, weight_scales = plain(x, weight, weight_scales)
     x2 = rows_of(x)
     t = x2.shape[0]
     y = x.new_empty((t, n), dtype=out_dtype or x.dtype)
@@ -170,7 +174,7 @@ class _ScaledLinear(Function):
         x2, kept = ctx.saved_tensors
         device, xt, g8, x_shape, (n, k), w_dtype, x_dtype = ctx.args
         need_x, need_w, _ = ctx.needs_input_grad
-        dy2 = rows_of(dy)
+        dy2 = rows_of(dy.resolve_neg())
         t = dy2.shape[0]
         ld = (n + 15) // 16 * 16
         dx = dy.new_empty((t, k), dtype=x_dtype) if need_x else None
@@ -203,7 +207,7 @@ def torch_scaled_linear(x, weight, grad_dtype=E4M3):
     code_of("torch_scaled_linear", "grad_dtype", grad_dtype, FLOAT8)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError("torch_scaled_linear: the last axis of x does not fit the weights")
-    return _ScaledLinear.apply(x, weight, grad_dtype)
+    return _ScaledLinear.apply(*plain(x, weight), grad_dtype)
 
 
 __all__ = ["quantize_blocks", "scaled_gemm", "scaled_linear", "torch_scaled_linear"]
