@@ -525,6 +525,13 @@ int ndt_b200_expert_layer_dev(int x_type, const void* x, long tokens, long h, lo
                               const float* out_scales, long i, long top, int renormalize, void* y, long ldy, int* ids,
                               float* weights, void* stream);
 
+/* Diagnostics: a kernel of one thread that waits for what never comes and gives
+ * up after `clocks` SM clocks (1 to 2^31 - 1), as the operators' kernels give up
+ * a wait after some two seconds.  Once it has run, the next call of a
+ * language-model operator reports it (NDT_INTERNAL_ERROR); for testing how a
+ * program takes that report. */
+int ndt_b200_give_up_wait(long clocks, void* stream);
+
 /* Library control and diagnostics */
 int ndt_b200_device_available(void);
 int ndt_b200_set_stream(void* stream); /* NULL restores the library's own stream */

@@ -35,13 +35,14 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
 }
 // A wait that ends: after some two seconds, or once another wait of this CTA has
 // given up, it raises the flags and returns false.
-__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
+__device__ __forceinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag,
+                                               long long limit = kWaitLimit) {
   const long long t0 = clock64();
   while (true) {
     for (int i = 0; i < 32; i++)
       if (mbar_try(bar, parity)) return true;
     if (*gave_up) return false;
-    if (clock64() - t0 > kWaitLimit) {
+    if (clock64() - t0 > limit) {
       *gave_up = 1;
       atomicExch_system(flag, 1);
       return false;

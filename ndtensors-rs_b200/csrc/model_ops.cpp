@@ -14,6 +14,15 @@ namespace ndt {
 namespace {
 std::mutex g_flag_mu;
 int* g_flag = nullptr;  // host memory, mapped for every device
+
+// One thread waits on a barrier that nothing arrives at.
+__global__ void give_up_kernel(long long limit, int* flag) {
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ int gave_up;
+  gave_up = 0;
+  mbar_init(smem_u32(&bar), 1);
+  mbar_wait_slow(smem_u32(&bar), 0, &gave_up, flag, limit);
+}
 }  // namespace
 
 int* wait_flag_device() {
@@ -32,7 +41,10 @@ bool wait_flag_raised() {
   *(volatile int*)g_flag = 0;
   return true;
 }
-
+static void give_up_wait(long long clocks, cudaStream_t s) {
+  give_up_kernel<<<1, 1, 0, s>>>(clocks, wait_flag_device());
+  NDT_CUDA(cudaGetLastError());
+}
 
 CUtensorMap byte_map(const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
   using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -69,7 +81,7 @@ int entry(const char* name, F&& body) {
   try {
     ctx();
     if (wait_flag_raised())
-      throw Error(ErrKind::Cuda, "an earlier scaled product gave up waiting inside its kernel: its result is not valid");
+      throw Error(ErrKind::Cuda, "an earlier scaled product or expert layer gave up waiting inside its kernel: its result is not valid");
     body();
     return NDT_SUCCESS;
   } catch (const Error& e) {
@@ -333,6 +345,13 @@ int ndt_b200_expert_layer_dev(int x_type, const void* x, long tokens, long h, lo
     a.renormalize = renormalize != 0;
     a.y = y, a.ids = ids, a.weights = weights;
     expert_layer(a, (cudaStream_t)stream);
+  });
+}
+
+int ndt_b200_give_up_wait(long clocks, void* stream) {
+  return entry("give_up_wait", [&] {
+    if (clocks < 1 || clocks > INT_MAX) bad("clocks must be from 1 to 2^31 - 1");
+    give_up_wait(clocks, (cudaStream_t)stream);
   });
 }
 

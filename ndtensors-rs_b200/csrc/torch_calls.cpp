@@ -5,7 +5,10 @@
 // (the thread that runs the backward pass has to get the interpreter).  These
 // functions make the plain calls - CUDA tensors of the current device, types
 // and strides that need no copy - and return nothing for any other, which the
-// Python functions of the same names then check, lay out or refuse.
+// Python functions of the same names then check, lay out or refuse.  A call that
+// was made and failed raises what it would raise from Python: it is not made
+// again, since its entry point may have reported an earlier call's failure,
+// which it does once.
 //
 // They call the C entry points of libndtensors_capi.so through addresses that
 // bind() is given, so this file needs torch alone.
@@ -13,6 +16,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -43,10 +47,13 @@ template <typename F>
 void set(F& f, uintptr_t address) {
   f = reinterpret_cast<F>(address);
 }
-void bind(const std::vector<uintptr_t>& at) {
+PyObject* failure = nullptr;  // the package's exception for a status
+
+void bind(const std::vector<uintptr_t>& at, py::object exception) {
   TORCH_CHECK(at.size() == 6, "bind: six addresses");
   set(entry.scaled_linear, at[0]), set(entry.scaled_linear_fwd, at[1]), set(entry.scaled_linear_vjp, at[2]);
   set(entry.embedding, at[3]), set(entry.embedding_grad, at[4]), set(entry.last_error, at[5]);
+  failure = exception.release().ptr();
 }
 
 // The C ABI's code of a 32- or 16-bit floating type, or 0.
@@ -83,7 +90,19 @@ Tensor like_rows(const Tensor& y, const Tensor& x, int64_t last) {  // y [tokens
   sizes.back() = last;
   return y.view(sizes);
 }
-void check(int status) { TORCH_CHECK(status == NDT_SUCCESS, entry.last_error()); }
+// Raises as the Python functions do (from a backward pass's thread too).
+void check(int status) {
+  if (status == NDT_SUCCESS) return;
+  const std::string text = entry.last_error();  // (of this thread)
+  py::gil_scoped_acquire gil;
+  if (status == NDT_SHAPE_MISMATCH)
+    PyErr_SetString(PyExc_ValueError, text.c_str());
+  else
+    PyErr_SetString(failure, (text + " (status " + std::to_string(status) + ")").c_str());
+  python_error e;
+  e.persist();
+  throw e;
+}
 
 // A gradient that a graph was asked of: differentiating it again is an error.
 variable_list once(variable_list grads) {
@@ -110,9 +129,9 @@ Maybe embedding(const Tensor& table, const Tensor& ids, double scale, int64_t fi
   auto sizes = ids.sizes().vec();
   sizes.push_back(d);
   Tensor out = at::empty(sizes, table.options().requires_grad(false));
-  const int status = entry.embedding(real_code(table), data(table), v, d, at_least(d, table.stride(0)), data(ids),
-                                     ids.scalar_type() == at::kLong, ids.numel(), first, (float)scale, data(out), d, stream());
-  return status == NDT_SUCCESS ? Maybe(out) : std::nullopt;
+  check(entry.embedding(real_code(table), data(table), v, d, at_least(d, table.stride(0)), data(ids), ids.scalar_type() == at::kLong,
+                        ids.numel(), first, (float)scale, data(out), d, stream()));
+  return out;
 }
 
 struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
@@ -122,9 +141,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["first"] = first;
     ctx->saved_data["type"] = (int64_t)table.scalar_type();
-    Maybe out = embedding(table, ids, scale, first);
-    TORCH_CHECK(out.has_value(), entry.last_error());
-    return *out;
+    return *embedding(table, ids, scale, first);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor grad = grads[0];
@@ -160,10 +177,10 @@ Maybe scaled_linear(const Tensor& x, const Tensor& w, const Tensor& scales, std:
   const int64_t t = x2->size(0);
   Tensor y = at::empty({t, n}, x.options().dtype(out_type.value_or(x.scalar_type())).requires_grad(false));
   if (!real_code(y)) return std::nullopt;
-  const int status = entry.scaled_linear(real_code(x), data(*x2), t, k, x2->stride(0), x2->stride(1), code8(w.scalar_type()), data(w), n,
-                                         w.stride(0), w.stride(1), static_cast<const float*>(data(scales)), scales.stride(0),
-                                         scales.stride(1), real_code(y), data(y), n, stream());
-  return status == NDT_SUCCESS ? Maybe(like_rows(y, x, n)) : std::nullopt;
+  check(entry.scaled_linear(real_code(x), data(*x2), t, k, x2->stride(0), x2->stride(1), code8(w.scalar_type()), data(w), n, w.stride(0),
+                            w.stride(1), static_cast<const float*>(data(scales)), scales.stride(0), scales.stride(1), real_code(y),
+                            data(y), n, stream()));
+  return like_rows(y, x, n);
 }
 
 struct ScaledLinearFunction : torch::autograd::Function<ScaledLinearFunction> {

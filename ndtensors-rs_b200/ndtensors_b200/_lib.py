@@ -182,6 +182,7 @@ SIGNATURES = [
     ("ndt_b200_embedding_grad_dev", ctypes.c_int, [ci, vp, cl, vp, ci, cl, cl, cl, cl, cf, ci, vp, cl, ci, vp]),
     ("ndt_b200_expert_layer_dev", ctypes.c_int,
      [ci, vp, cl, cl, cl, vp, cl, ci, vp, vp, vp, vp, cl, cl, ci, vp, cl, vp, vp, vp]),
+    ("ndt_b200_give_up_wait", ctypes.c_int, [cl, vp]),
     ("ndt_b200_device_available", ctypes.c_int, []),
     ("ndt_b200_set_stream", ctypes.c_int, [vp]),
     ("ndt_b200_get_stream", vp, []),

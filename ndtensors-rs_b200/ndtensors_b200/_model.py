@@ -27,7 +27,7 @@ def _load_calls():
     loader.exec_module(module)
     lib = get_lib()
     names = ("scaled_linear_dev", "scaled_linear_fwd_dev", "scaled_linear_vjp_dev", "embedding_dev", "embedding_grad_dev", "last_error")
-    module.bind([ctypes.cast(getattr(lib, f"ndt_b200_{n}"), ctypes.c_void_p).value for n in names])
+    module.bind([ctypes.cast(getattr(lib, f"ndt_b200_{n}"), ctypes.c_void_p).value for n in names], NDTensorsError)
     return module
 
 
