@@ -84,11 +84,12 @@ Maybe rows_of(const Tensor& x) {
   if (x.dim() < 1 || !x.is_contiguous() || x.size(-1) == 0) return std::nullopt;
   return x.view({-1, x.size(-1)});
 }
-Tensor like_rows(const Tensor& y, const Tensor& x, int64_t last) {  // y [tokens, last] in x's shape
-  if (x.dim() == 2) return y;
+// An empty result in x's shape with another last axis.  (Not a view of a matrix:
+// torch refuses to change a view that comes out of a Function in place.)
+Tensor result(const Tensor& x, int64_t last, at::ScalarType type) {
   auto sizes = x.sizes().vec();
   sizes.back() = last;
-  return y.view(sizes);
+  return at::empty(sizes, x.options().dtype(type).requires_grad(false));
 }
 // Raises as the Python functions do (from a backward pass's thread too).
 void check(int status) {
@@ -175,12 +176,12 @@ Maybe scaled_linear(const Tensor& x, const Tensor& w, const Tensor& scales, std:
   const Maybe x2 = rows_of(x);
   if (!x2) return std::nullopt;
   const int64_t t = x2->size(0);
-  Tensor y = at::empty({t, n}, x.options().dtype(out_type.value_or(x.scalar_type())).requires_grad(false));
+  Tensor y = result(x, n, out_type.value_or(x.scalar_type()));
   if (!real_code(y)) return std::nullopt;
   check(entry.scaled_linear(real_code(x), data(*x2), t, k, x2->stride(0), x2->stride(1), code8(w.scalar_type()), data(w), n, w.stride(0),
                             w.stride(1), static_cast<const float*>(data(scales)), scales.stride(0), scales.stride(1), real_code(y),
                             data(y), n, stream()));
-  return like_rows(y, x, n);
+  return y;
 }
 
 struct ScaledLinearFunction : torch::autograd::Function<ScaledLinearFunction> {
@@ -189,7 +190,7 @@ struct ScaledLinearFunction : torch::autograd::Function<ScaledLinearFunction> {
     const int64_t n = w.size(0), k = w.size(1);
     const Tensor x2 = *rows_of(x);
     const int64_t t = x2.size(0);
-    Tensor y = at::empty({t, n}, x.options().requires_grad(false));
+    Tensor y = result(x, n, x.scalar_type());
     // the weights' 8-bit transpose, kept for x's gradient: values and scales in one buffer
     const int64_t ld = (n + 15) / 16 * 16, kb = (k + 127) / 128, nb = (n + 127) / 128;
     Tensor kept = need_x ? at::empty({k * ld + 4 * kb * nb}, x.options().dtype(at::kByte).requires_grad(false)) : Tensor();
@@ -201,7 +202,7 @@ struct ScaledLinearFunction : torch::autograd::Function<ScaledLinearFunction> {
     ctx->saved_data["n"] = n;
     ctx->saved_data["grad8"] = grad8;
     ctx->saved_data["w_type"] = (int64_t)w.scalar_type();
-    return like_rows(y, x, n);
+    return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor dy = grads[0];

@@ -136,10 +136,10 @@ def scaled_linear(x, weight, weight_scales, out_dtype=None):
     x, weight, weight_scales = plain(x, weight, weight_scales)
     x2 = rows_of(x)
     t = x2.shape[0]
-    y = x.new_empty((t, n), dtype=out_dtype or x.dtype)
+    y = x.new_empty(x.shape[:-1] + (n,), dtype=out_dtype or x.dtype)
     launch("ndt_b200_scaled_linear_dev", device, xt, x2.data_ptr(), t, k, *x2.stride(), wt, weight.data_ptr(), n,
            *weight.stride(), weight_scales.data_ptr(), *weight_scales.stride(), yt, y.data_ptr(), n)
-    return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
+    return y
 
 
 class _ScaledLinear(Function):
@@ -152,7 +152,7 @@ class _ScaledLinear(Function):
         n, k = weight.shape
         x2 = rows_of(x)
         t = x2.shape[0]
-        y = x.new_empty((t, n))
+        y = x.new_empty(x.shape[:-1] + (n,))  # (a view of a matrix could not be changed in place)
         need_x, need_w, _ = ctx.needs_input_grad
         # the weights' 8-bit transpose, kept for x's gradient: values and scales in one buffer
         ld, kb, nb = (n + 15) // 16 * 16, (k + 127) // 128, (n + 127) // 128
@@ -162,7 +162,7 @@ class _ScaledLinear(Function):
                *weight.stride(), y.data_ptr(), max(1, n), at or None, ld, at + k * ld if need_x else None)
         ctx.save_for_backward(x2 if need_w else None, kept)
         ctx.args = device, xt, FLOAT8[grad_dtype], x.shape, weight.shape, weight.dtype, x.dtype
-        return y if x.dim() == 2 else y.view(x.shape[:-1] + (n,))
+        return y
 
     @staticmethod
     def backward(ctx, dy):
