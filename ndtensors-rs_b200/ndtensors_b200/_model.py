@@ -82,6 +82,12 @@ def out_of(what: str, out) -> None:
         raise ValueError(f"{what}: out must not have torch's negative bit")
 
 
+def written(out) -> None:
+    """``out`` was changed in place: a graph that saved it before must not be differentiated with what it holds now."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def code_of(what: str, name: str, dtype, allowed) -> int:
     """The C ABI's code of an element type, one of those allowed."""
     code = allowed.get(dtype)
@@ -106,4 +112,4 @@ def unit_rows(x):
     return x if cs == 1 and rs >= x.shape[1] else x.contiguous()
 
 
-__all__ = ["calls", "REAL", "FLOAT8", "launch", "device_of", "plain", "out_of", "code_of", "rows_of", "unit_rows"]
+__all__ = ["calls", "REAL", "FLOAT8", "launch", "device_of", "plain", "out_of", "written", "code_of", "rows_of", "unit_rows"]

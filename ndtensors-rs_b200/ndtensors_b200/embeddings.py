@@ -7,7 +7,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._model import REAL, calls, code_of, device_of, launch, out_of, plain, unit_rows
+from ._model import REAL, calls, code_of, device_of, launch, out_of, plain, unit_rows, written
 
 _IDS = {torch.int32: 0, torch.int64: 1}
 
@@ -65,6 +65,8 @@ def embedding_grad(grad, ids, rows: int, scale: float = 1.0, first: int = 0, out
         out = grad.new_empty((rows, d), dtype=out_dtype)
     launch("ndt_b200_embedding_grad_dev", device, gt, g.data_ptr(), max(d, g.stride(0)), ids.data_ptr(), it, n, rows, d,
            first, scale, ot, out.data_ptr(), max(d, out.stride(0)), accumulate)
+    if accumulate:
+        written(out)
     return out
 
 

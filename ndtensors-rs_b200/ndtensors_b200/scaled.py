@@ -16,7 +16,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._model import FLOAT8, REAL, calls, code_of, device_of, launch, out_of, plain, rows_of
+from ._model import FLOAT8, REAL, calls, code_of, device_of, launch, out_of, plain, rows_of, written
 
 E4M3 = torch.float8_e4m3fn
 
@@ -99,7 +99,8 @@ def scaled_gemm(a, a_scales, b, b_scales, out_dtype=torch.bfloat16, out=None, ac
         raise ValueError("scaled_gemm: the contracted sizes of a and b differ")
     out_of("scaled_gemm", out)
     a, a_scales, b, b_scales = plain(a, a_scales, b, b_scales)
-    if out is None:
+    given = out is not None
+    if not given:
         if accumulate:
             raise ValueError("scaled_gemm: accumulate needs out")
         ct = code_of("scaled_gemm", "out_dtype", out_dtype, REAL)
@@ -111,6 +112,8 @@ def scaled_gemm(a, a_scales, b, b_scales, out_dtype=torch.bfloat16, out=None, ac
     launch("ndt_b200_scaled_gemm_dev", device, m, n, k, at, a.data_ptr(), *a.stride(), ra, a_scales.data_ptr(),
            *a_scales.stride(), bt, b.data_ptr(), *b.stride(), rb, b_scales.data_ptr(), *b_scales.stride(), ct,
            out.data_ptr(), max(n, out.stride(0)), accumulate)
+    if given:
+        written(out)
     return out
 
 

@@ -27,3 +27,23 @@ def test_results_can_be_changed_in_place(gpu, gaps):
             y = y + r
         grads.append(torch.autograd.grad((y * y).sum(), (x, w, r)))
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_results_written_to_out_count_as_changed(gpu):
+    """A tensor that a graph has saved, overwritten by a call: its backward pass is refused, not wrong."""
+    q, s = gpu.quantize_blocks(normal(4, 8, 128))
+    ids = torch.arange(8, device="cuda")
+    for write in (lambda c: gpu.scaled_gemm(q, s, q, s, out=c), lambda c: gpu.scaled_gemm(q, s, q, s, out=c, accumulate=True),
+                  lambda c: gpu.embedding_grad(normal(5, 8, 8), ids, 8, out=c)):
+        p, c = normal(6, 8, 8).requires_grad_(), normal(7, 8, 8)
+        loss = (p * c).sum()
+        before = c._version
+        write(c)
+        assert c._version > before
+        with pytest.raises(RuntimeError, match="inplace"):
+            loss.backward()
+    with torch.inference_mode():
+        c = torch.zeros(8, 8, device="cuda")
+        gpu.scaled_gemm(q, s, q, s, out=c)
+    gpu.scaled_gemm(q, s, q, s, out=c)
+    assert bool(c.any())
