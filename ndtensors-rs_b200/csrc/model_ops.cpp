@@ -86,6 +86,7 @@ int entry(const char* name, F&& body) {
     return NDT_SUCCESS;
   } catch (const Error& e) {
     set_last_error(std::string(name) + ": " + e.what());
+    if (e.kind == ErrKind::Cuda) cudaGetLastError();  // the runtime keeps it for the next kernel launch of the library to find
     switch (e.kind) {
       case ErrKind::Panic:
       case ErrKind::Cuda:
