@@ -34,10 +34,12 @@ constexpr int kList = kPlacers * kPerThread + kPlacers;  // compacted ids of a r
 constexpr int kEntries = 32;                       // sorted entries a tile
 constexpr int kSumThreads = 128;                   // (256 leave a last wave of half the SMs)
 
-// The table's row of id i; at least 2^63 for an id below the table's first.
+// The table's row of id i; for an id below the table's first the largest number
+// (the difference alone comes round to a row where first is near 2^63).
 template <bool IDS64>
 __device__ __forceinline__ uint64_t row_at(const void* ids, int64_t i, int64_t first) {
-  return (uint64_t)(IDS64 ? ((const int64_t*)ids)[i] : (int64_t)((const int*)ids)[i]) - (uint64_t)first;
+  const int64_t id = IDS64 ? ((const int64_t*)ids)[i] : (int64_t)((const int*)ids)[i];
+  return id < first ? ~0ull : (uint64_t)id - (uint64_t)first;
 }
 
 // ---------------------------------------------------------------- lookup
