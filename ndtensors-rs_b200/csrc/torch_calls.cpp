@@ -72,6 +72,8 @@ int real_code(const Tensor& t) {
 int code8(at::ScalarType t) { return t == at::kFloat8_e4m3fn ? NDT_E4M3 : t == at::kFloat8_e5m2 ? NDT_E5M2 : 0; }
 // (with the negative bit memory holds the opposite of the tensor's numbers)
 bool here(const Tensor& t) { return t.is_cuda() && !t.is_neg() && t.get_device() == c10::cuda::current_device(); }
+// A call without a gradient of its own refuses these.
+bool asks(const Tensor& t) { return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined(); }
 bool beside(const Tensor& t, const Tensor& x) { return t.is_cuda() && !t.is_neg() && t.get_device() == x.get_device(); }
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 void* data(const Tensor& t) { return t.data_ptr(); }
@@ -124,8 +126,7 @@ bool plain_embedding(const Tensor& table, const Tensor& ids) {
   return here(table) && beside(ids, table) && table.dim() == 2 && real_code(table) &&
          unit_rows(table) && (ids.scalar_type() == at::kLong || ids.scalar_type() == at::kInt) && ids.is_contiguous();
 }
-Maybe embedding(const Tensor& table, const Tensor& ids, double scale, int64_t first) {
-  if (!plain_embedding(table, ids)) return std::nullopt;
+Tensor lookup(const Tensor& table, const Tensor& ids, double scale, int64_t first) {
   const int64_t v = table.size(0), d = table.size(1);
   auto sizes = ids.sizes().vec();
   sizes.push_back(d);
@@ -133,6 +134,10 @@ Maybe embedding(const Tensor& table, const Tensor& ids, double scale, int64_t fi
   check(entry.embedding(real_code(table), data(table), v, d, at_least(d, table.stride(0)), data(ids), ids.scalar_type() == at::kLong,
                         ids.numel(), first, (float)scale, data(out), d, stream()));
   return out;
+}
+Maybe embedding(const Tensor& table, const Tensor& ids, double scale, int64_t first) {
+  if (!plain_embedding(table, ids) || asks(table)) return std::nullopt;
+  return lookup(table, ids, scale, first);
 }
 
 struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
@@ -142,7 +147,7 @@ struct EmbeddingFunction : torch::autograd::Function<EmbeddingFunction> {
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["first"] = first;
     ctx->saved_data["type"] = (int64_t)table.scalar_type();
-    return *embedding(table, ids, scale, first);
+    return lookup(table, ids, scale, first);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor grad = grads[0];
@@ -169,7 +174,7 @@ Maybe torch_embedding(const Tensor& table, const Tensor& ids, double scale, int6
 
 // ------------------------------------------------------------ scaled linear
 Maybe scaled_linear(const Tensor& x, const Tensor& w, const Tensor& scales, std::optional<at::ScalarType> out_type) {
-  if (!here(x) || !beside(w, x) || !beside(scales, x) || !real_code(x) || !code8(w.scalar_type()) || w.dim() != 2 || scales.dim() != 2 || scales.scalar_type() != at::kFloat)
+  if (!here(x) || !beside(w, x) || !beside(scales, x) || asks(x) || asks(w) || asks(scales) || !real_code(x) || !code8(w.scalar_type()) || w.dim() != 2 || scales.dim() != 2 || scales.scalar_type() != at::kFloat)
     return std::nullopt;
   const int64_t n = w.size(0), k = w.size(1);
   if (x.dim() < 1 || x.size(-1) != k || scales.size(0) != (n + 127) / 128 || scales.size(1) != (k + 127) / 128) return std::nullopt;

@@ -13,6 +13,7 @@ import importlib.util
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 from ._lib import get_lib, last_error
 from .tensor import NDTensorsError, StatusCode
@@ -71,6 +72,15 @@ def device_of(what: str, first, *others) -> int:
     return device
 
 
+def no_gradient(what: str, instead: str, *tensors) -> None:
+    """Refuse inputs that ask for a gradient: the result would carry none."""
+    asked = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if not asked and forward_ad._current_level >= 0:
+        asked = any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if asked:
+        raise NDTensorsError(f"{what}: an input requires a gradient, and the result would carry none: {instead}")
+
+
 def plain(*tensors):
     """The tensors with the numbers that they stand for in memory (torch may hold a tensor as its opposite)."""
     return [t if t is None or not t.is_neg() else t.resolve_neg() for t in tensors]
@@ -112,4 +122,4 @@ def unit_rows(x):
     return x if cs == 1 and rs >= x.shape[1] else x.contiguous()
 
 
-__all__ = ["calls", "REAL", "FLOAT8", "launch", "device_of", "plain", "out_of", "written", "code_of", "rows_of", "unit_rows"]
+__all__ = ["calls", "REAL", "FLOAT8", "launch", "device_of", "no_gradient", "plain", "out_of", "written", "code_of", "rows_of", "unit_rows"]

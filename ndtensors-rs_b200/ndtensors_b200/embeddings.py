@@ -7,7 +7,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._model import REAL, calls, code_of, device_of, launch, out_of, plain, unit_rows, written
+from ._model import REAL, calls, code_of, device_of, launch, no_gradient, out_of, plain, unit_rows, written
 
 _IDS = {torch.int32: 0, torch.int64: 1}
 
@@ -17,11 +17,18 @@ def embedding(table, ids, scale: float = 1.0, first: int = 0):
 
     An id outside ``[first, first + rows)`` gives zeros, so that ranks holding
     slices of a vocabulary (``first``: the slice's first id) add up to the
-    whole lookup.
+    whole lookup.  The result carries no gradient (``torch_embedding`` has one),
+    so a table that requires one is refused unless gradients are off.
     """
     out = calls.embedding(table, ids, scale, first)
     if out is not None:
         return out
+    device_of("embedding", table, ids)
+    no_gradient("embedding", "use torch_embedding, or call it under torch.no_grad()", table)
+    return _lookup(table, ids, scale, first)
+
+
+def _lookup(table, ids, scale, first):
     device = device_of("embedding", table, ids)
     tt, it = code_of("embedding", "table", table.dtype, REAL), code_of("embedding", "ids", ids.dtype, _IDS)
     if table.dim() != 2:
@@ -44,6 +51,7 @@ def embedding_grad(grad, ids, rows: int, scale: float = 1.0, first: int = 0, out
     it, and only the rows that ids name are touched.
     """
     device = device_of("embedding_grad", grad, ids, out)
+    no_gradient("embedding_grad", "call it under torch.no_grad()", grad, out)
     gt, it = code_of("embedding_grad", "grad", grad.dtype, REAL), code_of("embedding_grad", "ids", ids.dtype, _IDS)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape:
         raise ValueError("embedding_grad: grad must have the shape of ids and one axis more")
@@ -75,7 +83,7 @@ class _Embedding(Function):
     def forward(ctx, table, ids, scale, first):
         ctx.save_for_backward(ids)
         ctx.args = (table.shape[0], scale, first, table.dtype)
-        return embedding(table, ids, scale, first)
+        return _lookup(table, ids, scale, first)
 
     @staticmethod
     def backward(ctx, grad):

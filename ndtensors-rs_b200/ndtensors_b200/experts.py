@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import torch
 
-from ._model import code_of, device_of, launch, plain, rows_of, unit_rows
+from ._model import code_of, device_of, launch, no_gradient, plain, rows_of, unit_rows
 
 E4M3 = torch.float8_e4m3fn
 _HALF = {torch.bfloat16: 3, torch.float16: 4}
@@ -27,10 +27,12 @@ def expert_layer(x, router, w_in, w_out, top: int, in_scales=None, out_scales=No
     [experts, ceil(h / 128), ceil(i / 128)]).
 
     Returns ``(y, ids, weights)``: x's shape and type, and int32 / float32
-    [..., top].  Made for at most about a hundred tokens (a decoding batch);
+    [..., top].  They carry no gradient, so inputs that require one are refused
+    unless gradients are off.  Made for at most about a hundred tokens (a decoding batch);
     more are right, but each 8 or 16 tokens of an expert read its weights anew.
     """
     device = device_of("expert_layer", x, router, w_in, w_out, in_scales, out_scales)
+    no_gradient("expert_layer", "call it under torch.no_grad()", x, router, w_in, w_out, in_scales, out_scales)
     xt = code_of("expert_layer", "x", x.dtype, _HALF)
     code_of("expert_layer", "router", router.dtype, {x.dtype: xt})
     wt = code_of("expert_layer", "w_in", w_in.dtype, {x.dtype: xt, E4M3: 5})

@@ -16,7 +16,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._model import FLOAT8, REAL, calls, code_of, device_of, launch, out_of, plain, rows_of, written
+from ._model import FLOAT8, REAL, calls, code_of, device_of, launch, no_gradient, out_of, plain, rows_of, written
 
 E4M3 = torch.float8_e4m3fn
 
@@ -44,7 +44,8 @@ def quantize_blocks(x, block_rows: int = 1, dtype=E4M3, transposed: bool = False
 
     Returns ``(q, scales)``; with ``transposed`` ``(q, scales, qt, scales_t)``,
     qt being the 8-bit form of x's transpose from the same pass over x (and
-    with ``values=False`` only ``(qt, scales_t)``).
+    with ``values=False`` only ``(qt, scales_t)``).  They carry no gradient to
+    x: a parameter's 8-bit form is a constant.
     """
     device = device_of("quantize_blocks", x)
     xt, qt8 = code_of("quantize_blocks", "x", x.dtype, REAL), code_of("quantize_blocks", "dtype", dtype, FLOAT8)
@@ -88,9 +89,11 @@ def scaled_gemm(a, a_scales, b, b_scales, out_dtype=torch.bfloat16, out=None, ac
     Sums are in 32 bits and rounded once to ``out_dtype`` (float32, bfloat16 or
     float16).  ``out`` receives the result, added to what it holds with
     ``accumulate``.  Any strides are taken; rows that do not start on 16 bytes
-    cost a copy.
+    cost a copy.  The result carries no gradient, so inputs that require one
+    are refused unless gradients are off.
     """
     device = device_of("scaled_gemm", a, a_scales, b, b_scales, out)
+    no_gradient("scaled_gemm", "call it under torch.no_grad()", a, a_scales, b, b_scales, out)
     at, bt = code_of("scaled_gemm", "a", a.dtype, FLOAT8), code_of("scaled_gemm", "b", b.dtype, FLOAT8)
     ra, rb = _block_rows("scaled_gemm", a, a_scales), _block_rows("scaled_gemm", b, b_scales)
     m, k = a.shape
@@ -122,12 +125,14 @@ def scaled_linear(x, weight, weight_scales, out_dtype=None):
 
     ``weight_scales`` are those of the 128 x 128 blocks of w.  x is quantised
     in the call (e4m3, a scale for each row and 128 columns).  ``out_dtype``
-    defaults to x's type.
+    defaults to x's type.  The result carries no gradient, so an x that requires
+    one is refused unless gradients are off.
     """
     y = calls.scaled_linear(x, weight, weight_scales, out_dtype)
     if y is not None:
         return y
     device = device_of("scaled_linear", x, weight, weight_scales)
+    no_gradient("scaled_linear", "use torch_scaled_linear, or call it under torch.no_grad()", x, weight, weight_scales)
     xt = code_of("scaled_linear", "x", x.dtype, REAL)
     wt = code_of("scaled_linear", "weight", weight.dtype, FLOAT8)
     if _block_rows("scaled_linear", weight, weight_scales) != 128:
