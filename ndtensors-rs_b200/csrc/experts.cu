@@ -78,7 +78,7 @@ struct LayerArgs {
   ExpertArgs e;
   int tokens, experts, top, h, i;
   int ip;           // i rounded up to 8: the pitch of b's rows
-  int unit;         // tokens of an expert that a CTA takes at a time
+  int unit;         // tokens of an expert that a CTA takes at a time (each unit reads the weights anew)
   int stages;
   int raw;             // slots for rows at any byte (kShift)
   int row_bytes[2];    // of a row in one stage of each product: even parts of the row
@@ -993,7 +993,8 @@ CUtensorMap weight_map(const void* w, int64_t rows, int64_t bytes, int stage_row
 template <typename W, typename X, typename M, int COPY, int NT>
 void launch(LayerArgs& a, int64_t row, cudaStream_t s) {
   auto kern = layer_kernel<W, X, M, COPY, NT>;
-  // as many tokens as fit beside kKeep of stages (at least one, beside two stages), and stages for the rest
+  // as many tokens as fit beside kKeep of stages (at least one, beside two stages), and stages for the rest.
+  // 16-bit weights: 8 up to i 2688 and h 5376, 6 for 7168 / 2048, 3 for i 6400, 1 for i 14336.
   const int space = room(NT), kStageBytes = stage_bytes(COPY), kKeep = (COPY == kShift ? 132 : 100) * 1024;
   if (row > space - 8192 - 2 * kStageBytes - (COPY == kShift ? kRawBytes : 0)) throw Error(ErrKind::InvalidArgument, "h or i is too large for a token's row to fit shared memory");
   a.unit = (int)std::max<int64_t>(1, std::min<int64_t>({NT * 8, a.tokens, (space - kKeep - (sizeof(W) == 1 ? 8192 : 0)) / row}));
