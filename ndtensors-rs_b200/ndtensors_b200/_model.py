@@ -2,7 +2,8 @@
 
 A call for a few tokens costs the host more than the GPU, so the plain cases
 go through ``calls``, a small C++ module (``csrc/torch_calls.cpp``) that
-returns None for any other; the wrappers then check, lay out or refuse.
+returns None for any other; the wrappers then check, lay out or refuse.  Where
+that module is missing they make every call themselves, with the same results.
 """
 
 from __future__ import annotations
@@ -10,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import importlib.machinery
 import importlib.util
+import warnings
 from pathlib import Path
 
 import torch
@@ -19,15 +21,27 @@ from ._lib import get_lib, last_error
 from .tensor import NDTensorsError, StatusCode
 
 
-def _load_calls():
-    path = Path(__file__).resolve().parent.parent / "lib" / "ndt_torch_calls.so"
-    if not path.exists():
-        raise FileNotFoundError(f"{path} not found: build it with `make -C ndtensors-rs_b200`")
-    loader = importlib.machinery.ExtensionFileLoader("ndt_torch_calls", str(path))
-    module = importlib.util.module_from_spec(importlib.util.spec_from_loader("ndt_torch_calls", loader))
-    loader.exec_module(module)
+class _NoCalls:
+    """In place of the C++ module: no call is a plain one, so the Python functions make them all."""
+
+    @staticmethod
+    def _none(*_):
+        return None
+
+    embedding = torch_embedding = scaled_linear = torch_scaled_linear = _none
+
+
+def _load_calls(path=Path(__file__).resolve().parent.parent / "lib" / "ndt_torch_calls.so"):
     lib = get_lib()
     names = ("scaled_linear_dev", "scaled_linear_fwd_dev", "scaled_linear_vjp_dev", "embedding_dev", "embedding_grad_dev", "last_error")
+    try:
+        loader = importlib.machinery.ExtensionFileLoader("ndt_torch_calls", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("ndt_torch_calls", loader))
+        loader.exec_module(module)
+    except ImportError as e:  # not built, or for another torch
+        warnings.warn(f"{path.name} does not load, so small calls take longer on the host; build it with "
+                      f"`make -C ndtensors-rs_b200` ({e})", RuntimeWarning, stacklevel=2)
+        return _NoCalls()
     module.bind([ctypes.cast(getattr(lib, f"ndt_b200_{n}"), ctypes.c_void_p).value for n in names], NDTensorsError)
     return module
 
