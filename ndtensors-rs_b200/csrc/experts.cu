@@ -476,12 +476,9 @@ struct Layer {
       } else {
         int stage = 0;
         uint32_t phase = 0;
-        copy_tiles<0>(a, maps, L, first0, end0, tiles0, ring, full, empty, stage, phase, gave_up);
-        copy_tiles<1>(a, maps + 1, L, first1, end1, tiles1, ring, full, empty, stage, phase, gave_up);
+        if (copy_tiles<0>(a, maps, L, first0, end0, tiles0, ring, full, empty, stage, phase, gave_up))
+          copy_tiles<1>(a, maps + 1, L, first1, end1, tiles1, ring, full, empty, stage, phase, gave_up);
       }
-      // after a wait that gave up: let the copies in flight land before the CTA's memory goes
-      if (*gave_up)
-        for (int n = 0; n < 1000; n++) __nanosleep(1000);
       __syncwarp();
     } else {
       const int team = warp / kTeam, part = warp % kTeam;
@@ -601,6 +598,7 @@ struct Layer {
       else
         *y = from_f32<X>(s[0]);
     }
+    if (*gave_up) settle_in_flight();
   }
 
   __device__ static __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kConsumers * 32) : "memory"); }
@@ -630,8 +628,9 @@ struct Layer {
   // Fill the ring with the tiles' rows.  PRODUCT 0: outputs 8 tile + r, their
   // gate rows of w_in in stage rows 0 - 7, their up rows in 8 - 15; 1: rows
   // 16 tile + r of w_out.  Rows past the end are others or zeros (not used).
+  // False after a wait that gave up: a stage still in use takes no copy.
   template <int PRODUCT>
-  __device__ static __forceinline__ void copy_tiles(const LayerArgs& a, const CUtensorMap* map, const Lists& L, int first, int end, int tiles,
+  __device__ static __forceinline__ bool copy_tiles(const LayerArgs& a, const CUtensorMap* map, const Lists& L, int first, int end, int tiles,
                                                     unsigned char* ring, uint32_t full, uint32_t empty, int& stage,
                                                     uint32_t& phase, volatile int* gave_up) {
     const int lane = threadIdx.x & 31;
@@ -646,8 +645,7 @@ struct Layer {
       const int64_t expert = L.unit_expert[u];
       const int row_bytes = a.row_bytes[PRODUCT], row_k = row_bytes / (int)sizeof(W);
       for (int k0 = 0; k0 < k; k0 += row_k) {
-        mbar_wait(empty + 8 * stage, phase ^ 1, gave_up, a.flag);
-        __syncwarp();
+        if (!warp_wait(empty + 8 * stage, phase ^ 1, gave_up, a.flag)) return false;
         unsigned char* dst = ring + stage * kStageBytes;
         if constexpr (COPY == kTensor) {
           if (lane == 0) {
@@ -666,6 +664,7 @@ struct Layer {
         if (++stage == a.stages) stage = 0, phase ^= 1;
       }
     }
+    return true;
   }
 
   // The same for rows that start at any byte: the 16-byte granules that a row

@@ -53,6 +53,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   if (mbar_try(bar, parity)) return true;
   return mbar_wait_slow(bar, parity, gave_up, flag);
 }
+// After a wait that gave up, by every thread of the CTA before its shared
+// memory and TMEM go: a millisecond, in which the copies and matrix instructions
+// in flight end (none is issued after a wait that gave up).
+__device__ __forceinline__ void settle_in_flight() {
+  for (int n = 0; n < 1000; n++) __nanosleep(1000);
+}
 // For a whole warp: all lanes go on, or none.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* gave_up, int* flag) {
   return __all_sync(~0u, mbar_wait(bar, parity, gave_up, flag));

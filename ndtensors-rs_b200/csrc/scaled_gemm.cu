@@ -318,9 +318,6 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, Shape<CTAS, BN>::kR
           if (++stage == S::kStages) stage = 0, phase ^= 1;
         }
       }
-      // after a wait that gave up: let the copies in flight land before the CTA's memory goes
-      if (!ok)
-        for (int i = 0; i < 1000; i++) __nanosleep(1000);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -511,6 +508,7 @@ __global__ void __launch_bounds__(Shape<CTAS, BN>::kThreads, Shape<CTAS, BN>::kR
   // every role is done with this CTA's barriers, TMEM and (pair) the peer's
   fence_before();
   __syncthreads();
+  if (*gave_up) settle_in_flight();
   if (CTAS == 1 && g.ksplit > 1) {
     cluster_sync();
     // each CTA adds its share of the tile over all parts, in rank order; neighbouring threads take neighbours in C
