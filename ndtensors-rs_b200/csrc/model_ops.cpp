@@ -340,7 +340,7 @@ int ndt_b200_expert_layer_dev(int x_type, const void* x, long tokens, long h, lo
     if (!x || !router || !w_in || !w_out || !y || !ids || !weights || (w8 && (!in_scales || !out_scales))) bad("NULL pointer");
     if (ldx < h || ldy < h) bad("a leading dimension is smaller than a row");
     ExpertArgs a{};
-    a.xt = a.rt = xt, a.wt = (MType)w_type;
+    a.xt = xt, a.wt = (MType)w_type;
     a.x = x, a.router = router, a.w_in = w_in, a.w_out = w_out, a.in_scales = in_scales, a.out_scales = out_scales;
     a.tokens = tokens, a.experts = experts, a.top = top, a.h = h, a.i = i, a.ldx = ldx, a.ldy = ldy;
     a.renormalize = renormalize != 0;

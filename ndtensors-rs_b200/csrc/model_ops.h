@@ -21,7 +21,6 @@ namespace ndt {
 // float64 and complex128, which they do not take).
 enum class MType : int { F32 = 2, BF16 = 3, F16 = 4, E4M3 = 5, E5M2 = 6 };
 inline int msize(MType t) { return t == MType::F32 ? 4 : (t == MType::BF16 || t == MType::F16) ? 2 : 1; }
-inline bool is8(MType t) { return t == MType::E4M3 || t == MType::E5M2; }
 
 // A matrix [rows, cols] in device memory; element (r, c) at r * rs + c * cs.
 struct MatView {
@@ -67,7 +66,7 @@ void embedding_grad(MType gt, const void* grad, int64_t ldg, const void* ids, bo
 
 // A mixture-of-experts layer (experts.cu).
 struct ExpertArgs {
-  MType xt, rt, wt;
+  MType xt, wt;        // of x, the router and y; of the experts' weights
   const void* x;       // [tokens, h]
   const void* router;  // [experts, h]
   const void* w_in;    // [experts, 2 i, h]
