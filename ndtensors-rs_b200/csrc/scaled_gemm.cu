@@ -619,8 +619,10 @@ void scaled_gemm(const ScaledOperand& a_, const ScaledOperand& b_, int64_t k, MT
            (uint32_t)(n / 8) << 17 | (uint32_t)(m / 16) << 24;
   };
   // Waves of 128 x 128 tiles against waves of 256 x 256 pairs, which take 5 / 4
-  // of the time (k 2048: 1024 x 2048 15.2 us in one wave of tiles, 16.9 of
-  // pairs; 1024 x 2560 25.1 in two of tiles, 17.7 in one of pairs).
+  // of the time.  us of tiles and of pairs, k 512 / 2048 / 8192: 1024 x 2048 12.3,
+  // 14.3 / 18.4, 20.5 / 38.9, 45.1 (one wave of each); 1024 x 2560 18.4, 16.4 /
+  // 28.7, 22.5 / 69.6, 47.1 (two of tiles, one of pairs); 2048 x 3000 26.6, 24.6 /
+  // 41.0, 36.9 / 102.4, 86.0; 4096 x 4096 49.2, 30.7 / 86.0, 57.3 / 229.4, 153.6.
   const int64_t pair_tiles = (int64_t)cdiv(g.m, 256) * cdiv(g.n, 256);
   const int64_t waves = ((int64_t)cdiv(g.m, 128) * cdiv(g.n, 128) + sms - 1) / sms, pair_waves = (pair_tiles + sms / 2 - 1) / (sms / 2);
   if (!swap && 5 * pair_waves < 4 * waves) {
@@ -636,11 +638,14 @@ void scaled_gemm(const ScaledOperand& a_, const ScaledOperand& b_, int64_t k, MT
   const int bn = !swap ? 128 : g.n <= 16 ? 16 : g.n <= 32 ? 32 : 64;
   g.tiles_m = cdiv(g.m, 128), g.tiles_n = cdiv(g.n, bn);
   g.idesc = idesc(128, bn);
-  // k is split while the CTAs fit the GPU at once and keep enough blocks each:
-  // adding the parts of a 128 x 128 tile costs what 16 blocks do (train step of
-  // 1000 tokens: 29 us for 7 blocks a CTA, 16 us unsplit with 9), of few columns less
+  // k is split while the CTAs fit the GPU at once and keep enough blocks each.
+  // 128 x 128 tiles are costly to add: 128 x 2048 with k 8192 / 16384 / 32768
+  // takes 36.9 / 61.4 / 114.6 us unsplit, 36.9 / 51.2 / 69.6 with 64 blocks or
+  // more a CTA, 49.2 / 127 / 148 with 16.  Of few rows it costs little (k 8192, one
+  // row against 1024 / 10240: 32.8 / 34.8 us unsplit, 16.4 / 28.7 with 4 or more;
+  // 16 rows, 8192 x 1024: 12.4 and 14.3).
   const int room = sms * (swap ? 2 : 1), tiles = g.tiles_m * g.tiles_n;
-  g.ksplit = std::max(1, std::min({8, room / tiles, g.kblocks / (swap ? 4 : 16)}));
+  g.ksplit = std::max(1, std::min({8, room / tiles, g.kblocks / (swap ? 4 : 64)}));
   const int grid = tiles * g.ksplit;
   if (!swap)
     b.per_row ? launch<1, 128, true>(a, b, k, g, grid, g.ksplit, s) : launch<1, 128, false>(a, b, k, g, grid, g.ksplit, s);

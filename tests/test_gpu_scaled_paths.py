@@ -31,7 +31,7 @@ def check(c, a, b, base=None):
 
 #: CTA pairs over two waves of tiles and several rounds of the ring; one CTA a
 #: tile; k split over a cluster with many rows and with few
-SIZES = [(2100, 2304, 2056), (2100, 2304, 4100), (1000, 700, 1300), (300, 520, 8200), (130, 140, 33000), (65, 129, 4096),
+SIZES = [(2100, 2304, 2056), (2100, 2304, 4100), (1000, 700, 1300), (300, 520, 8200), (130, 140, 33000), (300, 520, 16500), (65, 129, 4096),
          (40, 300, 4100), (17, 1000, 8200), (3, 5000, 2049)]
 
 
@@ -47,7 +47,8 @@ def test_product(gpu, m, n, k, ra, rb):
     assert torch.equal(gpu.scaled_gemm(a, sa, b, sb, out_dtype=torch.float32), first[torch.float32])
 
 
-@pytest.mark.parametrize("m,n,k", [(2100, 2304, 2056), (300, 520, 8200), (40, 300, 4100), (1000, 701, 1300)])
+@pytest.mark.parametrize("m,n,k", [(2100, 2304, 2056), (300, 520, 8200), (300, 520, 16500), (130, 139, 33000), (40, 300, 4100),
+                                   (1000, 701, 1300)])
 @pytest.mark.parametrize("dtype", REAL)
 def test_accumulates_into_wider_rows(gpu, m, n, k, dtype):
     a, sa, da = operand(30, m, k, 1, spread=0.5)
@@ -60,14 +61,14 @@ def test_accumulates_into_wider_rows(gpu, m, n, k, dtype):
 
 
 @pytest.mark.parametrize("ta,tb", [(E5, E4), (E4, E5)])
-@pytest.mark.parametrize("m,n,k", [(2100, 2304, 2056), (300, 520, 8200), (20, 300, 8200)])
+@pytest.mark.parametrize("m,n,k", [(2100, 2304, 2056), (300, 520, 8200), (300, 520, 16500), (20, 300, 8200)])
 def test_types(gpu, ta, tb, m, n, k):
     a, sa, da = operand(50, m, k, 1, ta)
     b, sb, db = operand(60, n, k, 1, tb)
     check(gpu.scaled_gemm(a, sa, b, sb, out_dtype=torch.float32), da, db)
 
 
-@pytest.mark.parametrize("tokens,n,k", [(8300, 200, 300), (4097, 129, 2500)])
+@pytest.mark.parametrize("tokens,n,k", [(8300, 200, 300), (4097, 129, 2500), (17000, 200, 140)])
 def test_gradients_of_many_tokens(gpu, tokens, n, k):
     """The weights' gradient sums over many tokens for few outputs: its k is split."""
     x, w = normal(gen(2), tokens, k).requires_grad_(), (normal(gen(3), n, k) * k ** -0.5).requires_grad_()
