@@ -993,8 +993,12 @@ template <typename W, typename X, typename M, int COPY, int NT>
 void launch(LayerArgs& a, int64_t row, cudaStream_t s) {
   auto kern = layer_kernel<W, X, M, COPY, NT>;
   // as many tokens as fit beside kKeep of stages (at least one, beside two stages), and stages for the rest.
-  // 16-bit weights: 8 up to i 2688 and h 5376, 6 for 7168 / 2048, 3 for i 6400, 1 for i 14336.
-  const int space = room(NT), kStageBytes = stage_bytes(COPY), kKeep = (COPY == kShift ? 132 : 100) * 1024;
+  // 16-bit weights: 8 up to i 3712 and h 7424, 4 for i 6400, 2 for i 14336.  us with 100 KB kept / 66 (two
+  // stages of row copies, four of tensor copies): 64 tokens, 2 of 16, 7168 / 2048 519 / 440, 2880 / 2880 282 /
+  // 264; 2 of 8, 4096 / 6400 1398 / 1154, 4096 / 14336 7990 / 4790; 8 tokens, 8 of 64, 2048 / 1024 128 / 130.
+  // Rows at any byte want two slots beside two stages (132 KB; 100 / 132 / 166: 64 tokens, 2 of 16, 4095 / 2047
+  // 939 / 730 / 1664; 4 of 64, 2049 / 641 411 / 411 / 546).
+  const int space = room(NT), kStageBytes = stage_bytes(COPY), kKeep = (COPY == kShift ? 132 : 66) * 1024;
   if (row > space - 8192 - 2 * kStageBytes - (COPY == kShift ? kRawBytes : 0)) throw Error(ErrKind::InvalidArgument, "h or i is too large for a token's row to fit shared memory");
   a.unit = (int)std::max<int64_t>(1, std::min<int64_t>({NT * 8, a.tokens, (space - kKeep - (sizeof(W) == 1 ? 8192 : 0)) / row}));
   a.op_bytes = (int)(a.unit * row);
@@ -1057,7 +1061,9 @@ void expert_layer(const ExpertArgs& e, cudaStream_t s) {
     a.xpitch = (a.h + 127) / 128 * 256 + pad, a.bpitch = (a.i + 127) / 128 * 256 + pad;
     const int64_t row = std::max((int64_t)a.xpitch, 2 * (int64_t)a.bpitch);
     // An expert's second unit of tokens reads its weights again (from L2): more
-    // columns where an expert gets more than 6 tokens on average and 16 fit.
+    // columns where an expert gets more than 6 tokens on average and 16 fit.  us of
+    // 8 / 16 columns, 512 / 256 with 8 experts: 6 tokens each 23.8 / 23.8, 16 each
+    // 30.0 / 30.6, 32 each 38.1 / 36.1; 768 / 384 with 64 each 110 / 89.
     const bool many = a.tokens * e.top > 6 * e.experts && a.tokens > 8 && 16 * row <= room(2) - 140 * 1024;
     auto go = [&](auto w, auto x, auto m) {
       using W = decltype(w);

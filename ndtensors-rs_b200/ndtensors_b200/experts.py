@@ -30,9 +30,9 @@ def expert_layer(x, router, w_in, w_out, top: int, in_scales=None, out_scales=No
     [..., top].  They carry no gradient, so inputs that require one are refused
     unless gradients are off.  Made for at most about a hundred tokens (a decoding batch);
     more are right, but an expert's weights are read anew for each group of its
-    tokens: 8 (or 16) where their rows are short, and as many as fit 85 KB of
-    shared memory at max(2 h, 4 i) bytes each where they are long (6 for h 7168,
-    i 2048; 3 for i 6400; 1 for i 14336; fewer for 8-bit weights or odd lengths).
+    tokens: 8 (or 16) where their rows are short, and as many as fit 119 KB of
+    shared memory at max(2 h, 4 i) bytes each where they are long (8 up to h 7424
+    and i 3712, 4 for i 6400, 2 for i 14336; fewer for 8-bit weights or odd lengths).
     """
     device = device_of("expert_layer", x, router, w_in, w_out, in_scales, out_scales)
     no_gradient("expert_layer", "call it under torch.no_grad()", x, router, w_in, w_out, in_scales, out_scales)
