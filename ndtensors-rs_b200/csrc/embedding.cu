@@ -17,7 +17,7 @@
 //
 // Measured on one B200 (16384 ids by frequency, 65536 x 2048 bf16, us under the
 // profiler): lookup 15, sort with 180 MB of zeros to DRAM 45, sum 17 for 67 MB,
-// join 13; the step 92, 5.1 TB/s of what it has to move.  Eight rows of grad in
+// join 13; the step 94, 5.0 TB/s of what it has to move.  Eight rows of grad in
 // flight a thread made the sum 50 -> 26, and chains added by groups of threads
 // the join 193 -> 29.
 #include <algorithm>

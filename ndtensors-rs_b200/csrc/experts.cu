@@ -35,7 +35,7 @@
 // Measured on one B200: 1 token, 8 of 64 experts, h 2048, i 1024, bf16 39 us
 // (router 1.4, choice 5, products 10 and 6, barriers 6, the rest the launch); 8
 // tokens of it 114 - 118 us, 4.6 TB/s; 64 tokens, 4 of 64, h 4096, i 1280, 8-bit
-// 322 - 356 us, 2.9 TB/s, where the short rows of w_out make each tile mostly
+// 319 - 324 us, 3.1 TB/s, where the short rows of w_out make each tile mostly
 // barriers.
 //
 // All sums are in 32 bits.  The activations b enter the second product as the

@@ -21,15 +21,19 @@
 // lanes and A's few the columns.  CTAS = 2: a CTA pair computes 256 x 256 with
 // cta_group::2 MMAs, each CTA staging its half of both operands; persistent.
 //
-// Measured on one B200 (1 x 128 by 128 x 128 scales, bf16 result): 4096^3 86 us
-// = 1600 TFLOP/s, 8192^3 537 us = 2050; with a scale for each row of both
-// 4096^3 125 us.  The tensor pipe is busy 45 % of the time.  With a quarter of
-// the MMAs 8192^3 still takes 463 us, with half the TMEM reads too 434: the
-// bound is the operand tiles' way from L2 to the SMs, 32 KB for each SM and
-// block of k (9.8 TB/s).  One row against 10240 x 8192 weights: 19 us, 4.5 TB/s.
+// Measured on one B200 (1 x 128 by 128 x 128 scales, bf16 result, L2 flushed):
+// 4096^3 90 us = 1530 TFLOP/s, 8192^3 522 us = 2110; with a scale for each row of
+// both 135 and 809 us.  Copies of the kernel, 4096^3 / 8192^3 in us: loads alone
+// (a quarter of the MMAs, no TMEM reads) 61 / 318, loads and all MMAs 76 / 424,
+// all 90 / 522, all but the loads (stages filled once) 90 / 502.  So the bound is
+// not L2 but the way of a block's sums: MMAs, reads from TMEM, scales, the buffer
+// given back, with two buffers to overlap them; a scale for each column as well
+// is one more multiplication there for two values.  The tensor pipe is busy 45 %
+// of the time.  One row against 10240 x 8192 weights: 19 us, 4.5 TB/s.
 //
 // sa * sb is formed in 32 bits: it stays finite while the product of two
-// blocks' largest values is below 2^127.
+// blocks' largest values is below 2^127, and has all its bits while that product
+// is above 2^-108.
 #include <algorithm>
 
 #include "mbarrier.h"
