@@ -6,6 +6,8 @@ package binds its C ABI with ctypes and mirrors the reference's Python API
 block-sparse tensors and whole-network contraction (contract_network).
 """
 
+from importlib.util import find_spec
+
 from . import blocksparse
 from ._lib import get_lib, last_error, lib_path
 from .network import contract_network
@@ -80,5 +82,5 @@ __all__ = [
     "synchronize",
     "launch_count",
     "set_stream",
-    *_TORCH_NAMES,
+    *(_TORCH_NAMES if find_spec("torch") else ()),  # (import * fetches every name)
 ]
